@@ -7,7 +7,7 @@ Drop-in for the reference's plugin surface (thromel/Image-Captioning-ML-Project)
 """
 import torch
 
-from . import _lib, ops  # noqa: F401
+from . import _lib, context, ops  # noqa: F401
 from .models.common import set_precision
 from .params import attach
 

@@ -170,6 +170,27 @@ SIGNATURES = {
     "capk_attn_coverage_reg": (_i, [_i, _i, _i, _c_p, _c_p, _c_p, _c_p, _c_p]),
     "capk_clamp": (_i, [_i64, _c_p, _f, _f, _c_p]),
     "capk_mask_rows_by_length": (_i, [_i, _i, _i, _i, _c_p, _i64, _i64, _c_p, _c_p]),
+    "capk_axis_rope": (_i, [_i, _i, _i, _i, _i, _i, _i, _i, _c_p, _i64, _i64, _c_p, _c_p, _i, _c_p, _i64, _i64, _i64,
+                            _c_p, _i64, _i64, _i64, _i, _c_p, _i64, _i64, _i64, _c_p, _i64, _i64, _i64, _c_p]),
+    "capk_sliding_attention_fwd_workspace": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i, _i]),
+    "capk_sliding_attention_fwd": (_i, [_i, _i, _i, _i, _i, _i, _i, _f, _i, _i, _c_p, _i64, _i64, _i64, _c_p, _i64,
+                                        _i64, _i64, _c_p, _i64, _i64, _i64, _c_p, _c_p, _c_p, _i64, _i64, _i64, _c_p,
+                                        _c_p, _sz, _c_p]),
+    "capk_sliding_attention_bwd_workspace": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i]),
+    "capk_sliding_attention_bwd": (_i, [_i, _i, _i, _i, _i, _i, _i, _f, _i, _i, _c_p, _i64, _i64, _i64, _c_p, _i64,
+                                        _i64, _i64, _c_p, _i64, _i64, _i64, _c_p, _c_p, _c_p, _i64, _i64, _i64, _c_p,
+                                        _i64, _i64, _i64, _c_p, _c_p, _i64, _i64, _i64, _c_p, _i64, _i64, _i64, _c_p,
+                                        _i64, _i64, _i64, _c_p, _sz, _c_p]),
+    "capk_kv4_append": (_i, [_i, _i, _i, _i, _i, _c_p, _i64, _i64, _i64, _c_p, _i64, _i64, _i64, _c_p, _c_p, _i, _i,
+                             _c_p, _i64, _i, _c_p, _c_p, _c_p]),
+    "capk_kv4_read": (_i, [_i, _i, _i, _i, _i, _c_p, _c_p, _i, _i, _c_p, _i64, _i, _c_p, _c_p, _i64, _i64, _i64, _c_p,
+                           _i64, _i64, _i64, _c_p]),
+    "capk_kv4_attention_workspace": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i, _i, _i]),
+    "capk_kv4_attention": (_i, [_i, _i, _i, _i, _i, _i, _f, _i, _i, _c_p, _i64, _i64, _i64, _c_p, _c_p, _i, _i, _c_p,
+                                _i64, _i, _c_p, _c_p, _i64, _i64, _i64, _c_p, _c_p, _sz, _c_p]),
+    "capk_verify_drafts_workspace": (_sz, [_i, _i, _i]),
+    "capk_verify_drafts": (_i, [_i, _i, _i, _i, _c_p, _i64, _i64, _c_p, _i64, _i64, _c_p, _i64, _c_p, _i64, _c_p,
+                                ctypes.c_double, _c_p, _c_p, _i64, _c_p, _sz, _c_p]),
     "capk_cider_d": (_i, [_i, _c_p, _c_p, _c_p, _c_p, _c_p, _i, ctypes.c_double, _i, _c_p]),
 }
 

@@ -1,0 +1,131 @@
+"""Operators of long-context decoding on libcapk kernels, differentiable where training needs them.
+
+    freq, axis = axis_frequencies((8, 12, 12))              # pairs for time, height, width
+    q, k = axis_rope(q, k, pos, freq, axis)                 # [B, N, heads, hd], pos [3, B, N]
+    o = sliding_attention(q, k, v, window=1024, sinks=4)    # training, prefill, a decoding step
+    cache = KV4Cache.empty(pages, heads, head_dim)          # 4.25 bits per element, paged
+    cache.append(k, v, table, start)
+    o = cache.attend(q, table, kv_len, window=1024, sinks=4)
+    accepted, tokens = verify_drafts(target, ids, u, draft)
+
+The tensor-level wrappers are capk.ops.axis_rope, sliding_attention_fwd / _bwd, kv4_* and verify_drafts;
+layouts and rules are those of include/capk.h.
+"""
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import ops
+from .ops import verify_drafts  # noqa: F401
+
+
+def axis_frequencies(sections, theta=10000.0, device="cuda"):
+    """(freq fp64 [pairs], axis uint8 [pairs]): sections[a] pairs follow axis a, each axis on its own ladder
+    theta^(-i / sections[a]).  Any other assignment of frequencies and axes to pairs works as well."""
+    if not sections or any(int(n) < 0 for n in sections) or not sum(sections):
+        raise ValueError(f"axis_frequencies: sections {sections!r}")
+    freq = [theta ** (-i / n) for n in sections for i in range(n)]
+    axis = [a for a, n in enumerate(sections) for _ in range(n)]
+    return (torch.tensor(freq, dtype=torch.float64, device=device), torch.tensor(axis, dtype=torch.uint8, device=device))
+
+
+def _rows(t):
+    """`t` itself where its rows start 16-B aligned with unit element stride, else a contiguous copy."""
+    if t is None or t.dim() != 4:
+        return t
+    n = 16 // t.element_size()
+    ok = t.data_ptr() % 16 == 0 and (t.stride(3) == 1 or t.shape[3] == 1)
+    ok = ok and all(s % n == 0 or d == 1 for s, d in zip(t.stride()[:3], t.shape[:3]))
+    return t if ok else t.contiguous()
+
+
+def _unit(t):
+    return t if t is None or t.dim() != 4 or t.stride(3) == 1 else t.contiguous()
+
+
+class _AxisRope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, pos, freq, axis, interleaved):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(pos, freq, axis)
+        ctx.interleaved = interleaved
+        return ops.axis_rope(_unit(q), _unit(k), pos, freq, axis, interleaved=interleaved)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gq, gk):
+        pos, freq, axis = ctx.saved_tensors
+        kw = dict(interleaved=ctx.interleaved, inverse=True)
+        if gq is None:
+            dq, dk = None, None if gk is None else ops.axis_rope(_unit(gk), None, pos, freq, axis, **kw)[0]
+        else:
+            dq, dk = ops.axis_rope(_unit(gq), _unit(gk), pos, freq, axis, **kw)
+        return dq, dk, None, None, None, None
+
+
+def axis_rope(q, k, pos, freq, axis, *, interleaved=False):
+    """(q', k') turned by their positions (ops.axis_rope); k may be None.  Differentiable in q and k."""
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _AxisRope.apply(q, k, pos, freq, axis, interleaved)
+    return ops.axis_rope(_unit(q), _unit(k), pos, freq, axis, interleaved=interleaved)
+
+
+class _SlidingAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, window, sinks, scale, key_pad, kv_len):
+        q, k, v = _rows(q), _rows(k), _rows(v)
+        o, lse = ops.sliding_attention_fwd(q, k, v, window, sinks, scale, key_pad, kv_len)
+        ctx.save_for_backward(q, k, v, o, lse, key_pad, kv_len)
+        ctx.rule = (window, sinks, scale)
+        return o
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do):
+        q, k, v, o, lse, key_pad, kv_len = ctx.saved_tensors
+        dq, dk, dv = ops.sliding_attention_bwd(q, k, v, o, _rows(do), lse, *ctx.rule, key_pad, kv_len)
+        return dq, dk, dv, None, None, None, None, None
+
+
+def sliding_attention(q, k, v, *, window=0, sinks=0, scale=None, key_pad=None, kv_len=None):
+    """o [B, Nq, H, hd]: the queries are the last Nq positions of kv_len[b] (default Nk) keys; position p sees
+    j <= p with j < sinks or p - j < window (0: no window), less key_pad[b, j].  k / v [B, Nk, Hk, hd] with
+    H % Hk == 0; scale defaults to hd ** -0.5.  Differentiable in q, k and v."""
+    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    if q.dim() == 4 and k.dim() == 4 and not (q.numel() and k.numel()):  # nothing to attend, or to
+        if q.dtype != k.dtype or q.dtype != v.dtype or k.shape != v.shape or q.shape[0] != k.shape[0]:
+            raise ValueError(f"sliding_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+        return q * 0
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _SlidingAttention.apply(q, k, v, window, sinks, scale, key_pad, kv_len)
+    return ops.sliding_attention_fwd(_rows(q), _rows(k), _rows(v), window, sinks, scale, key_pad, kv_len,
+                                     want_lse=False)[0]
+
+
+class KV4Cache:
+    """Pages of keys and values in 4 bits: codes [pages, 2, heads, page, hd/2] and scales [pages, 2, heads, page,
+    hd/32] (uint8).  The caller keeps the page tables (int [B, pages of a sequence]) and lengths, as one table
+    serves every layer's cache; a page may stand in several tables (shared prefixes, beams)."""
+
+    def __init__(self, codes, scales):
+        self.codes, self.scales = codes, scales
+
+    @classmethod
+    def empty(cls, pages, heads, head_dim, page=64, device="cuda"):
+        if head_dim % 32 or not 32 <= head_dim <= 128 or page % 16 or page < 16 or pages < 1 or heads < 1:
+            raise ValueError(f"KV4Cache: {pages} pages of {page} tokens, {heads} heads x {head_dim}: need head_dim "
+                             "32, 64, 96 or 128 and pages of a multiple of 16 tokens")
+        return cls(torch.zeros(pages, 2, heads, page, head_dim // 2, dtype=torch.uint8, device=device),
+                   torch.full((pages, 2, heads, page, head_dim // 32), 127, dtype=torch.uint8, device=device))
+
+    def append(self, k, v, table, start, count=None):
+        """k, v [B, n, heads, hd] become tokens start[b] + i (i < count[b]); tokens without a page are dropped."""
+        ops.kv4_append(_rows(k), _rows(v), self.codes, self.scales, table, start, count)
+
+    def read(self, table, start, n, dtype=torch.bfloat16):
+        """(k, v) [B, n, heads, hd] of tokens start[b] + i: the values the cache stands for."""
+        return ops.kv4_read(self.codes, self.scales, table, start, n, dtype)
+
+    def attend(self, q, table, kv_len, *, window=0, sinks=0, scale=None):
+        """o [B, Nq, H, hd] of the last Nq <= 64 tokens of kv_len[b], visible as in sliding_attention."""
+        scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+        return ops.kv4_attention(_rows(q), self.codes, self.scales, table, kv_len, window, sinks, scale)

@@ -1257,3 +1257,221 @@ def mask_rows_by_length(x, lengths_i32):
     check(lib().capk_mask_rows_by_length(dtype_code(x), B, T, C, _p(x), x.stride(1), x.stride(0), _p(lengths_i32),
                                          _stream()), "capk_mask_rows_by_length")
     return x
+
+
+# ------------------------------------------------- long-context decoding ---
+def _launch(dev, name, *args):
+    """Call an entry point on `dev`'s current stream (its arguments end with the stream)."""
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return _launch(dev, name, *args)
+    check(getattr(lib(), name)(*args, torch.cuda.current_stream().cuda_stream), name)
+
+
+def _same(what, first, *rest, dtype=True):
+    """All tensors on `first`'s GPU and, with dtype, of its type."""
+    _need_gpu(first)
+    for t in rest:
+        if t is None:
+            continue
+        if t.device != first.device:
+            raise _lib.CapkError(f"{what}: tensors on {first.device} and {t.device}")
+        if dtype and t.dtype != first.dtype:
+            raise _lib.CapkError(f"{what}: {first.dtype} and {t.dtype}")
+
+
+def _index(what, t, shape, dtype, dev):
+    """`t` as a contiguous index / flag tensor of `dtype`, after checks of shape, kind and device."""
+    if t is None:
+        return None
+    if t.device != dev:
+        raise _lib.CapkError(f"{what} on {t.device}, the operands on {dev}")
+    if tuple(t.shape) != tuple(shape) or t.dtype.is_floating_point or t.dtype.is_complex:
+        raise ValueError(f"{what}: need integers of shape {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    return t.to(dtype).contiguous()
+
+
+def _view4(what, t):
+    """(pointer, batch, token and head stride) of a [B, N, H, hd] view with unit element stride."""
+    if t.dim() != 4 or (t.stride(3) != 1 and t.shape[3] > 1):
+        raise ValueError(f"{what}: need [batch, tokens, heads, head_dim] with unit stride in the last, got "
+                         f"{tuple(t.shape)} / {t.stride()}")
+    (nb, nn, nh, _), s = t.shape, t.stride()  # (a dimension of one has no stride to speak of)
+    return t.data_ptr(), s[0] if nb > 1 else 0, s[1] if nn > 1 else 0, s[2] if nh > 1 else 0
+
+
+def axis_rope(q, k, pos, freq, axis, *, interleaved=False, inverse=False, out_q=None, out_k=None):
+    """Rotary positions over several axes (capk_axis_rope) of q [B, N, H, hd] and k [B, N, Hk, hd] (or
+    None); pos int [axes, B, N] or [axes, N], freq fp64 [pairs], axis [pairs].  out_q / out_k may be q / k."""
+    what = "axis_rope"
+    out_q = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out_q is None else out_q
+    if k is not None and out_k is None:
+        out_k = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    _same(what, q, k, out_q, out_k)
+    code = dtype_code(q)
+    qv, qov = _view4(what, q), _view4(what, out_q)
+    B, N, H, hd = q.shape
+    if out_q.shape != q.shape or (k is not None and (k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != hd
+                                                     or out_k.shape != k.shape)):
+        raise ValueError(f"axis_rope: q {tuple(q.shape)}, k {None if k is None else tuple(k.shape)} and the outputs differ")
+    if pos.dim() not in (2, 3) or tuple(pos.shape[1:]) not in ((B, N), (N,)) or not pos.shape[0]:
+        raise ValueError(f"axis_rope: positions [axes, {B}, {N}] or [axes, {N}], got {tuple(pos.shape)}")
+    pairs = freq.shape[0]
+    pos = _index("axis_rope: positions", pos, pos.shape, torch.int32, q.device)
+    axis = _index("axis_rope: axis", axis, (pairs,), torch.uint8, q.device)
+    if freq.dtype != torch.float64 or freq.dim() != 1 or freq.device != q.device:
+        raise ValueError("axis_rope: frequencies must be fp64 [pairs] on the operands' device")
+    freq = freq.contiguous()
+    kv, kov = (_view4(what, k), _view4(what, out_k)) if k is not None else ((None, 0, 0, 0), (None, 0, 0, 0))
+    _launch(q.device, "capk_axis_rope", code, B, N, hd, pairs, int(interleaved), int(inverse), pos.shape[0],
+            pos.data_ptr(), pos.stride(0), pos.stride(1) if pos.dim() == 3 else 0, freq.data_ptr(), axis.data_ptr(),
+            H, *qv, *qov, 0 if k is None else k.shape[2], *kv, *kov)
+    return out_q, out_k
+
+
+def _sliding_args(what, q, k, v, window, sinks, key_pad, kv_len):
+    _same(what, q, k, v)
+    code = dtype_code(q)
+    views = _view4(what, q) + _view4(what, k) + _view4(what, v)
+    B, Nq, H, hd = q.shape
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != hd:
+        raise ValueError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+    Nk, Hk = k.shape[1], k.shape[2]
+    key_pad = _index(f"{what}: key_pad", key_pad, (B, Nk), torch.uint8, q.device)
+    kv_len = _index(f"{what}: kv_len", kv_len, (B,), torch.int32, q.device)
+    return code, (B, H, Hk, Nq, Nk, hd), (int(window), int(sinks)), views, key_pad, kv_len
+
+
+def sliding_attention_fwd(q, k, v, window, sinks, scale, key_pad=None, kv_len=None, *, out=None, want_lse=True):
+    """(o, lse fp32 [B, H, Nq]) of capk_sliding_attention_fwd; q [B, Nq, H, hd], k / v [B, Nk, Hk, hd]."""
+    what = "sliding_attention_fwd"
+    code, dims, ws_args, views, key_pad, kv_len = _sliding_args(what, q, k, v, window, sinks, key_pad, kv_len)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _same(what, q, out)
+    if out.shape != q.shape:
+        raise ValueError(f"{what}: out {tuple(out.shape)} for q {tuple(q.shape)}")
+    lse = torch.empty(q.shape[0], q.shape[2], q.shape[1], dtype=torch.float32, device=q.device) if want_lse else None
+    wsb = lib().capk_sliding_attention_fwd_workspace(code, *dims, *ws_args)
+    ws = _ws(wsb, q.device)
+    _launch(q.device, "capk_sliding_attention_fwd", code, *dims, float(scale), *ws_args, *views, _p(key_pad), _p(kv_len),
+            *_view4(what, out), _p(lse), _p(ws), wsb)
+    return out, lse
+
+
+def sliding_attention_bwd(q, k, v, o, do, lse, window, sinks, scale, key_pad=None, kv_len=None):
+    """(dq, dk, dv) of capk_sliding_attention_bwd from the forward's o and lse."""
+    what = "sliding_attention_bwd"
+    code, dims, ws_args, views, key_pad, kv_len = _sliding_args(what, q, k, v, window, sinks, key_pad, kv_len)
+    _same(what, q, o, do)
+    _same(what, q, lse, dtype=False)
+    if o.shape != q.shape or do.shape != q.shape or lse.dtype != torch.float32 or not lse.is_contiguous() or \
+            tuple(lse.shape) != (q.shape[0], q.shape[2], q.shape[1]):
+        raise ValueError(f"{what}: o, do like q and a contiguous fp32 lse [B, H, Nq]")
+    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    wsb = lib().capk_sliding_attention_bwd_workspace(*dims, *ws_args)
+    ws = _ws(wsb, q.device)
+    _launch(q.device, "capk_sliding_attention_bwd", code, *dims, float(scale), *ws_args, *views, _p(key_pad), _p(kv_len),
+            *_view4(what, o), *_view4(what, do), _p(lse), *_view4(what, dq), *_view4(what, dk), *_view4(what, dv),
+            _p(ws), wsb)
+    return dq, dk, dv
+
+
+def _kv4_pages(what, codes, scales, table, B, dev):
+    """(pages, Hk, page, hd, the page-table arguments, the table kept alive) after checks of the cache's layout."""
+    if codes.device != dev or scales.device != dev:
+        raise _lib.CapkError(f"{what}: pages on {codes.device} / {scales.device}, the operands on {dev}")
+    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.dim() != 5 or scales.dim() != 5 or \
+            codes.shape[1] != 2 or codes.shape[:4] != scales.shape[:4] or codes.shape[4] != 16 * scales.shape[4] or \
+            not codes.is_contiguous() or not scales.is_contiguous():
+        raise ValueError(f"{what}: need contiguous uint8 codes [pages, 2, heads, page, hd/2] and scales [..., hd/32], "
+                         f"got {tuple(codes.shape)} and {tuple(scales.shape)}")
+    if table.dim() != 2 or table.shape[0] != B or not table.shape[1]:
+        raise ValueError(f"{what}: page table [{B}, pages of a sequence], got {tuple(table.shape)}")
+    table = _index(f"{what}: page table", table, table.shape, torch.int32, dev)
+    pages, _, Hk, page, half = codes.shape
+    return pages, Hk, page, 2 * half, (table.data_ptr(), table.stride(0), table.shape[1]), table
+
+
+def kv4_append(k, v, codes, scales, table, start, count=None):
+    """Write k, v [B, n, Hk, hd] as tokens start[b] + i (i < count[b]) of a 4-bit paged cache (capk_kv4_append)."""
+    what = "kv4_append"
+    _same(what, k, v)
+    kv, vv, code = _view4(what, k), _view4(what, v), dtype_code(k)
+    B, n, Hk, hd = k.shape
+    pages, ph, page, pd, targs, table = _kv4_pages(what, codes, scales, table, B, k.device)
+    if v.shape != k.shape or (ph, pd) != (Hk, hd):
+        raise ValueError(f"{what}: k {tuple(k.shape)}, v {tuple(v.shape)} for pages of {ph} heads x {pd}")
+    start = _index(f"{what}: start", start, (B,), torch.int32, k.device)
+    count = _index(f"{what}: count", count, (B,), torch.int32, k.device)
+    _launch(k.device, "capk_kv4_append", code, B, n, Hk, hd, *kv, *vv, codes.data_ptr(), scales.data_ptr(), pages, page,
+            *targs, _p(start), _p(count))
+
+
+def kv4_read(codes, scales, table, start, n, dtype):
+    """(k, v) [B, n, Hk, hd]: what tokens start[b] + i of the cache stand for (capk_kv4_read)."""
+    what = "kv4_read"
+    _need_gpu(codes)
+    dev, B = codes.device, table.shape[0]
+    if dtype not in _DT:
+        raise _lib.CapkError(f"capk: unsupported dtype {dtype}")
+    pages, Hk, page, hd, targs, table = _kv4_pages(what, codes, scales, table, B, dev)
+    start = _index(f"{what}: start", start, (B,), torch.int32, dev)
+    if n < 0:
+        raise ValueError(f"{what}: n = {n}")
+    k, v = (torch.empty(B, n, Hk, hd, dtype=dtype, device=dev) for _ in "kv")
+    _launch(dev, "capk_kv4_read", _DT[dtype], B, n, Hk, hd, codes.data_ptr(), scales.data_ptr(), pages, page, *targs,
+            _p(start), *_view4(what, k), *_view4(what, v))
+    return k, v
+
+
+def kv4_attention(q, codes, scales, table, kv_len, window, sinks, scale, *, lse=None):
+    """o [B, Nq, H, hd]: attention of the last Nq <= 64 tokens over the 4-bit cache (capk_kv4_attention)."""
+    what = "kv4_attention"
+    _need_gpu(q)
+    qv, code = _view4(what, q), dtype_code(q)
+    B, Nq, H, hd = q.shape
+    pages, Hk, page, pd, targs, table = _kv4_pages(what, codes, scales, table, B, q.device)
+    if pd != hd:
+        raise ValueError(f"{what}: heads of {hd} over pages of {pd}")
+    if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (B, H, Nq) or not lse.is_contiguous() or
+                            lse.device != q.device):
+        raise ValueError(f"{what}: lse must be contiguous fp32 [B, H, Nq]")
+    kv_len = _index(f"{what}: kv_len", kv_len, (B,), torch.int32, q.device)
+    if kv_len is None:
+        raise ValueError(f"{what}: kv_len is needed")
+    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    wsb = lib().capk_kv4_attention_workspace(code, B, H, Hk, Nq, hd, int(window), int(sinks), page, table.shape[1])
+    ws = _ws(wsb, q.device)
+    _launch(q.device, "capk_kv4_attention", code, B, H, Hk, Nq, hd, float(scale), int(window), int(sinks), *qv,
+            codes.data_ptr(), scales.data_ptr(), pages, page, *targs, _p(kv_len), *_view4(what, o), _p(lse), _p(ws), wsb)
+    return o
+
+
+def verify_drafts(target, ids, u, draft=None, *, draft_len=None, temperature=1.0, vocab_size=None):
+    """(accepted int32 [B], tokens int64 [B, K+1]) of capk_verify_drafts: target logits [B, K+1, >= V], drafted ids
+    [B, K], uniforms u fp32 [B, K+1], draft logits [B, K, >= V] or None (drafts without probabilities)."""
+    what = "verify_drafts"
+    _same(what, target, draft)
+    code, dev = dtype_code(target), target.device
+    if target.dim() != 3 or not target.shape[1]:
+        raise ValueError(f"{what}: target logits [B, K + 1, V], got {tuple(target.shape)}")
+    B, K, V = target.shape[0], target.shape[1] - 1, target.shape[2] if vocab_size is None else int(vocab_size)
+    for t, n in ((target, K + 1), (draft, K)):
+        if t is not None and (t.dim() != 3 or tuple(t.shape[:2]) != (B, n) or not 1 <= V <= t.shape[2] or
+                              (t.stride(2) != 1 and t.shape[2] > 1)):
+            raise ValueError(f"{what}: logits [{B}, {n}, >= {V}] with unit stride in the last, got {tuple(t.shape)}")
+    ids = _index(f"{what}: ids", ids, (B, K), torch.int64, dev)
+    draft_len = _index(f"{what}: draft_len", draft_len, (B,), torch.int32, dev)
+    if u.dtype != torch.float32 or tuple(u.shape) != (B, K + 1) or u.device != dev:
+        raise ValueError(f"{what}: u must be fp32 [{B}, {K + 1}] on {dev}")
+    u = u.contiguous()
+    accepted = torch.empty(B, dtype=torch.int32, device=dev)
+    tokens = torch.empty(B, K + 1, dtype=torch.int64, device=dev)
+    wsb = lib().capk_verify_drafts_workspace(B, K, V)
+    ws = _ws(wsb, dev)
+    dargs = (None, 0, 0) if draft is None or not K else (draft.data_ptr(), draft.stride(0), draft.stride(1))
+    _launch(dev, "capk_verify_drafts", code, B, K, V, target.data_ptr(), target.stride(0), target.stride(1), *dargs,
+            _p(ids), ids.stride(0), u.data_ptr(), u.stride(0), _p(draft_len), float(temperature), accepted.data_ptr(),
+            tokens.data_ptr(), tokens.stride(0), _p(ws), wsb)
+    return accepted, tokens

@@ -661,6 +661,87 @@ int capk_window_attn_bwd(int dtype, int nwin, int nw_img, int ws, int H, int hd,
 int capk_rowscale_add(int dtype, int rows, int cols, const void* x, int64_t ldx, const float* scale, int group_rows,
                       const void* res, int64_t ldr, void* y, int64_t ldy, void* stream);
 
+/* ------------------------------------------------- long-context decoding ----
+ * Rotary positions over several axes (time, height, width, ...), sliding-window attention whose
+ * first tokens stay visible, a paged key / value cache in 4 bits, and the verification of drafted
+ * tokens.  X views are [B, N, heads, hd]: element d of head h of token n of batch b at
+ * X + b*bs + n*rs + h*hs + d; rows must start 16-B aligned unless said otherwise.
+ *
+ * capk_axis_rope: pair i < pairs of a head turns by pos[axis[i]][b][n] * freq[i] radians
+ *   (pos + axis[i]*pos_as + b*pos_bs + n, int32; pos_bs = 0 shares positions over the batch;
+ *   freq fp64, axis uint8 < axes): (x1, x2) -> (x1 cos - x2 sin, x1 sin + x2 cos), angles in
+ *   64 bits.  interleaved = 0: pair i = elements i, i + pairs; 1: 2i, 2i + 1.  Elements from
+ *   2*pairs on are copied.  inverse = 1 turns back (the gradient).  q and k (Hk = 0: none) in one
+ *   launch; y may be x.  Any alignment (whole vectors where it allows).  hd <= 1024. */
+int capk_axis_rope(int dtype, int B, int N, int hd, int pairs, int interleaved, int inverse, int axes,
+                   const int32_t* pos, int64_t pos_as, int64_t pos_bs, const double* freq, const uint8_t* axis,
+                   int Hq, const void* q, int64_t q_bs, int64_t q_rs, int64_t q_hs, void* qo, int64_t qo_bs,
+                   int64_t qo_rs, int64_t qo_hs, int Hk, const void* k, int64_t k_bs, int64_t k_rs, int64_t k_hs,
+                   void* ko, int64_t ko_bs, int64_t ko_rs, int64_t ko_hs, void* stream);
+/* capk_sliding_attention_*: the Nq queries are the last positions of a sequence of kv_len[b] keys
+ *   (int32 [B], clamped to [0, Nk]; NULL: Nk).  The query at position p sees the keys j <= p with
+ *   j < sinks or p - j < window (window 0: every j <= p), less those with key_pad[b*Nk + j] != 0.
+ *   H query heads share Hk key heads (head h reads h / (H / Hk)).  o = softmax(scale q k^T) v,
+ *   lse (fp32 [B, H, Nq], optional forward) its log denominator; a query that sees nothing has
+ *   o = 0, lse = -inf.  Keys hidden from every query of a call are never used: NaN there is
+ *   harmless.  Nq <= 16 runs the decoding-step kernel (split over the keys, partial results in ws).
+ *   Backward: dq, dk, dv (all of them written), deterministic.  hd % 8 == 0, hd <= 128.
+ *   Lengths up to 2^28; no dropout. */
+size_t capk_sliding_attention_fwd_workspace(int dtype, int B, int H, int Hk, int Nq, int Nk, int hd, int window,
+                                            int sinks);
+int capk_sliding_attention_fwd(int dtype, int B, int H, int Hk, int Nq, int Nk, int hd, float scale, int window,
+                               int sinks, const void* q, int64_t q_bs, int64_t q_rs, int64_t q_hs, const void* k,
+                               int64_t k_bs, int64_t k_rs, int64_t k_hs, const void* v, int64_t v_bs, int64_t v_rs,
+                               int64_t v_hs, const uint8_t* key_pad, const int32_t* kv_len, void* o, int64_t o_bs,
+                               int64_t o_rs, int64_t o_hs, float* lse, void* ws, size_t ws_bytes, void* stream);
+size_t capk_sliding_attention_bwd_workspace(int B, int H, int Hk, int Nq, int Nk, int hd, int window, int sinks);
+int capk_sliding_attention_bwd(int dtype, int B, int H, int Hk, int Nq, int Nk, int hd, float scale, int window,
+                               int sinks, const void* q, int64_t q_bs, int64_t q_rs, int64_t q_hs, const void* k,
+                               int64_t k_bs, int64_t k_rs, int64_t k_hs, const void* v, int64_t v_bs, int64_t v_rs,
+                               int64_t v_hs, const uint8_t* key_pad, const int32_t* kv_len, const void* o,
+                               int64_t o_bs, int64_t o_rs, int64_t o_hs, const void* dout, int64_t do_bs,
+                               int64_t do_rs, int64_t do_hs, const float* lse, void* dq, int64_t dq_bs,
+                               int64_t dq_rs, int64_t dq_hs, void* dk, int64_t dk_bs, int64_t dk_rs, int64_t dk_hs,
+                               void* dv, int64_t dv_bs, int64_t dv_rs, int64_t dv_hs, void* ws, size_t ws_bytes,
+                               void* stream);
+/* The 4-bit cache: codes uint8 [pages][2: K, V][Hk][page][hd/2] (e2m1, the first of a pair in the low
+ *   half), scales uint8 [pages][2][Hk][page][hd/32] (E8M0), page a multiple of 16, hd in {32, 64, 96,
+ *   128}.  Token t of sequence b lives in page table[b*table_ld + t/page] (int32, table_cols columns),
+ *   slot t % page.  Per 32 elements the scale is the smallest power of two with amax <= 6 * scale
+ *   (code 127 for zeros, at least 1; 255, standing for NaN, for a block with an infinity or NaN).
+ * capk_kv4_append: rows i < n (i < count[b] where count != NULL) of k, v [B, n, Hk, hd] become tokens
+ *   start[b] + i; a token outside the table or on a page outside [0, pages) is dropped, everything
+ *   else is left as it was.  Two sequences must not write the same page slot in one call.
+ * capk_kv4_read: the values of tokens start[b] + i, i < n (zeros where there is no page).
+ * capk_kv4_attention: capk_sliding_attention_fwd over the cache for Nq <= 64 queries; keys without a
+ *   page are hidden.  kv_len is clamped to [0, table_cols * page]. */
+int capk_kv4_append(int dtype, int B, int n, int Hk, int hd, const void* k, int64_t k_bs, int64_t k_rs, int64_t k_hs,
+                    const void* v, int64_t v_bs, int64_t v_rs, int64_t v_hs, void* codes, void* scales, int pages,
+                    int page, const int32_t* table, int64_t table_ld, int table_cols, const int32_t* start,
+                    const int32_t* count, void* stream);
+int capk_kv4_read(int dtype, int B, int n, int Hk, int hd, const void* codes, const void* scales, int pages, int page,
+                  const int32_t* table, int64_t table_ld, int table_cols, const int32_t* start, void* k, int64_t k_bs,
+                  int64_t k_rs, int64_t k_hs, void* v, int64_t v_bs, int64_t v_rs, int64_t v_hs, void* stream);
+size_t capk_kv4_attention_workspace(int dtype, int B, int H, int Hk, int Nq, int hd, int window, int sinks, int page,
+                                    int table_cols);
+int capk_kv4_attention(int dtype, int B, int H, int Hk, int Nq, int hd, float scale, int window, int sinks,
+                       const void* q, int64_t q_bs, int64_t q_rs, int64_t q_hs, const void* codes, const void* scales,
+                       int pages, int page, const int32_t* table, int64_t table_ld, int table_cols,
+                       const int32_t* kv_len, void* o, int64_t o_bs, int64_t o_rs, int64_t o_hs, float* lse, void* ws,
+                       size_t ws_bytes, void* stream);
+/* capk_verify_drafts: p_i = softmax(target[b][i] / temperature), i <= K; q_i likewise from draft (NULL:
+ *   one-hot at the drafted token); V valid columns.  Drafts ids[b][i], i < draft_len[b] (clamped to
+ *   [0, K]; NULL: K), are accepted while u[b][i] * q_i(id) < p_i(id) (an id outside [0, V) never is);
+ *   accepted[b] = n of them, and one more token is drawn with u[b][K] by inverse CDF from
+ *   max(p_n - q_n, 0) after a refusal (from p_n where that leaves nothing), from p_n after draft_len
+ *   acceptances: the first token whose cumulative mass exceeds u times the whole.  tokens[b][0..K]
+ *   = the accepted ids, the drawn token, -1.  64-bit sums.  u in [0, 1) fp32 [B][K + 1]. */
+size_t capk_verify_drafts_workspace(int B, int K, int V);
+int capk_verify_drafts(int dtype, int B, int K, int V, const void* target, int64_t t_bs, int64_t t_rs,
+                       const void* draft, int64_t d_bs, int64_t d_rs, const int64_t* ids, int64_t ids_bs,
+                       const float* u, int64_t u_bs, const int32_t* draft_len, double temperature, int32_t* accepted,
+                       int64_t* tokens, int64_t tok_bs, void* ws, size_t ws_bytes, void* stream);
+
 /* ------------------------------------------------------ CIDEr-D (host) ----
  * SCST reward: replaces src/evaluate/metrics.py:46-110 (pycocoevalcap
  * CiderD, via CaptioningTrainer._calculate_rewards, src/train/trainer.py:440-484) with a

@@ -1,0 +1,703 @@
+"""Long-context decoding operators on the GPU against plain forms in 64 bits: rotary positions over
+several axes, sliding-window attention with visible first tokens (forward, gradients, decoding step), the
+4-bit paged cache, verification of drafted tokens, and a run of them together.
+
+Tolerances are worst-case bounds computed with each reference: U is half a step of the stored type (bf16
+2^-8, fp32 2^-24), counted once for every value that is rounded to that type (the output, the
+probabilities and score gradients that enter a product, the saved output), F = 2^-24 times the length of
+each 32-bit sum, and 2^-20 for the hardware's exp2 / log2 / sin / cos."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a GPU")]
+
+DT = {"bf16": torch.bfloat16, "fp32": torch.float32}
+U = {torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}
+F = 2.0 ** -24
+
+
+def _rand(*shape, seed=0, dtype=torch.float32, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device="cuda") * scale).to(dtype)
+
+
+def _close(got, ref, tol, what=""):
+    assert got.shape == ref.shape, what
+    assert torch.isfinite(got).all(), what
+    over = (got.double() - ref).abs() - tol
+    assert float(over.max()) <= 0, f"{what}: {float(over.max()):.3g} over the bound at {int(over.argmax())}"
+
+
+# ------------------------------------------------------------------------------------ rotary ---
+def _rope_ref(x, pos, freq, axis, interleaved, sign=1.0):
+    """(turned x, bound of the error besides the output's rounding) in 64 bits."""
+    P = freq.shape[0]
+    x = x.double()
+    pos = pos if pos.dim() == 3 else pos.unsqueeze(1).expand(-1, x.shape[0], -1)
+    a = (pos[axis.long()].double() * freq.view(-1, 1, 1)).permute(1, 2, 0).unsqueeze(2)
+    i = torch.arange(P, device="cuda")
+    e1, e2 = (2 * i, 2 * i + 1) if interleaved else (i, i + P)
+    y, slack = x.clone(), torch.zeros_like(x)
+    x1, x2, c, s = x[..., e1], x[..., e2], a.cos(), sign * a.sin()
+    y[..., e1], y[..., e2] = x1 * c - x2 * s, x1 * s + x2 * c
+    slack[..., e1] = slack[..., e2] = (x1.abs() + x2.abs()) * 2.0 ** -20
+    return y, slack
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("B,N,H,Hk,hd,pairs,interleaved", [
+    (1, 1, 1, 1, 64, 32, False), (3, 17, 12, 12, 64, 32, False), (2, 130, 8, 2, 128, 64, True),
+    (2, 9, 3, 1, 80, 20, False), (1, 33, 4, 4, 96, 24, True), (5, 7, 2, 1, 30, 11, False), (1, 2100, 2, 2, 32, 16, False)])
+def test_axis_rope(dtype, B, N, H, Hk, hd, pairs, interleaved):
+    from capk import context
+    dt = DT[dtype]
+    q, k = _rand(B, N, H, hd, seed=1, dtype=dt), _rand(B, N, Hk, hd, seed=2, dtype=dt)
+    axis = torch.arange(pairs, device="cuda") % 3
+    freq = torch.tensor([10000.0 ** (-i / pairs) for i in range(pairs)], dtype=torch.float64, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(3)
+    pos = torch.randint(-1000, 300000, (3, B, N), generator=g, device="cuda", dtype=torch.int32)
+    got = context.axis_rope(q, k, pos, freq, axis, interleaved=interleaved)
+    for x, y in zip((q, k), got):
+        ref, slack = _rope_ref(x, pos, freq, axis, interleaved)
+        _close(y, ref, U[dt] * ref.abs() + slack, "forward")
+    # the gradient turns back
+    q.requires_grad_(), k.requires_grad_()
+    y = context.axis_rope(q, k, pos, freq, axis, interleaved=interleaved)
+    w = [_rand(*t.shape, seed=4 + i, dtype=dt) for i, t in enumerate(y)]
+    for x, d, u in zip((q, k), torch.autograd.grad(y, (q, k), w), w):
+        ref, slack = _rope_ref(u, pos, freq, axis, interleaved, -1.0)
+        _close(d, ref, U[dt] * ref.abs() + slack, "gradient")
+
+
+def test_axis_rope_views_shared_positions_in_place_and_one_side():
+    from capk import context, ops
+    B, N, H, hd = 2, 21, 4, 64
+    freq, axis = context.axis_frequencies((8, 12, 12))
+    pos = torch.stack([torch.arange(N), torch.arange(N) // 5, torch.arange(N) % 5]).int().cuda()
+    qkv = _rand(B, N, 3, H, hd, seed=5)
+    q, k = qkv[:, :, 0], qkv[:, :, 1]
+    ref = [_rope_ref(x, pos, freq, axis, False) for x in (q, k)]
+    got = context.axis_rope(q, k, pos, freq, axis)
+    v0 = qkv[:, :, 2].clone()
+    ops.axis_rope(q, k, pos, freq, axis, out_q=q, out_k=k)  # in place, inside the fused buffer
+    for y, z, (r, slack) in zip(got, (q, k), ref):
+        _close(y, r, F * r.abs() + slack)
+        assert torch.equal(y, z)
+    assert torch.equal(qkv[:, :, 2], v0)
+    t = _rand(B, H, N, hd, seed=6).transpose(1, 2)  # [B, N, H, hd] with heads outside
+    y, none = context.axis_rope(t, None, pos, freq, axis)
+    r, slack = _rope_ref(t, pos, freq, axis, False)
+    _close(y, r, F * r.abs() + slack)
+    assert none is None
+    odd = _rand(B * N * H * hd + 1, seed=7)[1:].view(B, N, H, hd)  # 4-B aligned only
+    y, _ = context.axis_rope(odd, None, pos, freq, axis)
+    r, slack = _rope_ref(odd, pos, freq, axis, False)
+    _close(y, r, F * r.abs() + slack)
+    a = _rand(B, N, H, hd, seed=8).requires_grad_()
+    b = _rand(B, N, H, hd, seed=9).requires_grad_()
+    context.axis_rope(a, b, pos, freq, axis)[1].sum().backward()  # only k is used
+    assert a.grad is None or not a.grad.any()
+    r, slack = _rope_ref(torch.ones_like(b), pos, freq, axis, False, -1.0)
+    _close(b.grad, r, F * r.abs() + slack)
+    assert context.axis_rope(a[:0], b[:0], pos, freq, axis)[0].shape == (0, N, H, hd)
+
+
+# --------------------------------------------------------------------------------- attention ---
+def _see(B, Nq, Nk, window, sinks, key_pad, kv_len):
+    last = torch.full((B,), Nk, device="cuda") if kv_len is None else kv_len.clamp(0, Nk).long()
+    p = (last - Nq).view(B, 1, 1) + torch.arange(Nq, device="cuda").view(1, Nq, 1)
+    j = torch.arange(Nk, device="cuda").view(1, 1, Nk)
+    see = (j <= p) & (j < last.view(B, 1, 1))
+    if window:
+        see &= (j < sinks) | (p - j < window)
+    return see if key_pad is None else see & ~key_pad.view(B, 1, Nk)
+
+
+def _attention_ref(q, k, v, see, do=None, scale=None, u=0.0, up=None):
+    """{name: (value, bound)} in 64 bits; u: rounding of outputs, up: of the probabilities."""
+    up = u if up is None else up
+    B, Nq, H, hd = q.shape
+    G = H // k.shape[2]
+    scale = hd ** -0.5 if scale is None else scale
+    heads = lambda x: x.double().permute(0, 2, 1, 3).repeat_interleave(H // x.shape[2], 1)  # noqa: E731
+    back = lambda x: x.permute(0, 2, 1, 3)  # noqa: E731
+    q, k, v, see = heads(q), heads(k), heads(v), see.unsqueeze(1)
+    hide = ~see
+    k, v = (x.nan_to_num(0, 0, 0) if not torch.isfinite(x).all() else x for x in (k, v))
+    s = (q @ k.transpose(-1, -2) * scale).masked_fill(hide, -math.inf)
+    m = s.amax(-1, keepdim=True)
+    m = torch.where(m == -math.inf, 0.0, m)
+    p = torch.exp(s - m)
+    z = p.sum(-1, keepdim=True)
+    lse = (m + z.log()).squeeze(-1)
+    p = p / torch.where(z == 0, 1.0, z)
+    o = p @ v
+    # a probability's relative error: its score's (an hd-term sum) twice, the sum over keys, exp2 and log2
+    big = float(((q.abs() @ k.abs().transpose(-1, -2)) * scale * see).max())
+    ep = (2 * big * (hd + 4) + big + k.shape[2]) * F + 2.0 ** -20
+    A = p @ v.abs()
+    out = {"o": (back(o), back((up + 2 * ep) * A + u * o.abs())), "lse": (lse, lse.abs() * 2 * F + ep)}
+    if do is None:
+        return out
+    do = heads(do)
+    share = lambda x: back(x.view(B, H // G, G, *x.shape[2:]).sum(2))  # noqa: E731
+    dp, delta = do @ v.transpose(-1, -2), (do * o).sum(-1, keepdim=True)
+    ds = p * (dp - delta) * scale
+    # delta from the saved output (its own bound), 32-bit sums over hd
+    d_delta = (do.abs() * ((up + 2 * ep) * A + u * o.abs())).sum(-1, keepdim=True) + hd * F * (do * o).abs().sum(-1, keepdim=True)
+    d_dp = hd * F * (do.abs() @ v.abs().transpose(-1, -2))
+    d_ds = up * ds.abs() + p * scale * (d_delta + d_dp + 2 * ep * (dp.abs() + delta.abs()))
+    n = Nq * F * G
+    dv, dq, dk = p.transpose(-1, -2) @ do, ds @ k, ds.transpose(-1, -2) @ q
+    t_dv = (up + 2 * ep + n) * (p.transpose(-1, -2) @ do.abs())
+    t_dq = d_ds @ k.abs() + k.shape[2] * F * (ds.abs() @ k.abs())
+    t_dk = d_ds.transpose(-1, -2) @ q.abs() + n * (ds.abs().transpose(-1, -2) @ q.abs())
+    for name, x, t in (("dq", back(dq), back(t_dq)), ("dk", share(dk), share(t_dk)), ("dv", share(dv), share(t_dv))):
+        out[name] = (x, t + u * x.abs() + 1e-30)
+    return out
+
+
+def _slide_case(dtype, B, Nq, Nk, H, Hk, hd, window, sinks, pad=None, kv_len=None, grad=True, seed=0, scale=None):
+    from capk import context, ops
+    dt = DT[dtype]
+    q, k, v = (_rand(B, n, h, hd, seed=seed + i, dtype=dt) for i, (n, h) in enumerate(((Nq, H), (Nk, Hk), (Nk, Hk))))
+    do = _rand(B, Nq, H, hd, seed=seed + 3, dtype=dt) if grad else None
+    key_pad = None if pad is None else (torch.arange(Nk, device="cuda") >= torch.tensor(pad, device="cuda").view(B, 1))
+    kv_len = None if kv_len is None else torch.tensor(kv_len, dtype=torch.int32, device="cuda")
+    ref = _attention_ref(q, k, v, _see(B, Nq, Nk, window, sinks, key_pad, kv_len), do, scale, U[dt])
+    o, lse = ops.sliding_attention_fwd(q, k, v, window, sinks, hd ** -0.5 if scale is None else scale, key_pad, kv_len)
+    _close(o, *ref["o"], "o")
+    inf = torch.isinf(ref["lse"][0])
+    assert torch.equal(inf, lse == -math.inf)
+    _close(lse.masked_fill(inf, 0), ref["lse"][0].masked_fill(inf, 0), ref["lse"][1].nan_to_num(0, 0).masked_fill(inf, 0), "lse")
+    assert not o.permute(0, 2, 1, 3)[inf].any()
+    if not grad:
+        return
+    q, k, v = (x.requires_grad_() for x in (q, k, v))
+    kw = dict(window=window, sinks=sinks, scale=scale, key_pad=key_pad, kv_len=kv_len)
+    got = torch.autograd.grad(context.sliding_attention(q, k, v, **kw), (q, k, v), do)
+    for name, x in zip(("dq", "dk", "dv"), got):
+        _close(x, *ref[name], name)
+    again = torch.autograd.grad(context.sliding_attention(q, k, v, **kw), (q, k, v), do)
+    assert all(torch.equal(a, b) for a, b in zip(got, again))  # deterministic
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("B,N,H,Hk,hd,window,sinks", [
+    (1, 1, 1, 1, 64, 1, 0), (2, 2, 2, 1, 32, 1, 1), (1, 63, 2, 2, 64, 5, 0), (2, 64, 4, 2, 128, 64, 4),
+    (1, 65, 3, 1, 96, 200, 0), (1, 129, 2, 1, 80, 16, 3), (1, 200, 2, 2, 8, 0, 0), (2, 333, 4, 1, 64, 50, 130),
+    (1, 700, 2, 1, 64, 30, 4), (1, 1300, 2, 1, 128, 100, 131), (1, 900, 1, 1, 64, 900, 900), (1, 1500, 2, 2, 32, 1, 0)])
+def test_sliding_attention_sizes(dtype, B, N, H, Hk, hd, window, sinks):
+    _slide_case(dtype, B, N, N, H, Hk, hd, window, sinks)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("B,Nq,Nk,window,sinks,pad,kv_len", [
+    (3, 100, 100, 20, 0, (100, 37, 1), None),        # right-padded; late rows see nothing
+    (2, 100, 100, 20, 5, (0, 60), None),             # one sequence entirely hidden
+    (3, 70, 300, 64, 7, None, (300, 70, 129)),       # chunks against caches of different lengths
+    (3, 70, 300, 0, 0, None, (0, 30, 71)),           # fewer keys than queries, none at all
+    (2, 40, 1500, 200, 140, (1500, 900), (1400, 1500)),
+    (1, 300, 77, 16, 2, None, None),                 # more queries than keys
+])
+def test_sliding_attention_masks_and_lengths(dtype, B, Nq, Nk, window, sinks, pad, kv_len):
+    _slide_case(dtype, B, Nq, Nk, 4, 2, 64, window, sinks, pad, kv_len, seed=11)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("B,Nq,Nk,H,Hk,hd,window,sinks,pad,kv_len", [
+    (1, 1, 1, 1, 1, 64, 1, 0, None, None), (2, 1, 100, 12, 12, 64, 0, 0, None, (100, 1)),
+    (3, 1, 1000, 8, 1, 128, 100, 4, None, (1000, 513, 0)), (2, 7, 600, 6, 2, 96, 33, 50, (600, 400), (599, 600)),
+    (1, 16, 5000, 8, 1, 128, 0, 0, None, None), (2, 5, 3000, 32, 2, 80, 1024, 197, None, (3, 3000)),
+    (1, 16, 40, 6, 1, 32, 3, 0, None, (10,)), (40, 1, 300, 16, 16, 64, 64, 4, None, tuple(range(7, 287, 7)))])
+def test_sliding_attention_step(dtype, B, Nq, Nk, H, Hk, hd, window, sinks, pad, kv_len):
+    """Few queries: the kernel that splits the keys (gradients run the others)."""
+    _slide_case(dtype, B, Nq, Nk, H, Hk, hd, window, sinks, pad, kv_len, seed=21, grad=Nk <= 1000)
+
+
+def test_sliding_attention_step_matches_prefill_rows():
+    """Decoding token by token gives the rows of the whole pass."""
+    from capk import context
+    B, N, H, Hk, hd, kw = 2, 150, 4, 2, 64, dict(window=40, sinks=3)
+    q, k, v = _rand(B, N, H, hd, seed=31), _rand(B, N, Hk, hd, seed=32), _rand(B, N, Hk, hd, seed=33)
+    whole = context.sliding_attention(q, k, v, **kw)
+    for t in (0, 1, 39, 40, 42, 43, 149):
+        n = torch.full((B,), t + 1, dtype=torch.int32, device="cuda")
+        one = context.sliding_attention(q[:, t:t + 1], k, v, kv_len=n, **kw)
+        ref = _attention_ref(q[:, t:t + 1], k, v, _see(B, 1, N, 40, 3, None, n), u=F)["o"]
+        _close(one, *ref)
+        _close(whole[:, t:t + 1], *ref)
+
+
+@pytest.mark.parametrize("Nq", [1, 100])
+def test_sliding_attention_hidden_values_are_not_used(Nq):
+    """NaN and infinities behind kv_len, under key_pad and before the window change nothing."""
+    from capk import context
+    B, Nk, H, hd = 2, 400, 2, 64
+    q, k, v = (_rand(B, n, H, hd, seed=41 + i, dtype=torch.bfloat16) for i, n in enumerate((Nq, Nk, Nk)))
+    n = torch.tensor([300, 350], dtype=torch.int32, device="cuda")
+    pad = torch.zeros(B, Nk, dtype=torch.bool, device="cuda")
+    pad[:, 290:295] = True
+    kw = dict(window=50, sinks=4, key_pad=pad, kv_len=n)
+    clean = context.sliding_attention(q, k, v, **kw)
+    k2, v2 = k.clone(), v.clone()
+    for b in range(B):
+        first = int(n[b]) - Nq - 50 + 1
+        for x, bad in ((k2, math.nan), (v2, math.inf), (v2, math.nan)):
+            x[b, int(n[b]):] = bad
+            x[b, 290:295] = bad
+            x[b, 4:max(4, first)] = bad
+    assert torch.equal(clean, context.sliding_attention(q, k2, v2, **kw))
+    k3, v3 = (x.clone().requires_grad_() for x in (k2, v2))
+    q3 = q.clone().requires_grad_()
+    grads = torch.autograd.grad(context.sliding_attention(q3, k3, v3, **kw).sum(), (q3, k3, v3))
+    assert all(torch.isfinite(g).all() for g in grads)
+
+
+def test_sliding_attention_views_and_orders():
+    """Heads outside tokens, fused q/k/v rows, a batch-expanded cache, an unaligned slice and an expanded gradient."""
+    from capk import context
+    B, N, H, hd = 2, 90, 4, 64
+    kw = dict(window=25, sinks=2)
+    qkv = _rand(B, N, 3, H, hd, seed=51, dtype=torch.bfloat16)
+    q, k, v = qkv.unbind(2)
+    ref = _attention_ref(q, k, v, _see(B, N, N, 25, 2, None, None), u=2.0 ** -8)["o"]
+    _close(context.sliding_attention(q, k, v, **kw), *ref)
+    t = [x.transpose(1, 2).contiguous().transpose(1, 2) for x in (q, k, v)]
+    _close(context.sliding_attention(*t, **kw), *ref)
+    one = [x[:1].expand(B, N, H, hd) for x in (k, v)]
+    ref1 = _attention_ref(q, *one, _see(B, N, N, 25, 2, None, None), u=2.0 ** -8)["o"]
+    _close(context.sliding_attention(q, *one, **kw), *ref1)
+    odd = torch.empty(B, N, H, hd + 4, dtype=torch.bfloat16, device="cuda")[..., 4:]
+    odd.copy_(q)
+    _close(context.sliding_attention(odd, k, v, **kw), *ref)
+    x = [y.detach().clone().requires_grad_() for y in (q, k, v)]
+    context.sliding_attention(*x, **kw).sum().backward()  # a gradient of stride 0
+    y = [z.detach().clone().requires_grad_() for z in (q, k, v)]
+    context.sliding_attention(*y, **kw).backward(torch.ones_like(q))
+    assert all(torch.equal(a.grad, b.grad) for a, b in zip(x, y))
+    e = context.sliding_attention(q[:, :0], k, v, **kw)
+    assert e.shape == (B, 0, H, hd)
+    assert not context.sliding_attention(q, k[:, :0], v[:, :0], **kw).any()
+
+
+def test_sliding_attention_gradient_against_differences():
+    from capk import context
+    B, N, H, Hk, hd, window, sinks = 1, 70, 2, 1, 32, 20, 3
+    x = [_rand(B, N, h, hd, seed=61 + i) for i, h in enumerate((H, Hk, Hk))]
+    w = _rand(B, N, H, hd, seed=64).double()
+    see = _see(B, N, N, window, sinks, None, None)
+    loss = lambda y: float((_attention_ref(*y, see)["o"][0] * w).sum())  # noqa: E731
+    leaf = [y.clone().requires_grad_() for y in x]
+    grads = torch.autograd.grad(context.sliding_attention(*leaf, window=window, sinks=sinks), leaf, w.float())
+    for i, g in enumerate(grads):
+        d = _rand(*x[i].shape, seed=65 + i).double()
+        h = 1e-4
+        ends = [loss([y.double() + (s * h * d if j == i else 0) for j, y in enumerate(x)]) for s in (1, -1)]
+        num, ana = (ends[0] - ends[1]) / (2 * h), float((g.double() * d).sum())
+        # second-order term h^2 f''' (f''' of this loss is below 1e4 of its gradient's size), 32-bit gradients
+        assert abs(num - ana) <= 1e-4 * float((g.double() * d).abs().sum()), (i, num, ana)
+
+
+def test_sliding_attention_offsets_past_32_bits():
+    """A cache of more than 2^31 elements: the sinks at its start and the window at its end."""
+    from capk import context
+    N, hd, Nq = 17_000_000, 128, 3
+    k, v = (torch.zeros(1, N, 1, hd, dtype=torch.bfloat16, device="cuda") for _ in "kv")
+    tail = 200
+    for x, s in ((k, 71), (v, 72)):
+        x[:, :8] = _rand(1, 8, 1, hd, seed=s, dtype=torch.bfloat16)
+        x[:, -tail:] = _rand(1, tail, 1, hd, seed=s + 2, dtype=torch.bfloat16)
+    for nq in (Nq, 40):
+        q = _rand(1, nq, 2, hd, seed=75, dtype=torch.bfloat16)
+        got = context.sliding_attention(q, k, v, window=100, sinks=8)
+        ks, vs = (torch.cat([x[:, :8], x[:, -tail:]], 1) for x in (k, v))
+        _close(got, *_attention_ref(q, ks, vs, _see(1, nq, 8 + tail, 100, 8, None, None), u=2.0 ** -8)["o"])
+    del k, v
+    torch.cuda.empty_cache()
+
+
+# ----------------------------------------------------------------------------- 4-bit cache ---
+LEVELS = np.array([0, .5, 1, 1.5, 2, 3, 4, 6])
+
+
+def _kv4_ref(x):
+    """What 32-element blocks of x [..., hd] stand for after rounding, element by element in 64 bits."""
+    x = x.double().cpu().numpy()
+    b = x.reshape(-1, 32)
+    out = np.empty_like(b)
+    for i, r in enumerate(b):
+        if not np.isfinite(r).all():
+            out[i] = np.nan
+            continue
+        amax = np.abs(r).max()
+        e = 0
+        if amax > 0:
+            e = max(-126, math.frexp(amax)[1] - 5)
+            while amax > 6 * 2.0 ** e:
+                e += 1
+        y = np.abs(r) / 2.0 ** e
+        d = np.abs(y[:, None] - LEVELS)
+        best = d.min(1)
+        near = d == best[:, None]
+        pick = [next((c for c in np.flatnonzero(n) if c % 2 == 0), np.flatnonzero(n)[0]) for n in near]  # ties: even
+        out[i] = np.sign(r) * LEVELS[pick] * 2.0 ** e
+    return torch.from_numpy(out.reshape(x.shape)).cuda()
+
+
+def _table(B, per, pages, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randperm(pages, generator=g)[:B * per].view(B, per).int().cuda()
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("B,n,Hk,hd,page,start", [
+    (1, 1, 1, 32, 16, (0,)), (2, 37, 2, 64, 16, (0, 15)), (3, 20, 1, 96, 48, (5, 47, 100)), (2, 70, 3, 128, 64, (63, 1))])
+def test_kv4_append_and_read(dtype, B, n, Hk, hd, page, start):
+    from capk import context
+    dt = DT[dtype]
+    k, v = (_rand(B, n, Hk, hd, seed=81 + i, dtype=dt, scale=s) for i, s in enumerate((1.0, 37.0)))
+    # all the levels and the ties between them, at several powers of two; a block of zeros; tiny values
+    edge = torch.tensor([0, .25, .5, .75, 1, 1.25, 1.5, 1.75, 2, 2.5, 3, 3.5, 4, 5, 6, -6] * 2, device="cuda")
+    for i, s in enumerate((1.0, 2.0 ** -9, 2.0 ** 20, 0.0, 2.0 ** -130)):
+        k.view(-1, 32)[i % (k.numel() // 32)] = (edge * s).to(dt)
+    cache = context.KV4Cache.empty(B * 12 + 2, Hk, hd, page)
+    table = _table(B, 12, B * 12 + 2)
+    start = torch.tensor(start, dtype=torch.int32, device="cuda")
+    before = cache.codes.clone()
+    cache.append(k, v, table, start)
+    gk, gv = cache.read(table, start, n, torch.float32)
+    assert torch.equal(gk.double(), _kv4_ref(k)) and torch.equal(gv.double(), _kv4_ref(v))
+    # nothing beside the written tokens moved
+    t = start.long().view(-1, 1) + torch.arange(n, device="cuda")
+    at = table.long().gather(1, t // page), t % page
+    after = cache.codes.clone()
+    for i in (0, 1):
+        after[:, i].permute(0, 2, 1, 3)[at] = before[:, i].permute(0, 2, 1, 3)[at]
+    assert torch.equal(after, before)
+
+
+def test_kv4_bad_pages_counts_and_non_finite():
+    """Tokens without a page are dropped and read as zeros; count leaves the padded rows alone; a block with an
+    infinity or a NaN stands for NaN."""
+    from capk import context
+    B, n, Hk, hd, page = 3, 40, 1, 64, 16
+    k, v = (_rand(B, n, Hk, hd, seed=91 + i) for i in (0, 1))
+    k[1, 3, 0, 5], v[1, 4, 0, 40] = math.inf, math.nan
+    cache = context.KV4Cache.empty(9, Hk, hd, page)
+    table = torch.tensor([[0, -1, 2], [3, 4, 9], [6, 7, 8]], dtype=torch.int32, device="cuda")
+    start = torch.tensor([0, 0, 30], dtype=torch.int32, device="cuda")  # the last runs past its table
+    count = torch.tensor([40, 40, 12], dtype=torch.int32, device="cuda")
+    cache.append(k, v, table, start, count)
+    gk, gv = cache.read(table, torch.zeros_like(start), 48, torch.float32)
+    rk, rv = (_kv4_ref(x) for x in (k, v))
+    for got, ref in ((gk, rk), (gv, rv)):
+        got = got.double()
+        assert not got[0, 16:32].any() and torch.equal(got[0, :16], ref[0, :16]) and torch.equal(got[0, 32:40], ref[0, 32:])
+        assert torch.allclose(got[1, :32], ref[1, :32], rtol=0, atol=0, equal_nan=True) and not got[1, 32:].any()
+        assert not got[2, :30].any() and torch.equal(got[2, 30:42], ref[2, :12]) and not got[2, 42:].any()
+    assert torch.isnan(gk[1, 3, 0, :32]).all() and torch.isfinite(gk[1, 3, 0, 32:]).all()
+    assert torch.isnan(gv[1, 4, 0, 32:]).all()
+    # keys without a page are hidden
+    q = _rand(B, 1, 2, hd, seed=94)
+    kv_len = torch.tensor([40, 2, 42], dtype=torch.int32, device="cuda")
+    got = cache.attend(q, table, kv_len)
+    see = _see(B, 1, 48, 0, 0, None, kv_len)
+    see[0, :, 16:32] = False
+    _close(got, *_attention_ref(q, gk, gv, see, u=F)["o"])
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("B,Nq,H,Hk,hd,page,cols,kv_len,window,sinks", [
+    (1, 1, 1, 1, 32, 16, 1, (1,), 0, 0), (2, 1, 12, 12, 64, 64, 4, (256, 3), 0, 0), (3, 5, 8, 2, 128, 16, 40, (640, 5, 0), 0, 0),
+    (2, 8, 32, 2, 96, 48, 30, (1400, 700), 100, 5), (1, 2, 8, 1, 128, 128, 100, (12800,), 0, 0),
+    (2, 1, 16, 4, 64, 32, 70, (2240, 2000), 500, 40), (1, 64, 4, 1, 128, 16, 20, (300,), 0, 0), (1, 3, 4, 4, 64, 16, 3, (2,), 0, 0),
+    (70, 1, 4, 2, 64, 32, 5, tuple(range(1, 141, 2)), 40, 2)])
+def test_kv4_attention(dtype, B, Nq, H, Hk, hd, page, cols, kv_len, window, sinks):
+    from capk import context
+    dt = DT[dtype]
+    n = cols * page
+    cache = context.KV4Cache.empty(B * cols + 5, Hk, hd, page)
+    table = _table(B, cols, B * cols + 5, seed=1)
+    k, v = (_rand(B, n, Hk, hd, seed=101 + i, scale=2.0) for i in (0, 1))
+    zero = torch.zeros(B, dtype=torch.int32, device="cuda")
+    cache.append(k, v, table, zero)
+    k, v = cache.read(table, zero, n, torch.float32)
+    q = _rand(B, Nq, H, hd, seed=103, dtype=dt)
+    kv_len = torch.tensor(kv_len, dtype=torch.int32, device="cuda")
+    got = cache.attend(q, table, kv_len, window=window, sinks=sinks)
+    _close(got, *_attention_ref(q, k, v, _see(B, Nq, n, window, sinks, None, kv_len), u=U[dt])["o"])
+
+
+def test_kv4_stale_slots_and_shared_pages():
+    """NaN in slots behind the length is never used, and two sequences may read the same pages."""
+    from capk import context
+    cache = context.KV4Cache.empty(4, 1, 64, 16)
+    cache.scales.fill_(255)
+    table = torch.tensor([[0, 1], [0, 2]], dtype=torch.int32, device="cuda")
+    k = _rand(1, 20, 1, 64, seed=111)
+    cache.append(k, k, table[:1], torch.zeros(1, dtype=torch.int32, device="cuda"))
+    cache.append(k[:, 16:18], k[:, 16:18], table[1:], torch.full((1,), 16, dtype=torch.int32, device="cuda"))
+    q = _rand(1, 1, 2, 64, seed=112).expand(2, 1, 2, 64)
+    kv_len = torch.tensor([18, 18], dtype=torch.int32, device="cuda")
+    got = cache.attend(q, table, kv_len)
+    assert torch.isfinite(got).all() and torch.equal(got[0], got[1])
+
+
+def test_kv4_offsets_past_32_bits():
+    """Pages past 2^31 bytes of codes."""
+    from capk import context
+    page, Hk, hd = 128, 8, 128
+    pages = (1 << 31) // (2 * Hk * page * hd // 2) + 40
+    cache = context.KV4Cache(torch.zeros(pages, 2, Hk, page, hd // 2, dtype=torch.uint8, device="cuda"),
+                             torch.full((pages, 2, Hk, page, hd // 32), 127, dtype=torch.uint8, device="cuda"))
+    table = torch.arange(pages - 1, pages - 4, -1, dtype=torch.int32, device="cuda").view(1, 3)
+    k, v = (_rand(1, 300, Hk, hd, seed=121 + i) for i in (0, 1))
+    zero = torch.zeros(1, dtype=torch.int32, device="cuda")
+    cache.append(k, v, table, zero)
+    gk, gv = cache.read(table, zero, 300, torch.float32)
+    assert torch.equal(gk.double(), _kv4_ref(k)) and torch.equal(gv.double(), _kv4_ref(v))
+    q = _rand(1, 2, 16, hd, seed=123)
+    n = torch.tensor([300], dtype=torch.int32, device="cuda")
+    _close(cache.attend(q, table, n), *_attention_ref(q, gk, gv, _see(1, 2, 300, 0, 0, None, n), u=F)["o"])
+
+
+# ----------------------------------------------------------------------------- verification ---
+def _verify_ref(target, ids, u, draft, draft_len, t):
+    """Sequence by sequence in 64 bits on the host."""
+    B, K1, V = target.shape
+    soft = lambda x: (lambda e: e / e.sum())(np.exp(x - x.max()))  # noqa: E731
+    target = target.double().cpu().numpy() / t
+    draft = None if draft is None else draft.double().cpu().numpy() / t
+    ids, u = ids.cpu().numpy(), u.double().cpu().numpy()
+    acc, tok = np.zeros(B, np.int32), np.full((B, K1), -1, np.int64)
+    for b in range(B):
+        n, length = 0, K1 - 1 if draft_len is None else min(max(int(draft_len[b]), 0), K1 - 1)
+        rest = None
+        while n < length:
+            p = soft(target[b, n])
+            x = ids[b, n]
+            q = soft(draft[b, n]) if draft is not None else np.eye(1, V, x if 0 <= x < V else V)[0]
+            if not (0 <= x < V and u[b, n] * q[x] < p[x]):
+                rest = np.maximum(p - q, 0)
+                break
+            tok[b, n] = x
+            n += 1
+        if rest is None or not rest.sum() > 0:
+            rest = soft(target[b, n])
+        c = np.cumsum(rest)
+        tok[b, n] = np.argmax(c > u[b, K1 - 1] * c[-1])
+        acc[b] = n
+    return acc, tok
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("B,K,V,one_hot,ragged,t", [
+    (1, 1, 2, False, False, 1.0), (1, 0, 100, False, False, 1.0), (5, 4, 1000, False, True, 0.7), (3, 7, 4096, True, False, 1.0),
+    (2, 3, 4097, False, False, 1.5), (9, 5, 50257, False, True, 1.0), (4, 2, 50257, True, True, 0.9), (40, 1, 7, False, False, 1.0)])
+def test_verify_drafts(dtype, B, K, V, one_hot, ragged, t):
+    from capk import context
+    dt = DT[dtype]
+    g = torch.Generator(device="cuda").manual_seed(131)
+    target = (3 * _rand(B, K + 1, V, seed=132)).to(dt)
+    draft = (target[:, :K].float() + _rand(B, K, V, seed=133)).to(dt) if K else None
+    ids = torch.randint(0, V, (B, K), generator=g, device="cuda")
+    if K:
+        best = draft.float().argmax(-1)
+        ids = torch.where(torch.rand(B, K, generator=g, device="cuda") < 0.8, best, ids)
+    u = torch.rand(B, K + 1, generator=g, device="cuda")
+    draft_len = torch.randint(-1, K + 2, (B,), generator=g, device="cuda") if ragged else None
+    draft = None if one_hot else draft
+    n, tok = context.verify_drafts(target, ids, u, draft, draft_len=draft_len, temperature=t)
+    rn, rt = _verify_ref(target, ids, u, draft, draft_len, t)
+    assert n.cpu().numpy().tolist() == rn.tolist()
+    assert tok.cpu().numpy().tolist() == rt.tolist()
+
+
+def test_verify_drafts_edges():
+    """Padded vocabulary columns, hidden tokens (-inf), ids outside the vocabulary, equal distributions, u at its ends."""
+    from capk import context
+    B, K, V, ld = 6, 2, 300, 320
+    target, draft = _rand(B, K + 1, ld, seed=141), _rand(B, K, ld, seed=142)
+    target[..., V:] = draft[..., V:] = 1e30  # never read
+    target[:, :, 7] = -math.inf
+    draft[1], ids = target[1, :K], torch.randint(0, V, (B, K), device="cuda", generator=torch.Generator("cuda").manual_seed(143))
+    ids[0, 0], ids[2, 1], ids[3, 0], ids[4, 0] = 7, V, -1, 5
+    u = torch.rand(B, K + 1, device="cuda", generator=torch.Generator("cuda").manual_seed(144))
+    u[4], u[5] = 0.0, 1 - 2.0 ** -24
+    n, tok = context.verify_drafts(target, ids, u, draft, vocab_size=V)
+    rn, rt = _verify_ref(target[..., :V], ids, u, draft[..., :V], None, 1.0)
+    assert n.cpu().numpy().tolist() == rn.tolist() and tok.cpu().numpy().tolist() == rt.tolist()
+    assert (tok != 7).all()
+    # a refusal that leaves no residual (the same rows, an impossible token) draws from the target
+    draft[0] = target[0, :K]
+    n, tok = context.verify_drafts(target, ids, u, draft, vocab_size=V)
+    assert int(n[0]) == 0 and 0 <= int(tok[0, 0]) < V
+    # rows of NaN or of nothing but -inf still give a token of the vocabulary
+    for bad in (math.nan, -math.inf):
+        target[3] = bad
+        n, tok = context.verify_drafts(target, ids, u, draft, vocab_size=V)
+        assert int(n[3]) == 0 and 0 <= int(tok[3, 0]) < V and (tok[3, 1:] == -1).all()
+    # strides: every second row of a larger buffer
+    big = _rand(B, 2 * (K + 1), V, seed=145)
+    a = context.verify_drafts(big[:, ::2], ids, u, None)
+    b = context.verify_drafts(big[:, ::2].contiguous(), ids, u, None)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    assert context.verify_drafts(target[:0], ids[:0], u[:0], draft[:0], vocab_size=V)[1].shape == (0, K + 1)
+
+
+# --------------------------------------------------------------------------------- together ---
+def _decode_step(state, x, ids, pos, start, u):
+    """Rotate, append to the 4-bit cache, attend over it, project to logits and verify: one speculative step."""
+    from capk import context
+    B, n = x.shape[:2]
+    q, k, v = (torch.matmul(x.float(), w).to(x.dtype).view(B, n, -1, 64) for w in state["w"])
+    q, k = context.axis_rope(q, k, pos, state["freq"], state["axis"])
+    state["cache"].append(k, v, state["table"], start)
+    o = state["cache"].attend(q, state["table"], start + n, window=48, sinks=5)
+    logits = torch.matmul(o.reshape(B, n, -1).float(), state["head"]).to(x.dtype)
+    return o, logits, context.verify_drafts(logits, ids, u)
+
+
+def _state(B):
+    from capk import context
+    freq, axis = context.axis_frequencies((8, 12, 12))
+    return {"w": [_rand(128, d, seed=151 + d, scale=0.1) for d in (256, 128, 128)], "head": _rand(256, 500, seed=155, scale=0.2),
+            "freq": freq, "axis": axis, "cache": context.KV4Cache.empty(20, 2, 64, 16), "table": _table(B, 8, 20, seed=2)}
+
+
+@pytest.mark.parametrize("dtype", DT)
+def test_together(dtype):
+    """A prompt in one pass and two speculative steps, against the same computation in 64 bits on what the cache holds."""
+    from capk import context
+    B, n0, K, dt = 2, 60, 3, DT[dtype]
+    s = _state(B)
+    x = _rand(B, n0, 128, seed=161, dtype=dt)
+    pos = torch.arange(n0, device="cuda", dtype=torch.int32).expand(3, n0).contiguous()
+    q, k, v = (torch.matmul(x.float(), w).to(dt).view(B, n0, -1, 64) for w in s["w"])
+    q, k = context.axis_rope(q, k, pos, s["freq"], s["axis"])
+    o = context.sliding_attention(q, k, v, window=48, sinks=5)
+    _close(o, *_attention_ref(q, k, v, _see(B, n0, n0, 48, 5, None, None), u=U[dt])["o"])
+    start = torch.zeros(B, dtype=torch.int32, device="cuda")
+    s["cache"].append(k, v, s["table"], start)
+    start = start + n0
+    for step in range(2):
+        x = _rand(B, K + 1, 128, seed=162 + step, dtype=dt)
+        ids = torch.randint(0, 500, (B, K), device="cuda")
+        u = torch.rand(B, K + 1, device="cuda")
+        pos = (start.view(1, B, 1) + torch.arange(K + 1, device="cuda", dtype=torch.int32)).expand(3, B, K + 1).contiguous()
+        o, logits, (n, tok) = _decode_step(s, x, ids, pos, start, u)
+        q = torch.matmul(x.float(), s["w"][0]).to(dt).view(B, K + 1, -1, 64)
+        q, _ = context.axis_rope(q, None, pos, s["freq"], s["axis"])
+        ck, cv = s["cache"].read(s["table"], torch.zeros_like(start), 128, torch.float32)
+        _close(o, *_attention_ref(q, ck, cv, _see(B, K + 1, 128, 48, 5, None, start + K + 1), u=U[dt])["o"])
+        rn, rt = _verify_ref(logits, ids, u, None, None, 1.0)
+        assert n.cpu().numpy().tolist() == rn.tolist() and tok.cpu().numpy().tolist() == rt.tolist()
+        start = start + n + 1
+
+
+def test_together_captured_and_replayed():
+    """The speculative step in a HIP graph: every replay equals the eager call on the same inputs."""
+    B, K = 2, 3
+    s = _state(B)
+    start = torch.tensor([40, 17], dtype=torch.int32, device="cuda")
+    x = _rand(B, K + 1, 128, seed=171, dtype=torch.bfloat16)
+    ids = torch.randint(0, 500, (B, K), device="cuda")
+    u = torch.rand(B, K + 1, device="cuda")
+    pos = torch.zeros(3, B, K + 1, dtype=torch.int32, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        _decode_step(s, x, ids, pos, start, u)  # (work on another stream than the default one)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o, logits, (n, tok) = _decode_step(s, x, ids, pos, start, u)
+    for r in range(4):
+        x.copy_(_rand(B, K + 1, 128, seed=172 + r, dtype=torch.bfloat16))
+        u.copy_(torch.rand(B, K + 1, device="cuda"))
+        pos.copy_(torch.full_like(pos, 40 + r))
+        start.copy_(torch.tensor([40 + 3 * r, 17 + r], dtype=torch.int32))
+        graph.replay()
+        got = [t.clone() for t in (o, logits, n, tok)]
+        eo, el, (en, et) = _decode_step(s, x, ids, pos, start, u)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, (eo, el, en, et))), r
+
+
+def test_training_pass_captured_and_replayed():
+    """Forward and gradients of rotary positions and sliding attention in a graph (fresh leaves, no eager graph alive)."""
+    from capk import ops, context
+    B, N, H, Hk, hd = 2, 200, 4, 2, 64
+    freq, axis = context.axis_frequencies((8, 12, 12))
+    pos = torch.arange(N, device="cuda", dtype=torch.int32).expand(3, N).contiguous()
+    q, k, v, do = (_rand(B, N, h, hd, seed=181 + i, dtype=torch.bfloat16) for i, h in enumerate((H, Hk, Hk, H)))
+
+    def step():
+        rq, rk = ops.axis_rope(q, k, pos, freq, axis)
+        o, lse = ops.sliding_attention_fwd(rq, rk, v, 30, 140, hd ** -0.5)
+        dq, dk, dv = ops.sliding_attention_bwd(rq, rk, v, o, do, lse, 30, 140, hd ** -0.5)
+        return (o, dv) + ops.axis_rope(dq, dk, pos, freq, axis, inverse=True)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for r in range(3):
+        for i, t in enumerate((q, k, v, do)):
+            t.copy_(_rand(*t.shape, seed=190 + 4 * r + i, dtype=torch.bfloat16))
+        graph.replay()
+        got = [t.clone() for t in out]
+        ref = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, ref)), r
+
+
+# --------------------------------------------------------------------------------- refusals ---
+def test_refusals():
+    from capk import context, ops
+    from capk._lib import CapkError
+    q, k = _rand(2, 5, 4, 64), _rand(2, 5, 2, 64)
+    freq, axis = context.axis_frequencies((8, 12, 12))
+    pos = torch.zeros(3, 2, 5, dtype=torch.int32, device="cuda")
+    for call in (lambda: context.axis_rope(q.half(), k.half(), pos, freq, axis),
+                 lambda: context.axis_rope(q, k.bfloat16(), pos, freq, axis),
+                 lambda: context.axis_rope(q.cpu(), k, pos, freq, axis),
+                 lambda: context.axis_rope(q, k[:1], pos, freq, axis),
+                 lambda: context.axis_rope(q, k, pos[:, :, :4], freq, axis),
+                 lambda: context.axis_rope(q, k, pos.float(), freq, axis),
+                 lambda: context.axis_rope(q, k, pos, freq.float(), axis),
+                 lambda: context.axis_rope(q, k, pos, freq, axis[:-1]),
+                 lambda: context.axis_rope(q[..., :32], k[..., :32], pos, freq, axis),  # more pairs than the head has
+                 lambda: context.sliding_attention(q, k, k, window=-1),
+                 lambda: context.sliding_attention(q, k, k, window=1, sinks=-2),
+                 lambda: context.sliding_attention(q[:, :, :3], k, k, window=1),
+                 lambda: context.sliding_attention(q, k, k[:, :4], window=1),
+                 lambda: context.sliding_attention(q[..., :60], k[..., :60], k[..., :60], window=1),
+                 lambda: context.sliding_attention(q, k, k, kv_len=torch.ones(3, dtype=torch.int32, device="cuda")),
+                 lambda: context.sliding_attention(q, k, k, key_pad=torch.zeros(2, 5, device="cuda")),
+                 lambda: ops.sliding_attention_fwd(q[..., 1:], k[..., 1:], k[..., 1:], 1, 0, 1.0),
+                 lambda: context.KV4Cache.empty(4, 1, 48), lambda: context.KV4Cache.empty(4, 1, 64, page=20)):
+        with pytest.raises((CapkError, ValueError)):
+            call()
+    c = context.KV4Cache.empty(4, 2, 64, 16)
+    t, z = torch.zeros(2, 2, dtype=torch.int32, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+    u, ids = torch.rand(2, 3, device="cuda"), torch.zeros(2, 2, dtype=torch.int64, device="cuda")
+    logits = _rand(2, 3, 50)
+    for call in (lambda: c.append(k[..., :32], k[..., :32], t, z), lambda: c.append(k, k, t[:1], z),
+                 lambda: c.append(k, k, t.float(), z), lambda: c.append(k, k, t, z[:1]),
+                 lambda: c.append(q, q, t, z), lambda: c.read(t, z, 4, torch.float16), lambda: c.read(t, z, -1),
+                 lambda: c.attend(_rand(2, 65, 4, 64), t, z), lambda: c.attend(q[:, :, :3], t, z),
+                 lambda: c.attend(q, t, None), lambda: c.attend(q, t, z, window=-3),
+                 lambda: context.KV4Cache(c.codes[..., :16], c.scales).attend(q, t, z),
+                 lambda: context.verify_drafts(logits, ids, u, temperature=0.0),
+                 lambda: context.verify_drafts(logits, ids, u, vocab_size=51),
+                 lambda: context.verify_drafts(logits, ids[:, :1], u), lambda: context.verify_drafts(logits, ids, u[:, :2]),
+                 lambda: context.verify_drafts(logits, ids, u.double()), lambda: context.verify_drafts(logits, ids, u, logits),
+                 lambda: context.verify_drafts(logits, ids.float(), u)):
+        with pytest.raises((CapkError, ValueError)):
+            call()

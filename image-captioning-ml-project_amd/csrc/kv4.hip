@@ -175,6 +175,7 @@ extern "C" int capk_kv4_attention(int dtype, int B, int H, int Hk, int Nq, int h
   CAPK_CHECK_ARG(Nq >= 1 && Nq <= 64, "capk_kv4_attention: Nq=%d must be 1..64", Nq);
   CAPK_CHECK_ARG(B <= 65535 && Hk * (int64_t)cdiv((int64_t)Nq * (H / Hk), 16) <= 65535, "capk_kv4_attention: too many heads or sequences");
   CAPK_CHECK_ARG(window >= 0 && sinks >= 0, "capk_kv4_attention: window and sinks must not be negative");
+  CAPK_CHECK_ARG(scale > 0.f && scale < INFINITY, "capk_kv4_attention: scale must be positive");
   CAPK_CHECK_ARG(kv_len, "capk_kv4_attention: kv_len");
   StepArgs a = kv4_step(B, H, Hk, Nq, hd, scale, window, sinks, pages, page, table_cols);
   a.q = qv; a.o = ov; a.len = kv_len; a.lse = lse;

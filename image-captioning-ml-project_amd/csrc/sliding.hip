@@ -34,20 +34,21 @@ __device__ __forceinline__ int slide_len(const SlideArgs& a, int b) {
   return a.len ? min(max(a.len[b], 0), a.Nk) : a.Nk;
 }
 __device__ __forceinline__ bool slide_sees(const SlideArgs& a, int p, int j) {
-  return j <= p && (j < a.sinks || p - j < a.window);
+  return ((unsigned)(p - j) < (unsigned)a.window) | ((j < a.sinks) & (j <= p));  // (no branches: 32 of these per tile)
 }
 
-// KT rows of a [N, hd] head matrix into LDS (row stride ST), zeros where row_ok says no.
-template <typename T, int HDP, int KT, int ST, typename OK>
-__device__ __forceinline__ void slide_stage(T* img, const T* src, int64_t rs, int r0, int hd, OK row_ok) {
-  constexpr int C = HDP / 8;
-  for (int c = threadIdx.x; c < KT * C; c += 256) {
-    const int r = c / C, d = c % C * 8;
-    typename Tile<T>::V8 x = tile_zero8<T>();
-    if (d < hd && row_ok(r0 + r)) x = Tile<T>::load(src + (int64_t)(r0 + r) * rs + d);
-    *(typename Tile<T>::V8*)(img + r * ST + d) = x;
+// One-dimensional grids, key heads fastest: workgroups go round-robin over the 8 XCDs, so with B Hk a
+// multiple of 8 a key head's tiles run on one XCD and share its L2 (with 4, on two).  Long items first.
+struct SlideBlock {
+  int b, kvh, rest;
+  __device__ __forceinline__ explicit SlideBlock(const SlideArgs& a) {
+    const int i = blockIdx.x, n = a.B * a.Hk;
+    kvh = i % n % a.Hk;
+    b = i % n / a.Hk;
+    rest = i / n;
   }
-}
+};
+
 template <typename T, int HDP>
 __device__ __forceinline__ void slide_frags(typename Tile<T>::V8 (&f)[HDP / 16], const T* src, bool ok, int hd, int h) {
 #pragma unroll
@@ -56,8 +57,6 @@ __device__ __forceinline__ void slide_frags(typename Tile<T>::V8 (&f)[HDP / 16],
     if (ok && s * 16 + h * 8 < hd) f[s] = Tile<T>::load(src + s * 16 + h * 8);
   }
 }
-template <typename T> constexpr int slide_st(int hdp) { return hdp + 16 / (int)sizeof(T); }
-
 template <typename T, int HDP>
 __device__ __forceinline__ void slide_store(T* dst, const f32x16 (&acc)[HDP / 32], float f, int hd, int h) {
 #pragma unroll
@@ -70,71 +69,108 @@ __device__ __forceinline__ void slide_store(T* dst, const f32x16 (&acc)[HDP / 32
     }
 }
 
-// hidden keys of a 64-key tile, one bit each
-__device__ __forceinline__ uint64_t slide_hidden(const SlideArgs& a, int b, int j0, int len, int lane) {
-  const int j = j0 + lane;
-  return __builtin_amdgcn_ballot_w64(j >= len || (a.pad && a.pad[(int64_t)b * a.Nk + j]));
+// A tile of 64 keys of a workgroup's queries, in the double-buffered images (K, V): the next tile is on its
+// way from memory while this one is computed.
+template <typename T, int HDP> struct SlideKV {
+  using Img = TileImg<T, HDP>;
+  static constexpr int KT = 64, BUF = 2 * Img::bytes(KT);
+  const SlideArgs& a;
+  const T *k, *v;
+  int b, len, p_lo, p_hi, last, w, lane;
+  char* smem;
+  uint64_t hid;  // keys past the length or padded
+  __device__ __forceinline__ void fetch(int j0, int buf) const {
+    char* img = smem + buf * BUF;
+    Img::template dma<KT, 4>(img, k, a.k.rs, j0, last, a.hd, w, lane);
+    Img::template dma<KT, 4>(img + Img::bytes(KT), v, a.v.rs, j0, last, a.hd, w, lane);
+  }
+  // waits for the tile; keys that no query of the workgroup sees become zeros (they may hold anything)
+  __device__ __forceinline__ const char* arrive(int j0, int buf) {
+    char* img = smem + buf * BUF;
+    const int j = j0 + lane;
+    hid = __builtin_amdgcn_ballot_w64(j >= len || (a.pad && a.pad[(int64_t)b * a.Nk + j]));
+    const uint64_t out = hid | __builtin_amdgcn_ballot_w64(j > p_hi || (j >= a.sinks && p_lo - j >= a.window));
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (out) {
+      Img::clear(img, out);
+      Img::clear(img + Img::bytes(KT), out);
+      __syncthreads();
+    }
+    return img;
+  }
+};
+
+// which keys of a tile the 32 queries at pw_lo.. see: none, all, or some
+__device__ __forceinline__ bool slide_none(const SlideArgs& a, int j0, int pw_lo, int pw_hi) {
+  return j0 > pw_hi || (j0 >= a.sinks && pw_lo - (j0 + 63) >= a.window);
+}
+__device__ __forceinline__ bool slide_full(const SlideArgs& a, int j0, int pw_lo, int pw_hi, uint64_t hid) {
+  return hid == 0 && j0 + 63 <= pw_lo && (j0 + 64 <= a.sinks || pw_hi - j0 < a.window);
 }
 
 template <typename T, int HDP>
-__global__ __launch_bounds__(256) void slide_fwd(SlideArgs a) {
-  constexpr int KT = 64, ST = slide_st<T>(HDP), NS = HDP / 16, ND = HDP / 32;
+__global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void slide_fwd(SlideArgs a) {
+  using KV = SlideKV<T, HDP>;
+  using Img = typename KV::Img;
+  constexpr int NS = HDP / 16, ND = HDP / 32;
   extern __shared__ __align__(16) char smem[];
-  T* Ks = (T*)smem;
-  T* Vs = Ks + KT * ST;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, hh = lane >> 5;
-  const int h = blockIdx.y, b = blockIdx.z, kvh = h / (a.H / a.Hk), len = slide_len(a, b), off = len - a.Nq;
-  const int q0 = blockIdx.x * 128, qw = q0 + w * 32, qi = qw + (lane & 31), p = off + qi;
+  const SlideBlock at(a);
+  const int b = at.b, kvh = at.kvh, G = a.H / a.Hk, h = kvh * G + at.rest % G, len = slide_len(a, b), off = len - a.Nq;
+  const int q0 = ((a.Nq + 127) / 128 - 1 - at.rest / G) * 128, qw = q0 + w * 32, qi = qw + (lane & 31), p = off + qi;
   const int p_lo = off + q0, p_hi = off + min(q0 + 127, a.Nq - 1);
   const int pw_lo = off + qw, pw_hi = off + qw + 31;
   const float c = a.scale * kTileLog2e;
+  const SlideTiles<64> tiles(a.window, a.sinks, p_lo, p_hi, len);
+  KV kv{a, row<T>(a.k, b, 0, kvh), row<T>(a.v, b, 0, kvh), b, len, p_lo, p_hi, min(len, p_hi + 1) - 1, w, lane, smem, 0};
+  if (tiles.n) kv.fetch(tiles.key0(0), 0);
 
   typename Tile<T>::V8 qf[NS];
   slide_frags<T, HDP>(qf, row<T>(a.q, b, qi, h), qi < a.Nq, a.hd, hh);
   f32x16 o[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) o[d] = tile_zero<f32x16>();
-  float m = -INFINITY, l = 0.f;
-  const SlideTiles<KT> tiles(a.window, a.sinks, p_lo, p_hi, len);
-  auto ok = [&](int j) {
-    return j < len && j <= p_hi && (j < a.sinks || p_lo - j < a.window) && !(a.pad && a.pad[(int64_t)b * a.Nk + j]);
-  };
+  // mc: the exponent that the sums are relative to, the running maximum of c s or up to 8 below it (so
+  // that o is rescaled when the maximum has grown 2^8-fold, not with every step of it)
+  float mc = -INFINITY, l = 0.f;
   for (int t = 0; t < tiles.n; ++t) {
     const int j0 = tiles.key0(t);
-    __syncthreads();
-    slide_stage<T, HDP, KT, ST>(Ks, row<T>(a.k, b, 0, kvh), a.k.rs, j0, a.hd, ok);
-    slide_stage<T, HDP, KT, ST>(Vs, row<T>(a.v, b, 0, kvh), a.v.rs, j0, a.hd, ok);
-    __syncthreads();
-    if (j0 > pw_hi || (j0 >= a.sinks && pw_lo - (j0 + KT - 1) >= a.window)) continue;  // no key for this wave
-    const uint64_t hid = slide_hidden(a, b, j0, len, lane);
-    const bool full = hid == 0 && j0 + KT - 1 <= pw_lo && (j0 + KT <= a.sinks || pw_hi - j0 < a.window);
+    const char *ki = kv.arrive(j0, t & 1), *vi = ki + Img::bytes(64);
+    if (t + 1 < tiles.n) kv.fetch(tiles.key0(t + 1), (t + 1) & 1);
+    if (slide_none(a, j0, pw_lo, pw_hi)) continue;
     f32x16 s[2];
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
       s[kb] = tile_zero<f32x16>();
 #pragma unroll
-      for (int st = 0; st < NS; ++st)
-        s[kb] = Tile<T>::mma32(Tile<T>::load(Ks + (kb * 32 + (lane & 31)) * ST + st * 16 + hh * 8), qf[st], s[kb]);
+      for (int st = 0; st < NS; ++st) s[kb] = Tile<T>::mma32(Img::frag(ki, kb * 32, st, lane), qf[st], s[kb]);
+    }
+    if (!slide_full(a, j0, pw_lo, pw_hi, kv.hid)) {
+      const uint32_t hid[2] = {(uint32_t)kv.hid >> (4 * hh), (uint32_t)(kv.hid >> 32) >> (4 * hh)};
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int r = 8 * (i >> 2) + (i & 3);
+          const bool sees = slide_sees(a, p, j0 + kb * 32 + 4 * hh + r) & !(hid[kb] >> r & 1);
+          s[kb][i] = sees ? s[kb][i] : -INFINITY;
+        }
     }
     float mt = -INFINITY;
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
+    for (int i = 0; i < 16; ++i) mt = fmaxf(fmaxf(mt, s[0][i]), s[1][i]);
+    mt = fmaxf(mt, __shfl_xor(mt, 32, 64)) * c;
+    if (__builtin_amdgcn_ballot_w64(mt > mc + 8.f)) {
+      const float mn = fmaxf(mc, mt), alpha = mn == -INFINITY ? 1.f : tile_exp2(mc - mn);
+      mc = mn;
+      l *= alpha;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int jj = kb * 32 + 8 * (i >> 2) + 4 * hh + (i & 3);
-        float x = s[kb][i] * c;
-        if (!full && (((hid >> jj) & 1) || !slide_sees(a, p, j0 + jj))) x = -INFINITY;
-        s[kb][i] = x;
-        mt = fmaxf(mt, x);
-      }
-    mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
-    const float mn = fmaxf(m, mt), ms = mn == -INFINITY ? 0.f : mn, alpha = tile_exp2(m - ms);
-    m = mn;
-    l *= alpha;
+      for (int d = 0; d < ND; ++d)
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
+        for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
+    }
+    const float ms = mc == -INFINITY ? 0.f : mc;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -142,40 +178,49 @@ __global__ __launch_bounds__(256) void slide_fwd(SlideArgs a) {
         typename Tile<T>::V8 pf;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float x = tile_exp2(s[kb][st * 8 + e] - ms);
+          const float x = tile_exp2(fmaf(s[kb][st * 8 + e], c, -ms));
           l += x;
           pf[e] = (T)x;
         }
 #pragma unroll
-        for (int d = 0; d < ND; ++d)
-          o[d] = Tile<T>::mma32(tile_trans32(Vs, ST, kb * 32 + st * 16, d * 32, lane), pf, o[d]);
+        for (int d = 0; d < ND; ++d) o[d] = Tile<T>::mma32(Img::trans(vi, kb * 32 + st * 16, d * 32, lane), pf, o[d]);
       }
   }
   l += __shfl_xor(l, 32, 64);
   if (qi >= a.Nq) return;
   slide_store<T, HDP>(row<T>(a.o, b, qi, h), o, l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l), a.hd, hh);
   if (a.lse && hh == 0)
-    a.lse[((int64_t)b * a.H + h) * a.Nq + qi] = l > 0.f ? (m + __log2f(l)) * kTileLn2 : (l == 0.f ? -INFINITY : l);
+    a.lse[((int64_t)b * a.H + h) * a.Nq + qi] = l > 0.f ? (mc + __log2f(l)) * kTileLn2 : (l == 0.f ? -INFINITY : l);
 }
 
 template <typename T, int HDP>
-__global__ __launch_bounds__(256) void slide_dq(SlideArgs a) {
-  constexpr int KT = 64, ST = slide_st<T>(HDP), NS = HDP / 16, ND = HDP / 32;
+__global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void slide_dq(SlideArgs a) {
+  using KV = SlideKV<T, HDP>;
+  using Img = typename KV::Img;
+  constexpr int NS = HDP / 16, ND = HDP / 32;
   extern __shared__ __align__(16) char smem[];
-  T* Ks = (T*)smem;
-  T* Vs = Ks + KT * ST;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, hh = lane >> 5;
-  const int h = blockIdx.y, b = blockIdx.z, kvh = h / (a.H / a.Hk), len = slide_len(a, b), off = len - a.Nq;
-  const int q0 = blockIdx.x * 128, qw = q0 + w * 32, qi = qw + (lane & 31), p = off + qi;
+  const SlideBlock at(a);
+  const int b = at.b, kvh = at.kvh, G = a.H / a.Hk, h = kvh * G + at.rest % G, len = slide_len(a, b), off = len - a.Nq;
+  const int q0 = ((a.Nq + 127) / 128 - 1 - at.rest / G) * 128, qw = q0 + w * 32, qi = qw + (lane & 31), p = off + qi;
   const int p_lo = off + q0, p_hi = off + min(q0 + 127, a.Nq - 1);
   const int pw_lo = off + qw, pw_hi = off + qw + 31;
   const float c = a.scale * kTileLog2e;
+  const SlideTiles<64> tiles(a.window, a.sinks, p_lo, p_hi, len);
+  KV kv{a, row<T>(a.k, b, 0, kvh), row<T>(a.v, b, 0, kvh), b, len, p_lo, p_hi, min(len, p_hi + 1) - 1, w, lane, smem, 0};
+  if (tiles.n) kv.fetch(tiles.key0(0), 0);
 
   typename Tile<T>::V8 qf[NS], dof[NS];
   slide_frags<T, HDP>(qf, row<T>(a.q, b, qi, h), qi < a.Nq, a.hd, hh);
   slide_frags<T, HDP>(dof, row<T>(a.dout, b, qi, h), qi < a.Nq, a.hd, hh);
-  float delta = 0.f, lse2 = INFINITY;
-  {
+  const int64_t stat = ((int64_t)b * a.H + h) * a.Nq + qi;
+  const float lse2 = qi < a.Nq ? a.lse[stat] * kTileLog2e : INFINITY;
+  // D from the saved output costs a pass over one row, but inherits that output's rounding, which weighs
+  // where few keys share a row.  With at most 4 tiles of keys D is summed from P (do v^T) itself, in a
+  // walk of its own.
+  const bool walk = tiles.n <= 4;
+  float delta = 0.f;
+  if (!walk) {
     typename Tile<T>::V8 of[NS];
     slide_frags<T, HDP>(of, row<T>(a.o, b, qi, h), qi < a.Nq, a.hd, hh);
 #pragma unroll
@@ -183,82 +228,116 @@ __global__ __launch_bounds__(256) void slide_dq(SlideArgs a) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) delta = fmaf((float)of[s][e], (float)dof[s][e], delta);
     delta += __shfl_xor(delta, 32, 64);
-    if (qi < a.Nq) {
-      const int64_t at = ((int64_t)b * a.H + h) * a.Nq + qi;
-      lse2 = a.lse[at] * kTileLog2e;
-      if (hh == 0) a.delta[at] = delta;
-    }
   }
   f32x16 dq[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) dq[d] = tile_zero<f32x16>();
-  const SlideTiles<KT> tiles(a.window, a.sinks, p_lo, p_hi, len);
-  auto ok = [&](int j) {
-    return j < len && j <= p_hi && (j < a.sinks || p_lo - j < a.window) && !(a.pad && a.pad[(int64_t)b * a.Nk + j]);
-  };
-  for (int t = 0; t < tiles.n; ++t) {
-    const int j0 = tiles.key0(t);
-    __syncthreads();
-    slide_stage<T, HDP, KT, ST>(Ks, row<T>(a.k, b, 0, kvh), a.k.rs, j0, a.hd, ok);
-    slide_stage<T, HDP, KT, ST>(Vs, row<T>(a.v, b, 0, kvh), a.v.rs, j0, a.hd, ok);
-    __syncthreads();
-    if (j0 > pw_hi || (j0 >= a.sinks && pw_lo - (j0 + KT - 1) >= a.window)) continue;
-    const uint64_t hid = slide_hidden(a, b, j0, len, lane);
-    const bool full = hid == 0 && j0 + KT - 1 <= pw_lo && (j0 + KT <= a.sinks || pw_hi - j0 < a.window);
+  // P and do v^T of 32 keys of a tile, zeros where the query does not see the key
+  auto scores = [&](const char* ki, const char* vi, int j0, int kb, bool full, f32x16& s, f32x16& dp) {
+    s = dp = tile_zero<f32x16>();
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      f32x16 s = tile_zero<f32x16>(), dp = tile_zero<f32x16>();
+    for (int st = 0; st < NS; ++st) {
+      s = Tile<T>::mma32(Img::frag(ki, kb * 32, st, lane), qf[st], s);
+      dp = Tile<T>::mma32(Img::frag(vi, kb * 32, st, lane), dof[st], dp);
+    }
 #pragma unroll
-      for (int st = 0; st < NS; ++st) {
-        const int at = (kb * 32 + (lane & 31)) * ST + st * 16 + hh * 8;
-        s = Tile<T>::mma32(Tile<T>::load(Ks + at), qf[st], s);
-        dp = Tile<T>::mma32(Tile<T>::load(Vs + at), dof[st], dp);
-      }
+    for (int i = 0; i < 16; ++i) s[i] = tile_exp2(fmaf(s[i], c, -lse2));
+    if (!full) {
+      const uint32_t hid = (uint32_t)(kv.hid >> (32 * kb)) >> (4 * hh);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const int jj = kb * 32 + 8 * (i >> 2) + 4 * hh + (i & 3);
-        const float x = tile_exp2(fmaf(s[i], c, -lse2)) * (dp[i] - delta) * a.scale;
-        s[i] = !full && (((hid >> jj) & 1) || !slide_sees(a, p, j0 + jj)) ? 0.f : x;
+        const int r = 8 * (i >> 2) + (i & 3);
+        const bool sees = slide_sees(a, p, j0 + kb * 32 + 4 * hh + r) & !(hid >> r & 1);
+        s[i] = sees ? s[i] : 0.f;
+        dp[i] = sees ? dp[i] : 0.f;
       }
+    }
+  };
+  int buf = 0;
+  if (walk) {
+    for (int t = 0; t < tiles.n; ++t, buf ^= 1) {
+      const int j0 = tiles.key0(t);
+      const char *ki = kv.arrive(j0, buf), *vi = ki + Img::bytes(64);
+      kv.fetch(tiles.key0(t + 1 < tiles.n ? t + 1 : 0), buf ^ 1);
+      if (slide_none(a, j0, pw_lo, pw_hi)) continue;
+      const bool full = slide_full(a, j0, pw_lo, pw_hi, kv.hid);
+#pragma unroll 1
+      for (int kb = 0; kb < 2; ++kb) {
+        f32x16 s, dp;
+        scores(ki, vi, j0, kb, full, s, dp);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) delta = fmaf(s[i], dp[i], delta);
+      }
+    }
+    delta += __shfl_xor(delta, 32, 64);
+  }
+  for (int t = 0; t < tiles.n; ++t, buf ^= 1) {
+    const int j0 = tiles.key0(t);
+    const char *ki = kv.arrive(j0, buf), *vi = ki + Img::bytes(64);
+    if (t + 1 < tiles.n) kv.fetch(tiles.key0(t + 1), buf ^ 1);
+    if (slide_none(a, j0, pw_lo, pw_hi)) continue;
+    const bool full = slide_full(a, j0, pw_lo, pw_hi, kv.hid);
+#pragma unroll 1
+    for (int kb = 0; kb < 2; ++kb) {
+      f32x16 s, dp;
+      scores(ki, vi, j0, kb, full, s, dp);
 #pragma unroll
       for (int st = 0; st < 2; ++st) {
         typename Tile<T>::V8 df;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) df[e] = (T)s[st * 8 + e];
+        for (int e = 0; e < 8; ++e) df[e] = (T)(s[st * 8 + e] * (dp[st * 8 + e] - delta));
 #pragma unroll
-        for (int d = 0; d < ND; ++d)
-          dq[d] = Tile<T>::mma32(tile_trans32(Ks, ST, kb * 32 + st * 16, d * 32, lane), df, dq[d]);
+        for (int d = 0; d < ND; ++d) dq[d] = Tile<T>::mma32(Img::trans(ki, kb * 32 + st * 16, d * 32, lane), df, dq[d]);
       }
     }
   }
-  if (qi < a.Nq) slide_store<T, HDP>(row<T>(a.dq, b, qi, h), dq, 1.f, a.hd, hh);
+  if (qi >= a.Nq) return;
+  if (hh == 0) a.delta[stat] = delta;
+  slide_store<T, HDP>(row<T>(a.dq, b, qi, h), dq, a.scale, a.hd, hh);
 }
 
 // Keys [j0, j0 + 128) of a key head against queries [qa, qb) of its group; far = only the sinks among
 // the keys, at queries that no longer have them in their window.
 constexpr int kSlideKeys = 128;
 template <typename T, int HDP>
-__global__ __launch_bounds__(256) void slide_dkv(SlideArgs a) {
-  constexpr int QT = 64, ST = slide_st<T>(HDP), NS = HDP / 16, ND = HDP / 32;
+__global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void slide_dkv(SlideArgs a) {
+  using Img = TileImg<T, HDP>;
+  constexpr int QT = 64, NS = HDP / 16, ND = HDP / 32, BUF = 2 * Img::bytes(QT);
   extern __shared__ __align__(16) char smem[];
-  T* Qs = (T*)smem;
-  T* Ds = Qs + QT * ST;
-  float* Ls = (float*)(Ds + QT * ST);  // lse (base 2), then delta
+  float* Ls = (float*)(smem + 2 * BUF);  // per buffer: lse (base 2) and D of 64 queries
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, hh = lane >> 5;
-  const int kvh = blockIdx.y, b = blockIdx.z, G = a.H / a.Hk, len = slide_len(a, b), off = len - a.Nq;
+  const SlideBlock at(a);
+  const int b = at.b, kvh = at.kvh, G = a.H / a.Hk, len = slide_len(a, b), off = len - a.Nq;
   const int tiles = (a.Nk + kSlideKeys - 1) / kSlideKeys;
-  const bool far = (int)blockIdx.x >= tiles;
-  const int tile = far ? ((int)blockIdx.x - tiles) / a.far_chunks : (int)blockIdx.x;
-  const int chunk = far ? ((int)blockIdx.x - tiles) % a.far_chunks : a.far_chunks;
+  const bool far = at.rest >= tiles;
+  const int tile = far ? (at.rest - tiles) / a.far_chunks : at.rest;
+  const int chunk = far ? (at.rest - tiles) % a.far_chunks : a.far_chunks;
   const int j0 = tile * kSlideKeys, jw = j0 + w * 32, j = jw + (lane & 31);
   const bool key_ok = j < len && !(a.pad && a.pad[(int64_t)b * a.Nk + j]) && (!far || j < a.sinks);
-  // positions of the queries: near p in [j0, near_end), far p >= near_end in chunks of far_rows
-  const int64_t near_end = (int64_t)j0 + kSlideKeys - 1 + a.window;
+  // positions of the queries: near p in [j0, near_end), far p >= near_end in chunks of far_rows (no
+  // chunks: the owner of a tile with sinks walks all of them)
+  const int64_t near_end = tile < a.sink_tiles && a.far_chunks == 0 ? (int64_t)1 << 40 : (int64_t)j0 + kSlideKeys - 1 + a.window;
   const int qn = (int)min((int64_t)a.Nq, max((int64_t)0, near_end - off));
   const int qa = far ? qn + chunk * a.far_rows : max(0, j0 - off);
   const int qb = far ? min(a.Nq, qa + a.far_rows) : (j0 < len ? qn : 0);
   const float c = a.scale * kTileLog2e;
+  const int nq = qb > qa ? (qb - qa + QT - 1) / QT : 0, all = nq * G;
 
+  // the tile of 64 queries t: head kvh G + t / nq, queries qa + 64 (t % nq)
+  float ld = 0.f;  // threads 0..63 carry lse, 64..127 D
+  auto fetch = [&](int t, int buf) {
+    const int h = kvh * G + t / nq, q0 = qa + t % nq * QT;
+    char* img = smem + buf * BUF;
+    Img::template dma<QT, 4>(img, row<T>(a.q, b, 0, h), a.q.rs, q0, qb - 1, a.hd, w, lane);
+    Img::template dma<QT, 4>(img + Img::bytes(QT), row<T>(a.dout, b, 0, h), a.dout.rs, q0, qb - 1, a.hd, w, lane);
+    if (threadIdx.x < 128) {
+      const int q = q0 + (threadIdx.x & 63);
+      const int64_t at = ((int64_t)b * a.H + h) * a.Nq + q;
+      ld = threadIdx.x < 64 ? INFINITY : 0.f;
+      if (q < qb) ld = threadIdx.x < 64 ? a.lse[at] * kTileLog2e : a.delta[at];
+    }
+  };
+  if (all) fetch(0, 0);
   typename Tile<T>::V8 kf[NS], vf[NS];
   slide_frags<T, HDP>(kf, row<T>(a.k, b, j, kvh), key_ok, a.hd, hh);
   slide_frags<T, HDP>(vf, row<T>(a.v, b, j, kvh), key_ok, a.hd, hh);
@@ -266,67 +345,67 @@ __global__ __launch_bounds__(256) void slide_dkv(SlideArgs a) {
   f32x16 dk[ND], dv[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) dk[d] = dv[d] = tile_zero<f32x16>();
-  for (int g = 0; g < G; ++g) {
-    const int h = kvh * G + g;
-    for (int q0 = qa; q0 < qb; q0 += QT) {
-      auto ok = [&](int q) { return q < qb; };
-      __syncthreads();
-      slide_stage<T, HDP, QT, ST>(Qs, row<T>(a.q, b, 0, h), a.q.rs, q0, a.hd, ok);
-      slide_stage<T, HDP, QT, ST>(Ds, row<T>(a.dout, b, 0, h), a.dout.rs, q0, a.hd, ok);
-      if (threadIdx.x < QT) {
-        const int q = q0 + threadIdx.x;
-        const int64_t at = ((int64_t)b * a.H + h) * a.Nq + q;
-        Ls[threadIdx.x] = q < qb ? a.lse[at] * kTileLog2e : INFINITY;
-        Ls[QT + threadIdx.x] = q < qb ? a.delta[at] : 0.f;
+  for (int t = 0; t < all; ++t) {
+    const char *qi = smem + (t & 1) * BUF, *di = qi + Img::bytes(QT);
+    const float* ls = Ls + (t & 1) * 128;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (threadIdx.x < 128) Ls[(t & 1) * 128 + threadIdx.x] = ld;
+    __syncthreads();
+    if (t + 1 < all) fetch(t + 1, (t + 1) & 1);
+    const int q0 = qa + t % nq * QT, p0 = off + q0;
+    // no query of this tile sees a key of this wave
+    if (p0 + QT - 1 < jw || (jw >= a.sinks && p0 - (jw + 31) >= a.window)) continue;
+    const bool full = !hidden && q0 + QT <= qb && jw + 31 <= p0 && (jw + 32 <= a.sinks || p0 + QT - 1 - jw < a.window);
+#pragma unroll 1
+    for (int qt = 0; qt < 2; ++qt) {
+      f32x16 s = tile_zero<f32x16>(), dp = tile_zero<f32x16>();
+#pragma unroll
+      for (int st = 0; st < NS; ++st) {
+        s = Tile<T>::mma32(Img::frag(qi, qt * 32, st, lane), kf[st], s);
+        dp = Tile<T>::mma32(Img::frag(di, qt * 32, st, lane), vf[st], dp);
       }
-      __syncthreads();
-      const int p0 = off + q0;
-      // no query of this tile sees a key of this wave
-      if (p0 + QT - 1 < jw || (jw >= a.sinks && p0 - (jw + 31) >= a.window)) continue;
-      const bool full = !hidden && q0 + QT <= qb && jw + 31 <= p0 && (jw + 32 <= a.sinks || p0 + QT - 1 - jw < a.window);
 #pragma unroll
-      for (int qt = 0; qt < 2; ++qt) {
-        f32x16 s = tile_zero<f32x16>(), dp = tile_zero<f32x16>();
+      for (int i4 = 0; i4 < 4; ++i4) {
+        const int r = qt * 32 + 8 * i4 + 4 * hh;
+        const f32x4 lv = *(const f32x4*)(ls + r), dl = *(const f32x4*)(ls + 64 + r);
 #pragma unroll
-        for (int st = 0; st < NS; ++st) {
-          const int at = (qt * 32 + (lane & 31)) * ST + st * 16 + hh * 8;
-          s = Tile<T>::mma32(Tile<T>::load(Qs + at), kf[st], s);
-          dp = Tile<T>::mma32(Tile<T>::load(Ds + at), vf[st], dp);
+        for (int e = 0; e < 4; ++e) {
+          const int i = 4 * i4 + e;
+          const float x = tile_exp2(fmaf(s[i], c, -lv[e]));
+          s[i] = x;
+          dp[i] = x * (dp[i] - dl[e]);
         }
+      }
+      if (!full) {
 #pragma unroll
-        for (int i4 = 0; i4 < 4; ++i4) {
-          const int r = qt * 32 + 8 * i4 + 4 * hh;
-          const f32x4 ls = *(const f32x4*)(Ls + r), dl = *(const f32x4*)(Ls + QT + r);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int i = 4 * i4 + e;
-            float x = tile_exp2(fmaf(s[i], c, -ls[e])), y = x * (dp[i] - dl[e]) * a.scale;
-            if (!full && (!key_ok || q0 + r + e >= qb || !slide_sees(a, p0 + r + e, j))) x = y = 0.f;
-            s[i] = x;
-            dp[i] = y;
-          }
+        for (int i = 0; i < 16; ++i) {
+          const int r = qt * 32 + 8 * (i >> 2) + 4 * hh + (i & 3);
+          const bool sees = key_ok & (q0 + r < qb) & slide_sees(a, p0 + r, j);
+          s[i] = sees ? s[i] : 0.f;
+          dp[i] = sees ? dp[i] : 0.f;
         }
+      }
 #pragma unroll
-        for (int st = 0; st < 2; ++st) {
-          typename Tile<T>::V8 pf, df;
+      for (int st = 0; st < 2; ++st) {
+        typename Tile<T>::V8 pf, df;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) { pf[e] = (T)s[st * 8 + e]; df[e] = (T)dp[st * 8 + e]; }
+        for (int e = 0; e < 8; ++e) { pf[e] = (T)s[st * 8 + e]; df[e] = (T)dp[st * 8 + e]; }
 #pragma unroll
-          for (int d = 0; d < ND; ++d) {
-            dv[d] = Tile<T>::mma32(tile_trans32(Ds, ST, qt * 32 + st * 16, d * 32, lane), pf, dv[d]);
-            dk[d] = Tile<T>::mma32(tile_trans32(Qs, ST, qt * 32 + st * 16, d * 32, lane), df, dk[d]);
-          }
+        for (int d = 0; d < ND; ++d) {
+          dv[d] = Tile<T>::mma32(Img::trans(di, qt * 32 + st * 16, d * 32, lane), pf, dv[d]);
+          dk[d] = Tile<T>::mma32(Img::trans(qi, qt * 32 + st * 16, d * 32, lane), df, dk[d]);
         }
       }
     }
   }
+  if (far && j >= a.sinks) return;
   if (tile < a.sink_tiles && a.far_chunks > 0) {  // [B, Hk, sink tile, chunk][dK, dV][128][hd]
     float* dst = a.part + ((((int64_t)b * a.Hk + kvh) * a.sink_tiles + tile) * (a.far_chunks + 1) + chunk) * 2 *
                               kSlideKeys * a.hd + (int64_t)(w * 32 + (lane & 31)) * a.hd;
-    slide_store<float, HDP>(dst, dk, 1.f, a.hd, hh);
+    slide_store<float, HDP>(dst, dk, a.scale, a.hd, hh);
     slide_store<float, HDP>(dst + (int64_t)kSlideKeys * a.hd, dv, 1.f, a.hd, hh);
   } else if (j < a.Nk) {
-    slide_store<T, HDP>(row<T>(a.dk, b, j, kvh), dk, 1.f, a.hd, hh);
+    slide_store<T, HDP>(row<T>(a.dk, b, j, kvh), dk, a.scale, a.hd, hh);
     slide_store<T, HDP>(row<T>(a.dv, b, j, kvh), dv, 1.f, a.hd, hh);
   }
 }
@@ -342,7 +421,7 @@ __global__ __launch_bounds__(256) void slide_dkv_sum(SlideArgs a) {
   const float* src = a.part + (((int64_t)blockIdx.z * a.Hk + blockIdx.y) * a.sink_tiles + tile) * (a.far_chunks + 1) * 2 *
                                   kSlideKeys * a.hd + (int64_t)which * kSlideKeys * a.hd + e;
   f32x4 s = {0.f, 0.f, 0.f, 0.f};
-  for (int c = 0; c <= a.far_chunks; ++c) s += *(const f32x4*)(src + (int64_t)c * 2 * kSlideKeys * a.hd);
+  for (int c = j < a.sinks ? 0 : a.far_chunks; c <= a.far_chunks; ++c) s += *(const f32x4*)(src + (int64_t)c * 2 * kSlideKeys * a.hd);
   Tile<T>::store4(row<T>(which ? a.dv : a.dk, blockIdx.z, j, blockIdx.y) + e % a.hd, s);
 }
 
@@ -358,12 +437,14 @@ static int slide_launch(K kernel, dim3 grid, size_t shm, hipStream_t st, const S
 }
 
 static int slide_check(const char* who, int dtype, int B, int H, int Hk, int Nq, int Nk, int hd, int window, int sinks,
-                       const SlideView* v, int n) {
+                       float scale, const SlideView* v, int n) {
   CAPK_CHECK_ARG(dtype == CAPK_F32 || dtype == CAPK_BF16, "%s: dtype", who);
   CAPK_CHECK_ARG(B >= 1 && B <= 65535 && Nq >= 1 && Nk >= 1 && Nq <= (1 << 28) && Nk <= (1 << 28), "%s: bad sizes", who);
   CAPK_CHECK_ARG(Hk >= 1 && H >= Hk && H % Hk == 0 && H <= 65535, "%s: %d query heads over %d key heads", who, H, Hk);
   CAPK_CHECK_ARG(hd >= 8 && hd % 8 == 0 && hd <= 128, "%s: hd=%d must be a multiple of 8, <= 128", who, hd);
   CAPK_CHECK_ARG(window >= 0 && sinks >= 0, "%s: window and sinks must not be negative", who);
+  CAPK_CHECK_ARG((int64_t)B * H * (cdiv(Nq, 128) + 2 * (int64_t)cdiv(Nk, 128)) < (1 << 30), "%s: too many tiles", who);
+  CAPK_CHECK_ARG(scale > 0.f && scale < INFINITY, "%s: scale must be positive", who);
   const int ea = dtype == CAPK_BF16 ? 8 : 4;
   for (int i = 0; i < n; ++i)
     CAPK_CHECK_ARG(v[i].p && (uintptr_t)v[i].p % 16 == 0 && v[i].bs % ea == 0 && v[i].rs % ea == 0 && v[i].hs % ea == 0,
@@ -382,15 +463,27 @@ static SlideArgs slide_args(int B, int H, int Hk, int Nq, int Nk, int hd, float 
   return a;
 }
 
-// The far queries of the sink tiles: chunks of about a window (at least 512), so that no owner of a
-// chunk works much longer than the owner of an ordinary key tile.
+// The far queries of the sink tiles.  An item's length is its 64-query tiles; the launch runs about
+// `slots` workgroups at a time.  Where even the longest item (a sink tile with every query) is within
+// a slot's share of the whole, each sink tile has one owner; else its far queries go in chunks of a
+// quarter of that share (at least 256 queries, at most an ordinary tile's).  Measured at N = 16384,
+// window 1024, 4 sinks, 4 key heads: see slide_dkv.
 static void slide_far(SlideArgs& a) {
+  const int64_t slots = 512, G = a.H / a.Hk;
   a.sink_tiles = cdiv(a.sinks, kSlideKeys);
-  a.far_rows = a.window + kSlideKeys > 512 ? (a.window + kSlideKeys + 63) / 64 * 64 : 512;
   // the first sink tile has the most far queries: positions from 127 + window on
-  const int64_t most = (int64_t)a.Nk - (kSlideKeys - 1) - a.window;
-  const int64_t rows = most < a.Nq ? most : a.Nq;
-  a.far_chunks = a.sink_tiles && rows > 0 ? cdiv(rows, a.far_rows) : 0;
+  const int64_t most = (int64_t)a.Nk - (kSlideKeys - 1) - a.window, rows = most < a.Nq ? most : a.Nq;
+  a.far_rows = a.far_chunks = 0;
+  if (!a.sink_tiles || rows <= 0) return;
+  const int64_t near = cdiv(a.window + kSlideKeys < a.Nq ? a.window + kSlideKeys : a.Nq, 64) * G, far = cdiv(rows, 64) * G;
+  const int64_t share = a.B * (int64_t)a.Hk * (cdiv(a.Nk, kSlideKeys) * near + a.sink_tiles * far) / slots;
+  if (near + far <= share) return;
+  int64_t n = share / 4 / G * 64;
+  const int64_t top = (a.window + kSlideKeys + 63) / 64 * 64;
+  if (n > top) n = top;
+  if (n < 256) n = 256;
+  a.far_rows = (int)n;
+  a.far_chunks = cdiv(rows, n);
 }
 
 }  // namespace capk
@@ -423,17 +516,17 @@ extern "C" int capk_sliding_attention_fwd(int dtype, int B, int H, int Hk, int N
                                           void* stream) {
   const SlideView vs[] = {{(void*)q, q_bs, q_rs, q_hs}, {(void*)k, k_bs, k_rs, k_hs}, {(void*)v, v_bs, v_rs, v_hs},
                           {o, o_bs, o_rs, o_hs}};
-  int rc = slide_check("capk_sliding_attention_fwd", dtype, B, H, Hk, Nq, Nk, hd, window, sinks, vs, 4);
+  int rc = slide_check("capk_sliding_attention_fwd", dtype, B, H, Hk, Nq, Nk, hd, window, sinks, scale, vs, 4);
   if (rc) return rc;
   SlideArgs a = slide_args(B, H, Hk, Nq, Nk, hd, scale, window, sinks, key_pad, kv_len);
   a.q = vs[0]; a.k = vs[1]; a.v = vs[2]; a.o = vs[3]; a.lse = lse;
   if (slide_few(Nq)) return step_launch(dtype, slide_step(a), ws, ws_bytes, S(stream));
   const int hdp = slide_hdp(hd);
-  const dim3 grid(cdiv(Nq, 128), H, B);
+  const dim3 grid(cdiv(Nq, 128) * H * B);
   SLIDE_HD(hdp, {
     if (dtype == CAPK_BF16)
-      return slide_launch(slide_fwd<bf16, HDP>, grid, 2 * 64 * slide_st<bf16>(HDP) * 2, S(stream), a, "slide_fwd");
-    return slide_launch(slide_fwd<float, HDP>, grid, 2 * 64 * slide_st<float>(HDP) * 4, S(stream), a, "slide_fwd");
+      return slide_launch(slide_fwd<bf16, HDP>, grid, 2 * SlideKV<bf16, HDP>::BUF, S(stream), a, "slide_fwd");
+    return slide_launch(slide_fwd<float, HDP>, grid, 2 * SlideKV<float, HDP>::BUF, S(stream), a, "slide_fwd");
   });
 }
 
@@ -459,7 +552,7 @@ extern "C" int capk_sliding_attention_bwd(int dtype, int B, int H, int Hk, int N
   const SlideView vs[] = {{(void*)q, q_bs, q_rs, q_hs}, {(void*)k, k_bs, k_rs, k_hs}, {(void*)v, v_bs, v_rs, v_hs},
                           {(void*)o, o_bs, o_rs, o_hs}, {(void*)dout, do_bs, do_rs, do_hs}, {dq, dq_bs, dq_rs, dq_hs},
                           {dk, dk_bs, dk_rs, dk_hs}, {dv, dv_bs, dv_rs, dv_hs}};
-  int rc = slide_check("capk_sliding_attention_bwd", dtype, B, H, Hk, Nq, Nk, hd, window, sinks, vs, 8);
+  int rc = slide_check("capk_sliding_attention_bwd", dtype, B, H, Hk, Nq, Nk, hd, window, sinks, scale, vs, 8);
   if (rc) return rc;
   const size_t need = capk_sliding_attention_bwd_workspace(B, H, Hk, Nq, Nk, hd, window, sinks);
   CAPK_CHECK_ARG(lse && ws && ws_bytes >= need && (uintptr_t)ws % 16 == 0,
@@ -471,17 +564,17 @@ extern "C" int capk_sliding_attention_bwd(int dtype, int B, int H, int Hk, int N
   a.delta = (float*)ws;
   a.part = (float*)((char*)ws + ((size_t)B * H * Nq * 4 + 15) / 16 * 16);
   const int hdp = slide_hdp(hd), es = dtype == CAPK_BF16 ? 2 : 4;
-  const dim3 gq(cdiv(Nq, 128), H, B), gk(cdiv(Nk, kSlideKeys) + a.sink_tiles * a.far_chunks, Hk, B);
+  const dim3 gq(cdiv(Nq, 128) * H * B), gk((cdiv(Nk, kSlideKeys) + a.sink_tiles * a.far_chunks) * Hk * B);
   hipStream_t st = S(stream);
   SLIDE_HD(hdp, {
     if (dtype == CAPK_BF16) {
-      const size_t shm = 2 * 64 * slide_st<bf16>(HDP) * 2;
+      const size_t shm = 2 * SlideKV<bf16, HDP>::BUF;
       if ((rc = slide_launch(slide_dq<bf16, HDP>, gq, shm, st, a, "slide_dq"))) return rc;
-      if ((rc = slide_launch(slide_dkv<bf16, HDP>, gk, shm + 512, st, a, "slide_dkv"))) return rc;
+      if ((rc = slide_launch(slide_dkv<bf16, HDP>, gk, shm + 1024, st, a, "slide_dkv"))) return rc;
     } else {
-      const size_t shm = 2 * 64 * slide_st<float>(HDP) * 4;
+      const size_t shm = 2 * SlideKV<float, HDP>::BUF;
       if ((rc = slide_launch(slide_dq<float, HDP>, gq, shm, st, a, "slide_dq"))) return rc;
-      if ((rc = slide_launch(slide_dkv<float, HDP>, gk, shm + 512, st, a, "slide_dkv"))) return rc;
+      if ((rc = slide_launch(slide_dkv<float, HDP>, gk, shm + 1024, st, a, "slide_dkv"))) return rc;
     }
   });
   if (a.far_chunks) {

@@ -62,25 +62,86 @@ template <typename V> __device__ __forceinline__ V tile_zero() {
   return z;
 }
 
-// A fragment of the transpose of a row-major LDS image for a 32-deep-row product: lane column
-// c0 + (l & 31), slot (h, e) = image row r0 + 8 (e >> 2) + 4 h + (e & 3) -- the row order in which
-// eight accumulator registers of a 32x32 product hold their rows.
-__device__ __forceinline__ bf16x8 tile_trans32(const bf16* img, int st, int r0, int c0, int lane) {
-  const int i16 = lane & 15;
-  const bf16* a = img + (r0 + 4 * (lane >> 5) + (i16 >> 2)) * st + c0 + 16 * ((lane >> 4) & 1) + 4 * (i16 & 3);
-  const bf16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, a));
-  const bf16x4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, a + 8 * st));
-  return (bf16x8){x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
-}
-__device__ __forceinline__ f32x8 tile_trans32(const float* img, int st, int r0, int c0, int lane) {
-  const float* a = img + (r0 + 4 * (lane >> 5)) * st + c0 + (lane & 31);
-  f32x8 r;
+// An LDS image of a [rows][HDP] matrix: unpadded rows of 16-B chunks, chunk c of row r stored at chunk
+// c ^ swz(r).  The masks put the 16 lanes that a b128 read serves together ({0-3, 12-15, 20-27} and so on:
+// one chunk of 16 rows) and the 32 lanes of a transposed b64 read (four chunks of 4 rows) on distinct
+// banks, and leave whole 1-KiB pieces contiguous, as the copy straight from memory needs them.
+template <typename T, int HDP> struct TileImg {
+  static constexpr int RB = HDP * (int)sizeof(T), PER = 16 / (int)sizeof(T);  // bytes of a row, elements of a chunk
+  __device__ __forceinline__ static int swz(int r) {
+    if constexpr (sizeof(T) == 2) {
+      if constexpr (HDP == 128) return (r & 3) << 2 | ((r >> 2) & 3);
+      else if constexpr (HDP == 64) return ((r >> 1) & 1) << 2 | ((r >> 2) & 3);
+      else return (r >> 2) & 3;
+    } else {
+      if constexpr (RB % 256 == 0) return r & 15;
+      else return (r >> 1) & 7;
+    }
+  }
+  static constexpr int bytes(int rows) { return rows * RB; }
+
+  // Copies rows r0 .. r0 + ROWS - 1 of `src` (row stride rs) into the image, 1 KiB per wave and
+  // instruction; rows past `last` repeat it, columns past hd repeat column 0.  Arrives with vmcnt(0).
+  template <int ROWS, int WAVES>
+  __device__ __forceinline__ static void dma(char* img, const T* src, int64_t rs, int r0, int last, int hd, int w, int lane) {
+    static_assert(ROWS * RB % (1024 * WAVES) == 0, "whole pieces for every wave");
+    constexpr int STEP = 1024 * WAVES / RB;  // rows from one piece of a wave to its next
+    const int o = w * 1024 + lane * 16, r = o / RB, c = (o % RB / 16) ^ swz(r), col = c * PER < hd ? c * PER : 0;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) r[e] = a[(8 * (e >> 2) + (e & 3)) * st];
-  return r;
-}
-// The same for a 16x16 product over 32 image rows: lane column c0 + (l & 15), slot (g, e) = image row
-// r0 + 16 (e >> 2) + 4 g + (e & 3), the row order of two 16x16 accumulators.
+    for (int i = 0; i < ROWS * RB / 1024 / WAVES; ++i) {
+      int ri = r + i * STEP, ci = col;
+      if constexpr (1024 * WAVES % RB != 0 || STEP % 16 != 0) {  // the mask changes from piece to piece
+        const int oi = o + i * 1024 * WAVES;
+        ri = oi / RB;
+        ci = ((oi % RB / 16) ^ swz(ri)) * PER;
+        ci = ci < hd ? ci : 0;
+      }
+      __builtin_amdgcn_global_load_lds((const void*)(src + (int64_t)min(r0 + ri, last) * rs + ci),
+                                       (__attribute__((address_space(3))) void*)(img + (i * WAVES + w) * 1024), 16, 0, 0);
+    }
+  }
+  // zeros in the rows whose bit of `rows` is set (all 256 threads)
+  __device__ __forceinline__ static void clear(char* img, uint64_t rows) {
+    for (int o = threadIdx.x * 16; o < 64 * RB; o += 256 * 16)
+      if (rows >> (o / RB) & 1) *(f32x4*)(img + o) = (f32x4){0.f, 0.f, 0.f, 0.f};
+  }
+  // A / B fragment of a 32x32 product: row r0 + (l & 31), columns 16 s + 8 h (r0 a multiple of 32)
+  __device__ __forceinline__ static typename Tile<T>::V8 frag(const char* img, int r0, int s, int lane) {
+    const int r = lane & 31, f = swz(r), c = (2 * s + (lane >> 5)) * 8 / PER;
+    const char* at = img + (r0 + r) * RB;
+    if constexpr (sizeof(T) == 2) return *(const bf16x8*)(at + ((c ^ f) << 4));
+    else {
+      const f32x4 x = *(const f32x4*)(at + ((c ^ f) << 4)), y = *(const f32x4*)(at + (((c + 1) ^ f) << 4));
+      return (f32x8){x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+    }
+  }
+  // A fragment of the transpose for a 32x32 product: lane column c0 + (l & 31), slot (h, e) = row
+  // r0 + 8 (e >> 2) + 4 h + (e & 3) -- the order in which eight accumulator registers of a 32x32
+  // product hold their rows (r0 a multiple of 16, c0 of 32).
+  __device__ __forceinline__ static typename Tile<T>::V8 trans(const char* img, int r0, int c0, int lane) {
+    const int h = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+      const int i16 = lane & 15, r = 4 * h + (i16 >> 2), c = c0 / 8 + 2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1);
+      const char *a = img + (r0 + r) * RB + ((c ^ swz(r)) << 4) + (i16 & 1) * 8,
+                 *b = img + (r0 + 8 + r) * RB + ((c ^ swz(r + 8)) << 4) + (i16 & 1) * 8;
+      const bf16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, a));
+      const bf16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, b));
+      return (bf16x8){x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+    } else {
+      const int d = c0 + (lane & 31);
+      f32x8 v;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int r = 8 * (e >> 2) + 4 * h + (e & 3);
+        v[e] = *(const float*)(img + (r0 + r) * RB + (((d / 4) ^ swz(r)) << 4) + (d & 3) * 4);
+      }
+      return v;
+    }
+  }
+};
+// A fragment of the transpose of a row-major LDS image (row stride st) for a 16x16 product over 32 rows:
+// lane column c0 + (l & 15), slot (g, e) = row r0 + 16 (e >> 2) + 4 g + (e & 3), the row order of two
+// 16x16 accumulators.
 __device__ __forceinline__ bf16x8 tile_trans16(const bf16* img, int st, int r0, int c0, int lane) {
   const int i16 = lane & 15;
   const bf16* a = img + (r0 + 4 * (lane >> 4) + (i16 >> 2)) * st + c0 + 4 * (i16 & 3);

@@ -122,6 +122,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void s
   const int p_lo = off + q0, p_hi = off + min(q0 + 127, a.Nq - 1);
   const int pw_lo = off + qw, pw_hi = off + qw + 31;
   const float c = a.scale * kTileLog2e;
+  typename Img::Lane ln(lane);
   const SlideTiles<64> tiles(a.window, a.sinks, p_lo, p_hi, len);
   KV kv{a, row<T>(a.k, b, 0, kvh), row<T>(a.v, b, 0, kvh), b, len, p_lo, p_hi, min(len, p_hi + 1) - 1, w, lane, smem, 0};
   if (tiles.n) kv.fetch(tiles.key0(0), 0);
@@ -144,7 +145,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void s
     for (int kb = 0; kb < 2; ++kb) {
       s[kb] = tile_zero<f32x16>();
 #pragma unroll
-      for (int st = 0; st < NS; ++st) s[kb] = Tile<T>::mma32(Img::frag(ki, kb * 32, st, lane), qf[st], s[kb]);
+      for (int st = 0; st < NS; ++st) s[kb] = Tile<T>::mma32(Img::frag(ki, kb * 32, st, ln), qf[st], s[kb]);
     }
     if (!slide_full(a, j0, pw_lo, pw_hi, kv.hid)) {
       const uint32_t hid[2] = {(uint32_t)kv.hid >> (4 * hh), (uint32_t)(kv.hid >> 32) >> (4 * hh)};
@@ -183,7 +184,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void s
           pf[e] = (T)x;
         }
 #pragma unroll
-        for (int d = 0; d < ND; ++d) o[d] = Tile<T>::mma32(Img::trans(vi, kb * 32 + st * 16, d * 32, lane), pf, o[d]);
+        for (int d = 0; d < ND; ++d) o[d] = Tile<T>::mma32(Img::trans(vi, kb * 32 + st * 16, d * 32, ln), pf, o[d]);
       }
   }
   l += __shfl_xor(l, 32, 64);
@@ -206,6 +207,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void s
   const int p_lo = off + q0, p_hi = off + min(q0 + 127, a.Nq - 1);
   const int pw_lo = off + qw, pw_hi = off + qw + 31;
   const float c = a.scale * kTileLog2e;
+  typename Img::Lane ln(lane);
   const SlideTiles<64> tiles(a.window, a.sinks, p_lo, p_hi, len);
   KV kv{a, row<T>(a.k, b, 0, kvh), row<T>(a.v, b, 0, kvh), b, len, p_lo, p_hi, min(len, p_hi + 1) - 1, w, lane, smem, 0};
   if (tiles.n) kv.fetch(tiles.key0(0), 0);
@@ -237,8 +239,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void s
     s = dp = tile_zero<f32x16>();
 #pragma unroll
     for (int st = 0; st < NS; ++st) {
-      s = Tile<T>::mma32(Img::frag(ki, kb * 32, st, lane), qf[st], s);
-      dp = Tile<T>::mma32(Img::frag(vi, kb * 32, st, lane), dof[st], dp);
+      s = Tile<T>::mma32(Img::frag(ki, kb * 32, st, ln), qf[st], s);
+      dp = Tile<T>::mma32(Img::frag(vi, kb * 32, st, ln), dof[st], dp);
     }
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = tile_exp2(fmaf(s[i], c, -lse2));
@@ -287,7 +289,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void s
 #pragma unroll
         for (int e = 0; e < 8; ++e) df[e] = (T)(s[st * 8 + e] * (dp[st * 8 + e] - delta));
 #pragma unroll
-        for (int d = 0; d < ND; ++d) dq[d] = Tile<T>::mma32(Img::trans(ki, kb * 32 + st * 16, d * 32, lane), df, dq[d]);
+        for (int d = 0; d < ND; ++d) dq[d] = Tile<T>::mma32(Img::trans(ki, kb * 32 + st * 16, d * 32, ln), df, dq[d]);
       }
     }
   }
@@ -321,21 +323,18 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void s
   const int qa = far ? qn + chunk * a.far_rows : max(0, j0 - off);
   const int qb = far ? min(a.Nq, qa + a.far_rows) : (j0 < len ? qn : 0);
   const float c = a.scale * kTileLog2e;
+  typename Img::Lane ln(lane);
   const int nq = qb > qa ? (qb - qa + QT - 1) / QT : 0, all = nq * G;
 
   // the tile of 64 queries t: head kvh G + t / nq, queries qa + 64 (t % nq)
-  float ld = 0.f;  // threads 0..63 carry lse, 64..127 D
+  const float* stat = (threadIdx.x & 64 ? a.delta : a.lse) + (int64_t)b * a.H * a.Nq;
+  float ld = 0.f;  // threads 0..63 carry lse, 64..127 D (unconditional loads: nothing waits for them here)
   auto fetch = [&](int t, int buf) {
     const int h = kvh * G + t / nq, q0 = qa + t % nq * QT;
     char* img = smem + buf * BUF;
     Img::template dma<QT, 4>(img, row<T>(a.q, b, 0, h), a.q.rs, q0, qb - 1, a.hd, w, lane);
     Img::template dma<QT, 4>(img + Img::bytes(QT), row<T>(a.dout, b, 0, h), a.dout.rs, q0, qb - 1, a.hd, w, lane);
-    if (threadIdx.x < 128) {
-      const int q = q0 + (threadIdx.x & 63);
-      const int64_t at = ((int64_t)b * a.H + h) * a.Nq + q;
-      ld = threadIdx.x < 64 ? INFINITY : 0.f;
-      if (q < qb) ld = threadIdx.x < 64 ? a.lse[at] * kTileLog2e : a.delta[at];
-    }
+    ld = stat[(int64_t)h * a.Nq + min(q0 + lane, qb - 1)];
   };
   if (all) fetch(0, 0);
   typename Tile<T>::V8 kf[NS], vf[NS];
@@ -349,20 +348,21 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void s
     const char *qi = smem + (t & 1) * BUF, *di = qi + Img::bytes(QT);
     const float* ls = Ls + (t & 1) * 128;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if (threadIdx.x < 128) Ls[(t & 1) * 128 + threadIdx.x] = ld;
+    const int q0 = qa + t % nq * QT, p0 = off + q0;
+    if (w < 2) Ls[(t & 1) * 128 + threadIdx.x] = q0 + lane >= qb ? (w ? 0.f : INFINITY) : (w ? ld : ld * kTileLog2e);
     __syncthreads();
     if (t + 1 < all) fetch(t + 1, (t + 1) & 1);
-    const int q0 = qa + t % nq * QT, p0 = off + q0;
     // no query of this tile sees a key of this wave
     if (p0 + QT - 1 < jw || (jw >= a.sinks && p0 - (jw + 31) >= a.window)) continue;
     const bool full = !hidden && q0 + QT <= qb && jw + 31 <= p0 && (jw + 32 <= a.sinks || p0 + QT - 1 - jw < a.window);
 #pragma unroll 1
     for (int qt = 0; qt < 2; ++qt) {
+      if constexpr (sizeof(T) == 2) ln.forget();
       f32x16 s = tile_zero<f32x16>(), dp = tile_zero<f32x16>();
 #pragma unroll
       for (int st = 0; st < NS; ++st) {
-        s = Tile<T>::mma32(Img::frag(qi, qt * 32, st, lane), kf[st], s);
-        dp = Tile<T>::mma32(Img::frag(di, qt * 32, st, lane), vf[st], dp);
+        s = Tile<T>::mma32(Img::frag(qi, qt * 32, st, ln), kf[st], s);
+        dp = Tile<T>::mma32(Img::frag(di, qt * 32, st, ln), vf[st], dp);
       }
 #pragma unroll
       for (int i4 = 0; i4 < 4; ++i4) {
@@ -392,8 +392,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void s
         for (int e = 0; e < 8; ++e) { pf[e] = (T)s[st * 8 + e]; df[e] = (T)dp[st * 8 + e]; }
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
-          dv[d] = Tile<T>::mma32(Img::trans(di, qt * 32 + st * 16, d * 32, lane), pf, dv[d]);
-          dk[d] = Tile<T>::mma32(Img::trans(qi, qt * 32 + st * 16, d * 32, lane), df, dk[d]);
+          dv[d] = Tile<T>::mma32(Img::trans(di, qt * 32 + st * 16, d * 32, ln), pf, dv[d]);
+          dk[d] = Tile<T>::mma32(Img::trans(qi, qt * 32 + st * 16, d * 32, ln), df, dk[d]);
         }
       }
     }

@@ -43,68 +43,82 @@ __device__ __forceinline__ bf16x8 step_fp4(uint32_t x, float scale) {
   return (bf16x8){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// One tile of 32 keys in registers: lane l holds, for the keys (l & 15) and 16 + (l & 15), NS runs of 8
-// elements: dense from 32 t + 8 g (g = l >> 4), 4-bit from g * HDP / 4 + 8 t (one dword each).
+// A tile of 32 keys in registers: lane l holds, for the keys (l & 15) and 16 + (l & 15), NS runs of 8
+// elements: dense from 32 t + 8 g (g = l >> 4), 4-bit from g * HDP / 4 + 8 t (one dword each).  Loads are
+// unconditional, of a valid row where the key is hidden (`hid`, one bit per key), so that nothing waits
+// for them before their tile's turn; hidden values become zeros then (they may be anything).
 template <bool KV4, typename T, int HDP> struct StepTile;
 template <typename T, int HDP> struct StepTile<false, T, HDP> {
   static constexpr int NS = HDP / 32;
   typename Tile<T>::V8 k[2][NS], v[2][NS];
   uint32_t hid;
   __device__ __forceinline__ static int elem(int t, int g) { return 32 * t + 8 * g; }
-  __device__ __forceinline__ void load(const StepArgs& a, int b, int kvh, int j0, int last, int lo, int lane) {
+  __device__ __forceinline__ void load(const StepArgs& a, int b, int kvh, int j0, int last, int lo, int, int, int lane) {
     hid = 0;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const int j = j0 + 16 * s + (lane & 15);
-      const bool ok = j < last && (j < a.sinks || j >= lo) && !(a.pad && a.pad[(int64_t)b * a.cap + j]);
+      const int j = min(j0 + 16 * s + (lane & 15), last - 1);
+      const bool ok = (j0 + 16 * s + (lane & 15) < last) & ((j < a.sinks) | (j >= lo));
       hid |= (uint32_t)(~__builtin_amdgcn_ballot_w64(ok) & 0xffff) << (16 * s);
+      if (a.pad) hid |= (uint32_t)(__builtin_amdgcn_ballot_w64(a.pad[(int64_t)b * a.cap + j]) & 0xffff) << (16 * s);
       const T *kr = row<T>(a.k, b, j, kvh), *vr = row<T>(a.v, b, j, kvh);
 #pragma unroll
       for (int t = 0; t < NS; ++t) {
-        const int d = elem(t, lane >> 4);
-        k[s][t] = v[s][t] = tile_zero8<T>();
-        if (ok && d < a.hd) {
-          k[s][t] = Tile<T>::load(kr + d);
-          v[s][t] = Tile<T>::load(vr + d);
-        }
+        const int d = elem(t, lane >> 4) < a.hd ? elem(t, lane >> 4) : 0;
+        k[s][t] = Tile<T>::load(kr + d);
+        v[s][t] = Tile<T>::load(vr + d);
       }
     }
+  }
+  __device__ __forceinline__ void clear(int s, bool hidden) {
+#pragma unroll
+    for (int t = 0; t < NS; ++t)
+      if (hidden) v[s][t] = tile_zero8<T>();
   }
   __device__ __forceinline__ typename Tile<T>::V8 kf(int s, int t, int) const { return k[s][t]; }
   __device__ __forceinline__ typename Tile<T>::V8 vf(int s, int t, int) const { return v[s][t]; }
 };
 template <typename T, int HDP> struct StepTile<true, T, HDP> {
   static constexpr int NS = HDP / 32, NB = HDP / 32;
-  uint32_t k[2][NS], v[2][NS], ks[2], vs[2], hid;  // ks, vs: scale codes of the first and the last run
+  uint32_t k[2][NS], v[2][NS];
+  uint8_t ks[2][HDP == 96 ? 2 : 1], vs[2][HDP == 96 ? 2 : 1];  // scale codes of the first (and the last) run
+  uint32_t hid;
   __device__ __forceinline__ static int elem(int t, int g) { return g * (HDP / 4) + 8 * t; }
-  __device__ __forceinline__ void load(const StepArgs& a, int b, int kvh, int j0, int last, int lo, int lane) {
+  // pages: the page of every 16 keys of the next tiles, one per lane; `at` is this tile's first
+  __device__ __forceinline__ void load(const StepArgs& a, int b, int kvh, int j0, int last, int lo, int pages, int at, int lane) {
     hid = 0;
     const int g = lane >> 4, e0 = elem(0, g) / 32, e1 = elem(NS - 1, g) / 32;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const int js = j0 + 16 * s, j = js + (lane & 15);
-      // 16 keys from a multiple of 16 lie in one page
-      const int pg = js < last ? a.table[(int64_t)b * a.table_ld + js / a.page] : -1;
-      const bool ok = j < last && (j < a.sinks || j >= lo) && pg >= 0 && pg < a.pages;
+      const int pg = __builtin_amdgcn_readlane(pages, at + s);  // 16 keys from a multiple of 16 lie in one page
+      const bool page_ok = pg >= 0 && pg < a.pages;
+      const bool ok = (j < last) & ((j < a.sinks) | (j >= lo)) & page_ok;
       hid |= (uint32_t)(~__builtin_amdgcn_ballot_w64(ok) & 0xffff) << (16 * s);
-      ks[s] = vs[s] = 127 | 127 << 8;
+      const int64_t kr = ((int64_t)(page_ok ? pg : 0) * 2 * a.Hk + kvh) * a.page + js % a.page, vr = kr + (int64_t)a.Hk * a.page;
+      const uint32_t o = (lane & 15) * (HDP / 2) + g * (HDP / 8), so = (lane & 15) * NB;
+      const uint32_t *kc = (const uint32_t*)(a.codes + kr * (HDP / 2) + o), *vc = (const uint32_t*)(a.codes + vr * (HDP / 2) + o);
 #pragma unroll
-      for (int t = 0; t < NS; ++t) k[s][t] = v[s][t] = 0;
-      if (ok) {
-        const int64_t kr = (((int64_t)pg * 2) * a.Hk + kvh) * a.page + js % a.page + (lane & 15), vr = kr + (int64_t)a.Hk * a.page;
-        const uint32_t *kc = (const uint32_t*)(a.codes + kr * (HDP / 2) + g * (HDP / 8)),
-                       *vc = (const uint32_t*)(a.codes + vr * (HDP / 2) + g * (HDP / 8));
-#pragma unroll
-        for (int t = 0; t < NS; ++t) { k[s][t] = kc[t]; v[s][t] = vc[t]; }
-        ks[s] = a.scales[kr * NB + e0] | (uint32_t)a.scales[kr * NB + e1] << 8;
-        vs[s] = a.scales[vr * NB + e0] | (uint32_t)a.scales[vr * NB + e1] << 8;
+      for (int t = 0; t < NS; ++t) { k[s][t] = kc[t]; v[s][t] = vc[t]; }
+      const uint8_t *kss = a.scales + kr * NB + so, *vss = a.scales + vr * NB + so;
+      ks[s][0] = kss[e0];
+      vs[s][0] = vss[e0];
+      if constexpr (HDP == 96) {
+        ks[s][1] = kss[e1];
+        vs[s][1] = vss[e1];
       }
     }
   }
-  __device__ __forceinline__ static float scale(uint32_t c, int t, int g) {
+  __device__ __forceinline__ void clear(int s, bool hidden) {
+#pragma unroll
+    for (int t = 0; t < NS; ++t) v[s][t] = hidden ? 0 : v[s][t];
+    vs[s][0] = hidden ? 127 : vs[s][0];
+    if constexpr (HDP == 96) vs[s][1] = hidden ? 127 : vs[s][1];
+  }
+  __device__ __forceinline__ static float scale(const uint8_t* c, int t, int g) {
     // run t lies in the block of the first run or in that of the last
-    const bool second = HDP == 96 && elem(t, g) / 32 != elem(0, g) / 32;
-    return __uint_as_float((second ? c >> 8 : c & 255) << 23);
+    if constexpr (HDP == 96) return __uint_as_float((uint32_t)(elem(t, g) / 32 != elem(0, g) / 32 ? c[1] : c[0]) << 23);
+    else return __uint_as_float((uint32_t)c[0] << 23);
   }
   __device__ __forceinline__ bf16x8 kf(int s, int t, int g) const { return step_fp4(k[s][t], scale(ks[s], t, g)); }
   __device__ __forceinline__ bf16x8 vf(int s, int t, int g) const { return step_fp4(v[s][t], scale(vs[s], t, g)); }
@@ -116,20 +130,50 @@ template <typename T> __device__ __forceinline__ void step_row(const StepArgs& a
   h = kvh * G + r % G;
 }
 
+// waves per SIMD that the registers of each form allow
+template <bool KV4, typename T, int HDP, int NRT> constexpr int step_waves() {
+  if (NRT == 4 || (NRT == 2 && HDP > 64 && !(KV4 && sizeof(T) == 2))) return 1;
+  if (sizeof(T) == 4) return KV4 || (HDP <= 64 && NRT == 1) ? 2 : 1;
+  return NRT == 1 && HDP <= 64 ? 3 : 2;
+}
+
 // Grid: (splits, Hk * row groups of 16 NRT, B); 4 waves.
 template <bool KV4, typename T, int HDP, int NRT>
-__global__ __launch_bounds__(256) void step_attn(StepArgs a) {
+__global__ __launch_bounds__(256, (step_waves<KV4, T, HDP, NRT>())) void step_attn(StepArgs a) {
   using Ty = StepTypes<KV4, T>;
   using F = typename Ty::F;
   using E = typename Ty::E;
   using St = StepTile<KV4, T, HDP>;
   constexpr int NS = HDP / 32, ND = HDP / 16, PARTS = Ty::PARTS, IST = HDP + 16, OST = HDP + 4;
+  constexpr int KT = 32, GROUP = 32;  // keys of a tile; tiles whose pages a wave holds at a time
   extern __shared__ __align__(16) char smem[];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4;
   const int b = blockIdx.z, kvh = blockIdx.y % a.Hk, r0 = blockIdx.y / a.Hk * 16 * NRT, R = a.Nq * (a.H / a.Hk);
   const int len = a.len ? min(max(a.len[b], 0), a.cap) : a.cap, off = len - a.Nq;
   const float c = a.scale * kTileLog2e;
   E* img = (E*)smem + w * 32 * IST;
+
+  const SlideTiles<KT> tiles(a.window, a.sinks, off, len - 1, len);
+  const int lo = off - a.window + 1;  // first key of the first query's window
+  // this wave's share of the tiles
+  const int64_t part = (int64_t)blockIdx.x * 4 + w, parts = (int64_t)a.splits * 4;
+  const int ta = (int)(tiles.n * part / parts), tb = (int)(tiles.n * (part + 1) / parts);
+  // tiles in flight: 4-bit ones are small, and three of them cover the latency of memory
+  constexpr int RING = KV4 ? 3 : 2;
+  St ring[RING];
+  int pages = -1;  // the pages of the GROUP tiles from ta + i GROUP on, one 16-key piece per lane
+  auto fetch = [&](St& st, int t) {
+    if constexpr (KV4) {
+      if ((t - ta) % GROUP == 0) {
+        const int tt = t + lane / 2, j = tt < tb ? tiles.key0(tt) + lane % 2 * 16 : len;
+        pages = j < len ? a.table[(int64_t)b * a.table_ld + j / a.page] : -1;
+      }
+    }
+    st.load(a, b, kvh, tiles.key0(t), len, lo, pages, (t - ta) % GROUP * 2, lane);
+  };
+#pragma unroll
+  for (int i = 0; i + 1 < RING; ++i)
+    if (ta + i < tb) fetch(ring[i], ta + i);
 
   F qf[NRT][NS][PARTS];
   int pos[NRT];
@@ -150,7 +194,7 @@ __global__ __launch_bounds__(256) void step_attn(StepArgs a) {
     }
   }
   f32x4 o[NRT][ND];
-  float m[NRT], l[NRT];
+  float m[NRT], l[NRT];  // m: the exponent that the sums are relative to (c s), within 8 of the running maximum
 #pragma unroll
   for (int rt = 0; rt < NRT; ++rt) {
     m[rt] = -INFINITY;
@@ -158,29 +202,14 @@ __global__ __launch_bounds__(256) void step_attn(StepArgs a) {
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[rt][d] = (f32x4){0.f, 0.f, 0.f, 0.f};
   }
-  const SlideTiles<32> tiles(a.window, a.sinks, off, len - 1, len);
-  const int lo = off - a.window + 1;  // first key of the first query's window
-  const int t1 = (int)((int64_t)tiles.n * (blockIdx.x + 1) / a.splits);
-  int t = (int)((int64_t)tiles.n * blockIdx.x / a.splits) + w;
-  St cur, nxt;
-  if (t < t1) cur.load(a, b, kvh, tiles.key0(t), len, lo, lane);
-  for (; t < t1; t += 4) {
+  auto compute = [&](St& cur, int t) {
     const int j0 = tiles.key0(t);
-    if (t + 4 < t1) nxt.load(a, b, kvh, tiles.key0(t + 4), len, lo, lane);
-    // V rows into the wave's own image: a wave's LDS accesses run in order, so the last tile's reads are
-    // served before these writes, and these before the reads below (the fences hold the compiler to it)
-    asm volatile("" ::: "memory");
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int i = 0; i < NS; ++i) *(F*)(img + (16 * s + (lane & 15)) * IST + St::elem(i, g)) = cur.vf(s, i, g);
-    asm volatile("" ::: "memory");
-    const bool full = cur.hid == 0 && j0 + 31 <= off && (j0 + 32 <= a.sinks || len - 1 - j0 < a.window);
+    const bool full = cur.hid == 0 && j0 + KT - 1 <= off && (j0 + KT <= a.sinks || len - 1 - j0 < a.window);
     f32x4 sc[NRT][2];
 #pragma unroll
-    for (int rt = 0; rt < NRT; ++rt) sc[rt][0] = sc[rt][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < 2; ++s) {
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+      for (int rt = 0; rt < NRT; ++rt) sc[rt][s] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
         const F k = cur.kf(s, i, g);
@@ -189,33 +218,49 @@ __global__ __launch_bounds__(256) void step_attn(StepArgs a) {
 #pragma unroll
           for (int p = PARTS - 1; p >= 0; --p) sc[rt][s] = Tile<E>::mma16(k, qf[rt][i][p], sc[rt][s]);
       }
+    }
+    if (cur.hid) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) cur.clear(s, cur.hid >> (16 * s + (lane & 15)) & 1);
+    }
+    // V rows into the wave's own image: a wave's LDS accesses run in order, so the last tile's reads are
+    // served before these writes, and these before the reads below (the fences hold the compiler to it)
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int i = 0; i < NS; ++i) *(F*)(img + (16 * s + (lane & 15)) * IST + St::elem(i, g)) = cur.vf(s, i, g);
+    asm volatile("" ::: "memory");
     F pf[NRT][PARTS];
 #pragma unroll
     for (int rt = 0; rt < NRT; ++rt) {
-      float mt = -INFINITY;
-      f32x8 x;
+      f32x8 x = {sc[rt][0][0], sc[rt][0][1], sc[rt][0][2], sc[rt][0][3], sc[rt][1][0], sc[rt][1][1], sc[rt][1][2], sc[rt][1][3]};
+      if (!full) {
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int jj = 16 * s + 4 * g + i, j = j0 + jj;
-          float y = sc[rt][s][i] * c;
-          if (!full && (((cur.hid >> jj) & 1) || j > pos[rt] || (j >= a.sinks && pos[rt] - j >= a.window))) y = -INFINITY;
-          x[4 * s + i] = y;
-          mt = fmaxf(mt, y);
+        for (int e = 0; e < 8; ++e) {
+          const int jj = 16 * (e >> 2) + 4 * g + (e & 3), j = j0 + jj;
+          const bool sees = (((unsigned)(pos[rt] - j) < (unsigned)a.window) | ((j < a.sinks) & (j <= pos[rt]))) & !(cur.hid >> jj & 1);
+          x[e] = sees ? x[e] : -INFINITY;
         }
+      }
+      float mt = x[0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) mt = fmaxf(mt, x[e]);
       mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
-      mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
-      const float mn = fmaxf(m[rt], mt), ms = mn == -INFINITY ? 0.f : mn, alpha = tile_exp2(m[rt] - ms);
-      m[rt] = mn;
-      l[rt] *= alpha;
+      mt = fmaxf(mt, __shfl_xor(mt, 32, 64)) * c;
+      if (__builtin_amdgcn_ballot_w64(mt > m[rt] + 8.f)) {
+        const float mn = fmaxf(m[rt], mt), alpha = mn == -INFINITY ? 1.f : tile_exp2(m[rt] - mn);
+        m[rt] = mn;
+        l[rt] *= alpha;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[rt][d] *= alpha;
+      }
+      const float ms = m[rt] == -INFINITY ? 0.f : m[rt];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        x[e] = tile_exp2(x[e] - ms);
+        x[e] = tile_exp2(fmaf(x[e], c, -ms));
         l[rt] += x[e];
       }
-#pragma unroll
-      for (int d = 0; d < ND; ++d) o[rt][d] *= alpha;
       step_parts<PARTS, F>(x, pf[rt]);
     }
 #pragma unroll
@@ -226,7 +271,15 @@ __global__ __launch_bounds__(256) void step_attn(StepArgs a) {
 #pragma unroll
         for (int p = PARTS - 1; p >= 0; --p) o[rt][d] = Tile<E>::mma16(v, pf[rt][p], o[rt][d]);
     }
-    cur = nxt;
+  };
+  // (a ring by unrolling: copying a tile that is on its way would wait for it)
+  for (int t = ta; t < tb; t += RING) {
+#pragma unroll
+    for (int i = 0; i < RING; ++i) {
+      if (t + i >= tb) break;
+      if (t + i + RING - 1 < tb) fetch(ring[(i + RING - 1) % RING], t + i + RING - 1);
+      compute(ring[i], t + i);
+    }
   }
   // join the 4 waves, 16 columns at a time
   float* os = (float*)smem;               // [4][16][OST]
@@ -271,40 +324,56 @@ __global__ __launch_bounds__(256) void step_attn(StepArgs a) {
   }
 }
 
-// One wave per (sequence, head, query): the splits' partial softmaxes joined in order.
+// One workgroup per (sequence, head, query): 8 groups of 32 lanes (4 elements each) share the splits, and
+// their sums are added in order.
 template <typename T>
 __global__ __launch_bounds__(256) void step_join(StepArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (at >= (int64_t)a.B * a.H * a.Nq) return;
+  __shared__ f32x4 os[8][32];
+  __shared__ float ls[8];
+  const int64_t at = blockIdx.x;
+  const int lane = threadIdx.x & 63, d = (threadIdx.x & 31) * 4, grp = threadIdx.x >> 5;
   const float* ml = a.pml + at * a.splits * 2;
   float mm = -INFINITY;
   for (int s = lane; s < a.splits; s += 64) mm = fmaxf(mm, ml[2 * s]);
   mm = wave_max(mm);
   float ll = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  const float* po = a.po + at * a.splits * a.hd + lane * 4;
-  for (int s = 0; s < a.splits; ++s) {
+  const float* po = a.po + at * a.splits * a.hd + d;
+#pragma unroll 4
+  for (int s = grp; s < a.splits; s += 8) {
     const float f = mm == -INFINITY ? 0.f : tile_exp2(ml[2 * s] - mm);
     ll += f * ml[2 * s + 1];
-    if (lane * 4 < a.hd) o += *(const f32x4*)(po + (int64_t)s * a.hd) * f;
+    if (d < a.hd) o += *(const f32x4*)(po + (int64_t)s * a.hd) * f;
+  }
+  os[grp][threadIdx.x & 31] = o;
+  if (d == 0) ls[grp] = ll;
+  __syncthreads();
+  if (grp || d >= a.hd) return;
+  for (int u = 1; u < 8; ++u) {
+    o += os[u][threadIdx.x];
+    ll += ls[u];
   }
   const int i = (int)(at % a.Nq), h = (int)(at / a.Nq % a.H), b = (int)(at / a.Nq / a.H);
-  if (lane * 4 < a.hd) Tile<T>::store4(row<T>(a.o, b, i, h) + lane * 4, o * (ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll)));
-  if (a.lse && lane == 0) a.lse[at] = ll > 0.f ? (mm + __log2f(ll)) * kTileLn2 : (ll == 0.f ? -INFINITY : ll);
+  Tile<T>::store4(row<T>(a.o, b, i, h) + d, o * (ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll)));
+  if (a.lse && d == 0) a.lse[at] = ll > 0.f ? (mm + __log2f(ll)) * kTileLn2 : (ll == 0.f ? -INFINITY : ll);
 }
 
-// 16-column tiles per wave: all of them up to 4 (fp32, whose queries take two or three times the
-// registers: 2); more rows take further workgroups, which read the cache again
-static int step_nrt(int dtype, int rows) { return rows <= 16 ? 1 : rows <= 32 || dtype == CAPK_F32 ? 2 : 4; }
+// 16-column tiles per wave: all of them, up to what registers hold; more rows take further workgroups,
+// which read the cache again
+static int step_nrt(int dtype, bool kv4, int hd, int rows) {
+  const int most = dtype == CAPK_BF16 ? (kv4 || hd <= 96 ? 4 : 2) : kv4 || hd <= 96 ? 2 : 1;
+  return rows <= 16 || most == 1 ? 1 : rows <= 32 || most == 2 ? 2 : 4;
+}
 
 size_t step_workspace(int dtype, const StepArgs& a, int* splits) {
-  const int rows = a.Nq * (a.H / a.Hk), nrt = step_nrt(dtype, rows);
+  const int rows = a.Nq * (a.H / a.Hk), nrt = step_nrt(dtype, a.page != 0, a.hd, rows);
   const int64_t blocks = (int64_t)a.B * a.Hk * cdiv(rows, 16 * nrt);
-  // workgroups for 4 on every CU, with at least a tile of 32 keys for each wave of a split
+  // two workgroups (what registers hold) on every CU, with at least a tile of 32 keys for each wave of a
+  // split.  131072 keys, 8 key heads of 128, 20 columns: 36 + 6 us (join) at 512 workgroups, 47 + 4 at
+  // 256, 42 + 10 at 1024
   int64_t most = (int64_t)a.window + a.Nq + a.sinks + 64;
   if (most > a.cap) most = a.cap;
-  int64_t s = 1024 / blocks;
+  int64_t s = 512 / blocks;
   if (s > cdiv(most, 128)) s = cdiv(most, 128);
   if (s < 1) s = 1;
   *splits = (int)s;
@@ -314,12 +383,13 @@ size_t step_workspace(int dtype, const StepArgs& a, int* splits) {
 template <bool KV4, typename T, int HDP>
 static int step_go(const StepArgs& a, hipStream_t st) {
   using E = typename StepTypes<KV4, T>::E;
-  const int rows = a.Nq * (a.H / a.Hk), nrt = step_nrt(sizeof(T) == 2 ? CAPK_BF16 : CAPK_F32, rows);
+  const int rows = a.Nq * (a.H / a.Hk), nrt = step_nrt(sizeof(T) == 2 ? CAPK_BF16 : CAPK_F32, KV4, a.hd, rows);
   const dim3 grid(a.splits, a.Hk * cdiv(rows, 16 * nrt), a.B);
   const size_t img = (size_t)4 * 32 * (HDP + 16) * sizeof(E), join = (size_t)4 * 16 * (HDP + 4) * 4 + 512;
   const size_t shm = img > join ? img : join;
-  const void* fn = nrt == 1 ? (const void*)step_attn<KV4, T, HDP, 1> : nrt == 2 ? (const void*)step_attn<KV4, T, HDP, 2>
-                                                                               : (const void*)step_attn<KV4, T, HDP, (sizeof(T) == 2 ? 4 : 2)>;
+  constexpr int N4 = sizeof(T) == 2 && (KV4 || HDP <= 96) ? 4 : 1, N2 = sizeof(T) == 4 && !KV4 && HDP > 96 ? 1 : 2;
+  const void* fn = nrt == 1 ? (const void*)step_attn<KV4, T, HDP, 1> : nrt == 2 ? (const void*)step_attn<KV4, T, HDP, N2>
+                                                                               : (const void*)step_attn<KV4, T, HDP, N4>;
   if (shm > 65536) {
     hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)shm);
     if (e != hipSuccess) return hip_status(e, "step_attn");
@@ -329,7 +399,7 @@ static int step_go(const StepArgs& a, hipStream_t st) {
   hipError_t e = hipLaunchKernel(fn, grid, dim3(256), args, shm, st);
   if (e != hipSuccess) return hip_status(e, "step_attn");
   if (a.splits > 1) {
-    hipLaunchKernelGGL(step_join<T>, dim3(cdiv((int64_t)a.B * a.H * a.Nq, 4)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(step_join<T>, dim3(a.B * a.H * a.Nq), dim3(256), 0, st, a);
     CAPK_LAUNCH_CHECK("step_join");
   }
   return CAPK_OK;

@@ -105,34 +105,53 @@ template <typename T, int HDP> struct TileImg {
     for (int o = threadIdx.x * 16; o < 64 * RB; o += 256 * 16)
       if (rows >> (o / RB) & 1) *(f32x4*)(img + o) = (f32x4){0.f, 0.f, 0.f, 0.f};
   }
-  // A / B fragment of a 32x32 product: row r0 + (l & 31), columns 16 s + 8 h (r0 a multiple of 32)
-  __device__ __forceinline__ static typename Tile<T>::V8 frag(const char* img, int r0, int s, int lane) {
-    const int r = lane & 31, f = swz(r), c = (2 * s + (lane >> 5)) * 8 / PER;
-    const char* at = img + (r0 + r) * RB;
-    if constexpr (sizeof(T) == 2) return *(const bf16x8*)(at + ((c ^ f) << 4));
-    else {
-      const f32x4 x = *(const f32x4*)(at + ((c ^ f) << 4)), y = *(const f32x4*)(at + (((c + 1) ^ f) << 4));
+  // Byte offsets of a lane's reads: of a row fragment, and (bf16) of the two halves of a transposed one.
+  struct Lane {
+    int f, ta, tb;
+    __device__ __forceinline__ explicit Lane(int lane) {
+      const int r = lane & 31, h = lane >> 5, i16 = lane & 15;
+      f = r * RB + ((h * 8 / PER ^ swz(r)) << 4);
+      if constexpr (sizeof(T) == 2) {
+        const int q = 4 * h + (i16 >> 2), c = 2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1);
+        ta = q * RB + ((c ^ swz(q)) << 4) + (i16 & 1) * 8;
+        tb = (q + 8) * RB + ((c ^ swz(q + 8)) << 4) + (i16 & 1) * 8;
+      } else {
+        ta = h;
+        tb = r;
+      }
+    }
+    // Makes the offsets opaque: what derives from them is computed again (an instruction each) where the
+    // loop would otherwise hold it in registers that it does not have.
+    __device__ __forceinline__ void forget() { asm volatile("" : "+v"(f), "+v"(ta), "+v"(tb)); }
+  };
+  static constexpr bool POW2 = (RB & (RB - 1)) == 0;
+  // A / B fragment of a 32x32 product: row r0 + (l & 31), columns 16 s + 8 h (r0 a multiple of 32).  Chunks
+  // 2 s (fp32: 4 s) beside the mask: an exclusive or, where rows are not a power of two of its masked bits.
+  __device__ __forceinline__ static typename Tile<T>::V8 frag(const char* img, int r0, int s, const Lane& l) {
+    if constexpr (sizeof(T) == 2) {
+      const int o = POW2 ? l.f ^ (s * 32) : (l.f ^ ((s & 1) * 32)) + (s >> 1) * 64;
+      return *(const bf16x8*)(img + r0 * RB + o);
+    } else {
+      const int o = POW2 ? l.f ^ (s * 64) : (l.f ^ ((s & 1) * 64)) + (s >> 1) * 128;
+      const f32x4 x = *(const f32x4*)(img + r0 * RB + o), y = *(const f32x4*)(img + r0 * RB + (o ^ 16));
       return (f32x8){x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
     }
   }
   // A fragment of the transpose for a 32x32 product: lane column c0 + (l & 31), slot (h, e) = row
   // r0 + 8 (e >> 2) + 4 h + (e & 3) -- the order in which eight accumulator registers of a 32x32
   // product hold their rows (r0 a multiple of 16, c0 of 32).
-  __device__ __forceinline__ static typename Tile<T>::V8 trans(const char* img, int r0, int c0, int lane) {
-    const int h = lane >> 5;
+  __device__ __forceinline__ static typename Tile<T>::V8 trans(const char* img, int r0, int c0, const Lane& l) {
     if constexpr (sizeof(T) == 2) {
-      const int i16 = lane & 15, r = 4 * h + (i16 >> 2), c = c0 / 8 + 2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1);
-      const char *a = img + (r0 + r) * RB + ((c ^ swz(r)) << 4) + (i16 & 1) * 8,
-                 *b = img + (r0 + 8 + r) * RB + ((c ^ swz(r + 8)) << 4) + (i16 & 1) * 8;
+      const char *a = img + r0 * RB + (POW2 ? l.ta ^ (c0 * 2) : l.ta + c0 * 2), *b = img + r0 * RB + (POW2 ? l.tb ^ (c0 * 2) : l.tb + c0 * 2);
       const bf16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, a));
       const bf16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, b));
       return (bf16x8){x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
     } else {
-      const int d = c0 + (lane & 31);
+      const int d = c0 + l.tb;
       f32x8 v;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int r = 8 * (e >> 2) + 4 * h + (e & 3);
+        const int r = 8 * (e >> 2) + 4 * l.ta + (e & 3);
         v[e] = *(const float*)(img + (r0 + r) * RB + (((d / 4) ^ swz(r)) << 4) + (d & 3) * 4);
       }
       return v;

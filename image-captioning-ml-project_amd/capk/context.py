@@ -32,10 +32,11 @@ def _rows(t):
     """`t` itself where its rows start 16-B aligned with unit element stride, else a contiguous copy."""
     if t is None or t.dim() != 4:
         return t
-    n = 16 // t.element_size()
-    ok = t.data_ptr() % 16 == 0 and (t.stride(3) == 1 or t.shape[3] == 1)
-    ok = ok and all(s % n == 0 or d == 1 for s, d in zip(t.stride()[:3], t.shape[:3]))
-    return t if ok else t.contiguous()
+    n, s, d = 16 // t.element_size(), t.stride(), t.shape
+    if (t.data_ptr() % 16 == 0 and (s[3] == 1 or d[3] == 1) and (s[0] % n == 0 or d[0] == 1)
+            and (s[1] % n == 0 or d[1] == 1) and (s[2] % n == 0 or d[2] == 1)):
+        return t
+    return t.contiguous()
 
 
 def _unit(t):

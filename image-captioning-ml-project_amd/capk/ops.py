@@ -1262,22 +1262,27 @@ def mask_rows_by_length(x, lengths_i32):
 # ------------------------------------------------- long-context decoding ---
 def _launch(dev, name, *args):
     """Call an entry point on `dev`'s current stream (its arguments end with the stream)."""
-    if dev.index != torch.cuda.current_device():
+    at = dev.index
+    if at != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
             return _launch(dev, name, *args)
-    check(getattr(lib(), name)(*args, torch.cuda.current_stream().cuda_stream), name)
+    rc = getattr(_lib.load(), name)(*args, torch._C._cuda_getCurrentRawStream(at))
+    if rc:
+        check(rc, name)
 
 
 def _same(what, first, *rest, dtype=True):
     """All tensors on `first`'s GPU and, with dtype, of its type."""
-    _need_gpu(first)
+    dev, dt = first.device, first.dtype
+    if dev.type != "cuda":
+        _need_gpu(first)
     for t in rest:
         if t is None:
             continue
-        if t.device != first.device:
-            raise _lib.CapkError(f"{what}: tensors on {first.device} and {t.device}")
-        if dtype and t.dtype != first.dtype:
-            raise _lib.CapkError(f"{what}: {first.dtype} and {t.dtype}")
+        if t.device != dev:
+            raise _lib.CapkError(f"{what}: tensors on {dev} and {t.device}")
+        if dtype and t.dtype != dt:
+            raise _lib.CapkError(f"{what}: {dt} and {t.dtype}")
 
 
 def _index(what, t, shape, dtype, dev):
@@ -1286,27 +1291,28 @@ def _index(what, t, shape, dtype, dev):
         return None
     if t.device != dev:
         raise _lib.CapkError(f"{what} on {t.device}, the operands on {dev}")
-    if tuple(t.shape) != tuple(shape) or t.dtype.is_floating_point or t.dtype.is_complex:
+    if t.shape != shape or t.dtype.is_floating_point or t.dtype.is_complex:
         raise ValueError(f"{what}: need integers of shape {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
-    return t.to(dtype).contiguous()
+    return t if t.dtype == dtype and t.is_contiguous() else t.to(dtype).contiguous()
 
 
 def _view4(what, t):
     """(pointer, batch, token and head stride) of a [B, N, H, hd] view with unit element stride."""
-    if t.dim() != 4 or (t.stride(3) != 1 and t.shape[3] > 1):
+    shape, s = t.shape, t.stride()
+    if len(shape) != 4 or (s[3] != 1 and shape[3] > 1):
         raise ValueError(f"{what}: need [batch, tokens, heads, head_dim] with unit stride in the last, got "
-                         f"{tuple(t.shape)} / {t.stride()}")
-    (nb, nn, nh, _), s = t.shape, t.stride()  # (a dimension of one has no stride to speak of)
-    return t.data_ptr(), s[0] if nb > 1 else 0, s[1] if nn > 1 else 0, s[2] if nh > 1 else 0
+                         f"{tuple(shape)} / {s}")
+    # (a dimension of one has no stride to speak of)
+    return t.data_ptr(), s[0] if shape[0] > 1 else 0, s[1] if shape[1] > 1 else 0, s[2] if shape[2] > 1 else 0
 
 
 def axis_rope(q, k, pos, freq, axis, *, interleaved=False, inverse=False, out_q=None, out_k=None):
     """Rotary positions over several axes (capk_axis_rope) of q [B, N, H, hd] and k [B, N, Hk, hd] (or
     None); pos int [axes, B, N] or [axes, N], freq fp64 [pairs], axis [pairs].  out_q / out_k may be q / k."""
     what = "axis_rope"
-    out_q = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out_q is None else out_q
+    out_q = q.new_empty(q.shape) if out_q is None else out_q
     if k is not None and out_k is None:
-        out_k = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        out_k = k.new_empty(k.shape)
     _same(what, q, k, out_q, out_k)
     code = dtype_code(q)
     qv, qov = _view4(what, q), _view4(what, out_q)
@@ -1347,10 +1353,11 @@ def sliding_attention_fwd(q, k, v, window, sinks, scale, key_pad=None, kv_len=No
     what = "sliding_attention_fwd"
     code, dims, ws_args, views, key_pad, kv_len = _sliding_args(what, q, k, v, window, sinks, key_pad, kv_len)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    _same(what, q, out)
-    if out.shape != q.shape:
-        raise ValueError(f"{what}: out {tuple(out.shape)} for q {tuple(q.shape)}")
+        out = q.new_empty(q.shape)
+    else:
+        _same(what, q, out)
+        if out.shape != q.shape:
+            raise ValueError(f"{what}: out {tuple(out.shape)} for q {tuple(q.shape)}")
     lse = torch.empty(q.shape[0], q.shape[2], q.shape[1], dtype=torch.float32, device=q.device) if want_lse else None
     wsb = lib().capk_sliding_attention_fwd_workspace(code, *dims, *ws_args)
     ws = _ws(wsb, q.device)
@@ -1368,7 +1375,7 @@ def sliding_attention_bwd(q, k, v, o, do, lse, window, sinks, scale, key_pad=Non
     if o.shape != q.shape or do.shape != q.shape or lse.dtype != torch.float32 or not lse.is_contiguous() or \
             tuple(lse.shape) != (q.shape[0], q.shape[2], q.shape[1]):
         raise ValueError(f"{what}: o, do like q and a contiguous fp32 lse [B, H, Nq]")
-    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
     wsb = lib().capk_sliding_attention_bwd_workspace(*dims, *ws_args)
     ws = _ws(wsb, q.device)
     _launch(q.device, "capk_sliding_attention_bwd", code, *dims, float(scale), *ws_args, *views, _p(key_pad), _p(kv_len),
@@ -1440,7 +1447,7 @@ def kv4_attention(q, codes, scales, table, kv_len, window, sinks, scale, *, lse=
     kv_len = _index(f"{what}: kv_len", kv_len, (B,), torch.int32, q.device)
     if kv_len is None:
         raise ValueError(f"{what}: kv_len is needed")
-    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    o = q.new_empty(q.shape)
     wsb = lib().capk_kv4_attention_workspace(code, B, H, Hk, Nq, hd, int(window), int(sinks), page, table.shape[1])
     ws = _ws(wsb, q.device)
     _launch(q.device, "capk_kv4_attention", code, B, H, Hk, Nq, hd, float(scale), int(window), int(sinks), *qv,

@@ -23,29 +23,37 @@ struct Kv4Args {
 
 // the row of K (V: + Hk * page) of token t of sequence b, -1 where the table has no page for it
 __device__ __forceinline__ int64_t kv4_row(const Kv4Args& a, int b, int64_t t, int h) {
-  if (t < 0 || t / a.page >= a.table_cols) return -1;
-  const int pg = a.table[b * a.table_ld + t / a.page];
-  return pg < 0 || pg >= a.pages ? -1 : ((int64_t)pg * 2 * a.Hk + h) * a.page + t % a.page;
+  if (t < 0 || t >= (int64_t)a.table_cols * a.page) return -1;
+  const int at = (int)t / a.page, pg = a.table[b * a.table_ld + at];
+  return pg < 0 || pg >= a.pages ? -1 : ((int64_t)pg * 2 * a.Hk + h) * a.page + ((int)t - at * a.page);
 }
 
-// Four lanes per block of 32: 8 elements each.  Grid-stride items (b, i, h, K / V, run of 8).
-template <typename T>
+// Grid: (tiles of tokens, Hk x {K, V}, B).  HD / 8 lanes per row of 8 elements each (four to a block of
+// 32), so a wave reads whole rows and writes the codes of successive tokens, which lie side by side.
+constexpr int kKv4Tile = 64;  // tokens per workgroup
+template <int HD> constexpr int kv4_rows() { return 256 / (HD / 8); }
+
+template <typename T, int HD>
 __global__ __launch_bounds__(256) void kv4_append(Kv4Args a) {
-  const int runs = a.hd / 8;
-  const int64_t items = (int64_t)a.B * a.n * a.Hk * 2 * runs;
-  for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < items; x += (int64_t)gridDim.x * 256) {
-    // the four lanes of a block share everything but the run, so they stay together
-    const int run = (int)(x % runs), h = (int)(x / runs % a.Hk), kv = (int)(x / runs / a.Hk % 2);
-    const int64_t bi = x / runs / a.Hk / 2;
-    const int b = (int)(bi / a.n), i = (int)(bi % a.n);
-    if (a.count && i >= a.count[b]) continue;
-    const int64_t r = kv4_row(a, b, (int64_t)a.start[b] + i, h);
-    if (r < 0) continue;
-    float v[8];
-    Vec8<T>::load(row<T>(kv ? a.v : a.k, b, i, h) + run * 8, v);
-    uint32_t amax = 0;  // the largest magnitude, as bits: infinities and NaN compare above every number
+  constexpr int RUNS = HD / 8, ROWS = kv4_rows<HD>(), IT = (kKv4Tile + ROWS - 1) / ROWS;
+  const int run = threadIdx.x % RUNS, r0 = threadIdx.x / RUNS, h = blockIdx.y >> 1, kv = blockIdx.y & 1, b = blockIdx.z;
+  const int n = a.count ? min(a.n, a.count[b]) : a.n, i0 = blockIdx.x * kKv4Tile;
+  const int64_t start = a.start[b];
+  const SlideView& x = kv ? a.v : a.k;
+  float v[IT][8];
+  int64_t at[IT];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) amax = max(amax, __float_as_uint(v[e]) & 0x7fffffffu);
+  for (int k = 0; k < IT; ++k) {  // every load before the first use
+    const int r = r0 + k * ROWS, i = i0 + r;
+    at[k] = r0 < ROWS && r < kKv4Tile && i < n ? kv4_row(a, b, start + i, h) : -1;
+    Vec8<T>::load(row<T>(x, b, min(i, a.n - 1), h) + run * 8, v[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < IT; ++k) {
+    if (at[k] < 0) continue;  // (the four lanes of a block together)
+    uint32_t amax = 0;        // the largest magnitude, as bits: infinities and NaN compare above every number
+#pragma unroll
+    for (int e = 0; e < 8; ++e) amax = max(amax, __float_as_uint(v[k][e]) & 0x7fffffffu);
     amax = max(amax, (uint32_t)__shfl_xor((int)amax, 1, 64));
     amax = max(amax, (uint32_t)__shfl_xor((int)amax, 2, 64));
     // amax = 1.f 2^(x - 127) lies within 6 = 1.5 * 2^2 scaled by 2^(x - 129), or the next power past 1.5
@@ -53,35 +61,40 @@ __global__ __launch_bounds__(256) void kv4_append(Kv4Args a) {
     code = amax == 0 ? 127 : amax >= 0x7f800000u ? 255 : code < 1 ? 1 : code;
     const float s = __uint_as_float((uint32_t)code << 23);
     uint32_t c = 0;
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[0], v[1], s, 0);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[2], v[3], s, 1);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[4], v[5], s, 2);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[6], v[7], s, 3);
-    const int64_t at = r + (int64_t)kv * a.Hk * a.page;
-    *(uint32_t*)(a.codes + at * (a.hd / 2) + run * 4) = code == 255 ? 0 : c;
-    if ((run & 3) == 0) a.scales[at * (a.hd / 32) + run / 4] = (uint8_t)code;
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[k][0], v[k][1], s, 0);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[k][2], v[k][3], s, 1);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[k][4], v[k][5], s, 2);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[k][6], v[k][7], s, 3);
+    const int64_t o = at[k] + (int64_t)kv * a.Hk * a.page;
+    *(uint32_t*)(a.codes + o * (HD / 2) + run * 4) = code == 255 ? 0 : c;
+    if ((run & 3) == 0) a.scales[o * (HD / 32) + run / 4] = (uint8_t)code;
   }
 }
 
-template <typename T>
+template <typename T, int HD>
 __global__ __launch_bounds__(256) void kv4_read(Kv4Args a) {
-  const int runs = a.hd / 8;
-  const int64_t items = (int64_t)a.B * a.n * a.Hk * 2 * runs;
-  for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < items; x += (int64_t)gridDim.x * 256) {
-    const int run = (int)(x % runs), h = (int)(x / runs % a.Hk), kv = (int)(x / runs / a.Hk % 2);
-    const int64_t bi = x / runs / a.Hk / 2;
-    const int b = (int)(bi / a.n), i = (int)(bi % a.n);
-    const int64_t r = kv4_row(a, b, (int64_t)a.start[b] + i, h);
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (r >= 0) {
-      const int64_t at = r + (int64_t)kv * a.Hk * a.page;
-      const uint32_t c = *(const uint32_t*)(a.codes + at * (a.hd / 2) + run * 4);
-      const float s = kv4_scale(a.scales[at * (a.hd / 32) + run / 4]);
-      const f32x2 p0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 0), p1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 1);
-      const f32x2 p2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 2), p3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 3);
-      v[0] = p0[0]; v[1] = p0[1]; v[2] = p1[0]; v[3] = p1[1]; v[4] = p2[0]; v[5] = p2[1]; v[6] = p3[0]; v[7] = p3[1];
-    }
-    Vec8<T>::store(row<T>(kv ? a.v : a.k, b, i, h) + run * 8, v);
+  constexpr int RUNS = HD / 8, ROWS = kv4_rows<HD>(), IT = (kKv4Tile + ROWS - 1) / ROWS;
+  const int run = threadIdx.x % RUNS, r0 = threadIdx.x / RUNS, h = blockIdx.y >> 1, kv = blockIdx.y & 1, b = blockIdx.z;
+  const int i0 = blockIdx.x * kKv4Tile;
+  const int64_t start = a.start[b];
+  const SlideView& y = kv ? a.v : a.k;
+  uint32_t c[IT], e[IT];
+#pragma unroll
+  for (int k = 0; k < IT; ++k) {
+    const int64_t at = kv4_row(a, b, start + i0 + r0 + k * ROWS, h), o = (at < 0 ? 0 : at) + (int64_t)kv * a.Hk * a.page;
+    c[k] = *(const uint32_t*)(a.codes + o * (HD / 2) + run * 4);
+    e[k] = a.scales[o * (HD / 32) + run / 4];
+    if (at < 0) c[k] = 0, e[k] = 127;
+  }
+#pragma unroll
+  for (int k = 0; k < IT; ++k) {
+    const int r = r0 + k * ROWS, i = i0 + r;
+    if (r0 >= ROWS || r >= kKv4Tile || i >= a.n) continue;
+    const float s = kv4_scale(e[k]);
+    const f32x2 p0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[k], s, 0), p1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[k], s, 1);
+    const f32x2 p2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[k], s, 2), p3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[k], s, 3);
+    const float v[8] = {p0[0], p0[1], p1[0], p1[1], p2[0], p2[1], p3[0], p3[1]};
+    Vec8<T>::store(row<T>(y, b, i, h) + run * 8, v);
   }
 }
 
@@ -89,7 +102,7 @@ static int kv4_check(const char* who, int dtype, int B, int n, int Hk, int hd, c
                      const void* codes, const void* scales, int pages, int page, const int32_t* table,
                      int64_t table_ld, int table_cols) {
   CAPK_CHECK_ARG(dtype == CAPK_F32 || dtype == CAPK_BF16, "%s: dtype", who);
-  CAPK_CHECK_ARG(B >= 0 && n >= 0 && Hk >= 1, "%s: bad sizes", who);
+  CAPK_CHECK_ARG(B >= 0 && B <= 65535 && n >= 0 && n <= (1 << 28) && Hk >= 1 && Hk <= 32767, "%s: bad sizes", who);
   CAPK_CHECK_ARG(hd == 32 || hd == 64 || hd == 96 || hd == 128, "%s: hd=%d must be 32, 64, 96 or 128", who, hd);
   CAPK_CHECK_ARG(page >= 16 && page % 16 == 0 && page <= 4096, "%s: page=%d must be a multiple of 16, <= 4096", who, page);
   CAPK_CHECK_ARG(pages >= 1 && codes && scales && (uintptr_t)codes % 16 == 0, "%s: pages must be 16-B aligned", who);
@@ -107,10 +120,15 @@ static int kv4_check(const char* who, int dtype, int B, int n, int Hk, int hd, c
 
 using namespace capk;
 
-static int kv4_blocks(const Kv4Args& a) {
-  const int64_t items = (int64_t)a.B * a.n * a.Hk * 2 * (a.hd / 8);
-  return (int)(cdiv(items, 256) < 16384 ? cdiv(items, 256) : 16384);
-}
+#define KV4_LAUNCH(KERNEL)                                                                               \
+  {                                                                                                     \
+    const dim3 grid(cdiv(n, kKv4Tile), 2 * Hk, B);                                                      \
+    SLIDE_HD(hd, {                                                                                      \
+      if (dtype == CAPK_BF16) hipLaunchKernelGGL((KERNEL<bf16, HDP>), grid, 256, 0, S(stream), a);      \
+      else hipLaunchKernelGGL((KERNEL<float, HDP>), grid, 256, 0, S(stream), a);                        \
+    })                                                                                                  \
+    CAPK_LAUNCH_CHECK(#KERNEL);                                                                         \
+  }
 
 extern "C" int capk_kv4_append(int dtype, int B, int n, int Hk, int hd, const void* k, int64_t k_bs, int64_t k_rs,
                                int64_t k_hs, const void* v, int64_t v_bs, int64_t v_rs, int64_t v_hs, void* codes,
@@ -122,9 +140,7 @@ extern "C" int capk_kv4_append(int dtype, int B, int n, int Hk, int hd, const vo
   if (rc) return rc;
   if (B == 0 || n == 0) return CAPK_OK;
   CAPK_CHECK_ARG(start, "capk_kv4_append: start");
-  if (dtype == CAPK_BF16) hipLaunchKernelGGL(kv4_append<bf16>, kv4_blocks(a), 256, 0, S(stream), a);
-  else hipLaunchKernelGGL(kv4_append<float>, kv4_blocks(a), 256, 0, S(stream), a);
-  CAPK_LAUNCH_CHECK("kv4_append");
+  KV4_LAUNCH(kv4_append);
   return CAPK_OK;
 }
 
@@ -138,9 +154,7 @@ extern "C" int capk_kv4_read(int dtype, int B, int n, int Hk, int hd, const void
   if (rc) return rc;
   if (B == 0 || n == 0) return CAPK_OK;
   CAPK_CHECK_ARG(start, "capk_kv4_read: start");
-  if (dtype == CAPK_BF16) hipLaunchKernelGGL(kv4_read<bf16>, kv4_blocks(a), 256, 0, S(stream), a);
-  else hipLaunchKernelGGL(kv4_read<float>, kv4_blocks(a), 256, 0, S(stream), a);
-  CAPK_LAUNCH_CHECK("kv4_read");
+  KV4_LAUNCH(kv4_read);
   return CAPK_OK;
 }
 

@@ -20,6 +20,7 @@ struct RopeSide {
 };
 struct RopeArgs {
   int B, N, hd, pairs, axes, tokens;  // tokens: per workgroup
+  uint32_t per_mul, heads_mul;        // ceil(2^32 / .) of the items of a head and of the heads
   const int32_t* pos;
   int64_t pos_as, pos_bs;
   const double* freq;
@@ -44,71 +45,87 @@ __device__ __forceinline__ void rope_st(T* p, const float (&f)[V]) {
   *(vec*)p = v;
 }
 
-// V pairs per item; the elements past the rotated part are copied V at a time.
+// i / d for i < 2^32 / d, from mul = ceil(2^32 / d) (d = 1: mul wraps to 0); i < 8 tokens x 1024 heads x
+// 512 items and d <= 1024 here
+__device__ __forceinline__ int rope_div(int i, uint32_t mul) { return mul ? (int)__umulhi((uint32_t)i, mul) : i; }
+
+// V pairs per item; the elements past the rotated part are copied V at a time.  A thread loads four items
+// before it stores the first.
 template <typename T, int V, bool INTER>
 __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
-  extern __shared__ float2 cs[];  // [tokens][pairs]
+  constexpr int U = 4;
+  extern __shared__ float2 cs[];  // [tokens][pairs], then [tokens][4] row offsets: q in, q out, k in, k out
+  int64_t* offs = (int64_t*)(cs + a.tokens * a.pairs);
   const int64_t t0 = (int64_t)blockIdx.x * a.tokens, all = (int64_t)a.B * a.N;
   const int nt = (int)min((int64_t)a.tokens, all - t0);
   for (int i = threadIdx.x; i < nt * a.pairs; i += 256) {
-    const int64_t t = t0 + i / a.pairs;
+    const int64_t t = t0 + i / a.pairs, b = t / a.N, n = t % a.N;
     const int p = i % a.pairs, ax = min((int)a.axis[p], a.axes - 1);
-    const int pos = a.pos[ax * a.pos_as + (t / a.N) * a.pos_bs + t % a.N];
+    const int pos = a.pos[ax * a.pos_as + b * a.pos_bs + n];
     const double turns = (double)pos * a.freq[p] * 0.15915494309189535;
     float s, c;
     sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
     cs[i] = make_float2(c, s * a.sign);
   }
+  if ((int)threadIdx.x < nt * 4) {
+    const int64_t t = t0 + threadIdx.x / 4, b = t / a.N, n = t % a.N;
+    const RopeSide& s = a.side[threadIdx.x >> 1 & 1];
+    offs[threadIdx.x] = threadIdx.x & 1 ? b * s.y_bs + n * s.y_rs : b * s.x_bs + n * s.x_rs;
+  }
   __syncthreads();
   const int rot = 2 * a.pairs, nrot = a.pairs / V, per = nrot + (a.hd - rot) / V;
-  const int heads = a.side[0].H + a.side[1].H;
-  for (int i = threadIdx.x; i < nt * heads * per; i += 256) {
-    const int c = i % per, hh = (i / per) % heads, tl = i / (per * heads);
-    const int64_t t = t0 + tl, b = t / a.N, n = t % a.N;
-    const RopeSide& s = a.side[hh >= a.side[0].H];
-    const int h = hh >= a.side[0].H ? hh - a.side[0].H : hh;
-    const T* x = (const T*)s.x + b * s.x_bs + n * s.x_rs + h * s.x_hs;
-    T* y = (T*)s.y + b * s.y_bs + n * s.y_rs + h * s.y_hs;
-    float u[V], w[V];
-    if (c >= nrot) {
-      const int d = rot + (c - nrot) * V;
-      rope_ld<T, V>(x + d, u);
-      rope_st<T, V>(y + d, u);
-      continue;
-    }
-    const float2* r = cs + tl * a.pairs + c * V;
-    const int d1 = INTER ? 2 * c * V : c * V, d2 = INTER ? d1 + V : d1 + a.pairs;
-    rope_ld<T, V>(x + d1, u);
-    rope_ld<T, V>(x + d2, w);
-    if (INTER) {  // the 2V elements are V pairs (x1, x2) in a row
-      float z[2 * V];
+  const int heads = a.side[0].H + a.side[1].H, items = nt * heads * per;
+  for (int base = threadIdx.x; base < items; base += 256 * U) {
+    float x1[U][V], x2[U][V];
+    T* out[U];
+    int d2[U], tr[U];  // second element's offset (0: a copy), the item's first (cos, sin)
 #pragma unroll
-      for (int k = 0; k < V; ++k) { z[k] = u[k]; z[V + k] = w[k]; }
+    for (int u = 0; u < U; ++u) {
+      const int i = min(base + u * 256, items - 1);
+      const int th = rope_div(i, a.per_mul), c = i - th * per, tl = rope_div(th, a.heads_mul), hh = th - tl * heads;
+      const bool k = hh >= a.side[0].H, copy = c >= nrot;
+      const RopeSide& s = a.side[k];
+      const int h = k ? hh - a.side[0].H : hh, d1 = copy ? rot + (c - nrot) * V : INTER ? 2 * c * V : c * V;
+      const T* x = (const T*)s.x + offs[tl * 4 + 2 * k] + h * s.x_hs + d1;
+      out[u] = (T*)s.y + offs[tl * 4 + 2 * k + 1] + h * s.y_hs + d1;
+      d2[u] = copy ? 0 : INTER ? V : a.pairs;
+      tr[u] = copy ? 0 : tl * a.pairs + c * V;
+      rope_ld<T, V>(x, x1[u]);
+      rope_ld<T, V>(x + d2[u], x2[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (base + u * 256 >= items) break;
+      if (d2[u] == 0) {
+        rope_st<T, V>(out[u], x1[u]);
+        continue;
+      }
+      const float2* r = cs + tr[u];
+      float y1[V], y2[V];
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        const float x1 = z[2 * k], x2 = z[2 * k + 1];
-        z[2 * k] = x1 * r[k].x - x2 * r[k].y;
-        z[2 * k + 1] = x1 * r[k].y + x2 * r[k].x;
+        // interleaved: the 2V elements are V pairs (x1, x2) in a row
+        const float f = INTER ? (2 * k < V ? x1[u][2 * k % V] : x2[u][2 * k % V]) : x1[u][k];
+        const float g = INTER ? (2 * k + 1 < V ? x1[u][(2 * k + 1) % V] : x2[u][(2 * k + 1) % V]) : x2[u][k];
+        const float p = f * r[k].x - g * r[k].y, q = f * r[k].y + g * r[k].x;
+        if (INTER) {
+          (2 * k < V ? y1[2 * k % V] : y2[2 * k % V]) = p;
+          (2 * k + 1 < V ? y1[(2 * k + 1) % V] : y2[(2 * k + 1) % V]) = q;
+        } else {
+          y1[k] = p;
+          y2[k] = q;
+        }
       }
-#pragma unroll
-      for (int k = 0; k < V; ++k) { u[k] = z[k]; w[k] = z[V + k]; }
-    } else {
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const float x1 = u[k], x2 = w[k];
-        u[k] = x1 * r[k].x - x2 * r[k].y;
-        w[k] = x1 * r[k].y + x2 * r[k].x;
-      }
+      rope_st<T, V>(out[u], y1);
+      rope_st<T, V>(out[u] + d2[u], y2);
     }
-    rope_st<T, V>(y + d1, u);
-    rope_st<T, V>(y + d2, w);
   }
 }
 
 template <typename T>
 static int rope_launch(const RopeArgs& a, int V, bool inter, hipStream_t st) {
   const int grid = cdiv((int64_t)a.B * a.N, a.tokens);
-  const size_t shm = (size_t)a.tokens * a.pairs * sizeof(float2);
+  const size_t shm = (size_t)a.tokens * (a.pairs * sizeof(float2) + 4 * sizeof(int64_t));
 #define ROPE_CASE(v)                                                                            \
   case v:                                                                                       \
     if (inter) hipLaunchKernelGGL((rope_kernel<T, v, true>), grid, 256, shm, st, a);            \
@@ -136,8 +153,8 @@ extern "C" int capk_axis_rope(int dtype, int B, int N, int hd, int pairs, int in
                               int64_t ko_hs, void* stream) {
   CAPK_CHECK_ARG(dtype == CAPK_F32 || dtype == CAPK_BF16, "capk_axis_rope: dtype");
   CAPK_CHECK_ARG(B >= 0 && N >= 0 && Hq >= 1 && Hk >= 0 && axes >= 1 && axes <= 255, "capk_axis_rope: bad sizes");
-  CAPK_CHECK_ARG(hd >= 2 && hd <= 1024 && pairs >= 1 && 2 * pairs <= hd,
-                 "capk_axis_rope: need 2 <= 2 * pairs <= hd <= 1024 (pairs %d, hd %d)", pairs, hd);
+  CAPK_CHECK_ARG(hd >= 2 && hd <= 512 && pairs >= 1 && 2 * pairs <= hd,
+                 "capk_axis_rope: need 2 <= 2 * pairs <= hd <= 512 (pairs %d, hd %d)", pairs, hd);
   if (B == 0 || N == 0) return CAPK_OK;
   CAPK_CHECK_ARG(pos && freq && axis && q && qo && (Hk == 0 || (k && ko)), "capk_axis_rope: null pointer");
   RopeArgs a{};
@@ -163,7 +180,10 @@ extern "C" int capk_axis_rope(int dtype, int B, int N, int hd, int pairs, int in
   // tokens per workgroup: enough workgroups for every CU first, then up to 8 to share the launch
   const int64_t all = (int64_t)B * N;
   a.tokens = (int)(all / 2048 < 1 ? 1 : all / 2048 > 8 ? 8 : all / 2048);
-  CAPK_CHECK_ARG(cdiv(all, a.tokens) < (1 << 30), "capk_axis_rope: too many tokens");
+  CAPK_CHECK_ARG(all / a.tokens < (1 << 30) && Hq + (int64_t)Hk <= 1024, "capk_axis_rope: too many tokens or heads");
+  const int per = pairs / V + (hd - 2 * pairs) / V, heads = Hq + Hk;
+  a.per_mul = (uint32_t)(((1ull << 32) + per - 1) / per);
+  a.heads_mul = (uint32_t)(((1ull << 32) + heads - 1) / heads);
   return dtype == CAPK_BF16 ? rope_launch<bf16>(a, V, interleaved != 0, S(stream))
                             : rope_launch<float>(a, V, interleaved != 0, S(stream));
 }

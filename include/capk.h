@@ -672,7 +672,7 @@ int capk_rowscale_add(int dtype, int rows, int cols, const void* x, int64_t ldx,
  *   freq fp64, axis uint8 < axes): (x1, x2) -> (x1 cos - x2 sin, x1 sin + x2 cos), angles in
  *   64 bits.  interleaved = 0: pair i = elements i, i + pairs; 1: 2i, 2i + 1.  Elements from
  *   2*pairs on are copied.  inverse = 1 turns back (the gradient).  q and k (Hk = 0: none) in one
- *   launch; y may be x.  Any alignment (whole vectors where it allows).  hd <= 1024. */
+ *   launch; y may be x.  Any alignment (whole vectors where it allows).  hd <= 512, Hq + Hk <= 1024. */
 int capk_axis_rope(int dtype, int B, int N, int hd, int pairs, int interleaved, int inverse, int axes,
                    const int32_t* pos, int64_t pos_as, int64_t pos_bs, const double* freq, const uint8_t* axis,
                    int Hq, const void* q, int64_t q_bs, int64_t q_rs, int64_t q_hs, void* qo, int64_t qo_bs,

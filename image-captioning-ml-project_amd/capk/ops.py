@@ -1293,6 +1293,8 @@ def _index(what, t, shape, dtype, dev):
         raise _lib.CapkError(f"{what} on {t.device}, the operands on {dev}")
     if t.shape != shape or t.dtype.is_floating_point or t.dtype.is_complex:
         raise ValueError(f"{what}: need integers of shape {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    if t.dtype == torch.bool and dtype == torch.uint8:
+        return t.contiguous().view(torch.uint8)
     return t if t.dtype == dtype and t.is_contiguous() else t.to(dtype).contiguous()
 
 

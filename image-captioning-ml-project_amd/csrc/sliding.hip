@@ -50,11 +50,12 @@ struct SlideBlock {
 };
 
 template <typename T, int HDP>
-__device__ __forceinline__ void slide_frags(typename Tile<T>::V8 (&f)[HDP / 16], const T* src, bool ok, int hd, int h) {
+__device__ __forceinline__ void slide_frags(typename Mat<T>::V8 (&f)[HDP / 16], const T* src, bool ok, int hd, int h) {
 #pragma unroll
   for (int s = 0; s < HDP / 16; ++s) {
-    f[s] = tile_zero8<T>();
-    if (ok && s * 16 + h * 8 < hd) f[s] = Tile<T>::load(src + s * 16 + h * 8);
+    typename Tile<T>::V8 x = tile_zero8<T>();
+    if (ok && s * 16 + h * 8 < hd) x = Tile<T>::load(src + s * 16 + h * 8);
+    f[s] = Mat<T>::from(x);
   }
 }
 template <typename T, int HDP>
@@ -101,16 +102,16 @@ template <typename T, int HDP> struct SlideKV {
   }
 };
 
-// which keys of a tile the 32 queries at pw_lo.. see: none, all, or some
-__device__ __forceinline__ bool slide_none(const SlideArgs& a, int j0, int pw_lo, int pw_hi) {
-  return j0 > pw_hi || (j0 >= a.sinks && pw_lo - (j0 + 63) >= a.window);
+// whether queries at positions p_lo..p_hi see none, or all, of the keys j0 .. j0 + n - 1
+__device__ __forceinline__ bool slide_none(const SlideArgs& a, int j0, int n, int p_lo, int p_hi) {
+  return j0 > p_hi || (j0 >= a.sinks && p_lo - (j0 + n - 1) >= a.window);
 }
-__device__ __forceinline__ bool slide_full(const SlideArgs& a, int j0, int pw_lo, int pw_hi, uint64_t hid) {
-  return hid == 0 && j0 + 63 <= pw_lo && (j0 + 64 <= a.sinks || pw_hi - j0 < a.window);
+__device__ __forceinline__ bool slide_full(const SlideArgs& a, int j0, int n, int p_lo, int p_hi) {
+  return j0 + n - 1 <= p_lo && (j0 + n <= a.sinks || p_hi - j0 < a.window);
 }
 
 template <typename T, int HDP>
-__global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void slide_fwd(SlideArgs a) {
+__global__ __launch_bounds__(256, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) : HDP <= 96 ? 3 : 2) void slide_fwd(SlideArgs a) {
   using KV = SlideKV<T, HDP>;
   using Img = typename KV::Img;
   constexpr int NS = HDP / 16, ND = HDP / 32;
@@ -127,7 +128,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void s
   KV kv{a, row<T>(a.k, b, 0, kvh), row<T>(a.v, b, 0, kvh), b, len, p_lo, p_hi, min(len, p_hi + 1) - 1, w, lane, smem, 0};
   if (tiles.n) kv.fetch(tiles.key0(0), 0);
 
-  typename Tile<T>::V8 qf[NS];
+  typename Mat<T>::V8 qf[NS];
   slide_frags<T, HDP>(qf, row<T>(a.q, b, qi, h), qi < a.Nq, a.hd, hh);
   f32x16 o[ND];
 #pragma unroll
@@ -139,15 +140,15 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void s
     const int j0 = tiles.key0(t);
     const char *ki = kv.arrive(j0, t & 1), *vi = ki + Img::bytes(64);
     if (t + 1 < tiles.n) kv.fetch(tiles.key0(t + 1), (t + 1) & 1);
-    if (slide_none(a, j0, pw_lo, pw_hi)) continue;
+    if (slide_none(a, j0, 64, pw_lo, pw_hi)) continue;
     f32x16 s[2];
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
       s[kb] = tile_zero<f32x16>();
 #pragma unroll
-      for (int st = 0; st < NS; ++st) s[kb] = Tile<T>::mma32(Img::frag(ki, kb * 32, st, ln), qf[st], s[kb]);
+      for (int st = 0; st < NS; ++st) s[kb] = Mat<T>::mma32(Img::frag(ki, kb * 32, st, ln), qf[st], s[kb]);
     }
-    if (!slide_full(a, j0, pw_lo, pw_hi, kv.hid)) {
+    if (kv.hid || !slide_full(a, j0, 64, pw_lo, pw_hi)) {
       const uint32_t hid[2] = {(uint32_t)kv.hid >> (4 * hh), (uint32_t)(kv.hid >> 32) >> (4 * hh)};
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
@@ -173,19 +174,20 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void s
     }
     const float ms = mc == -INFINITY ? 0.f : mc;
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
+    for (int kb = 0; kb < 2; ++kb) {
 #pragma unroll
       for (int st = 0; st < 2; ++st) {
-        typename Tile<T>::V8 pf;
+        float x[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float x = tile_exp2(fmaf(s[kb][st * 8 + e], c, -ms));
-          l += x;
-          pf[e] = (T)x;
+          x[e] = tile_exp2(fmaf(s[kb][st * 8 + e], c, -ms));
+          l += x[e];
         }
+        const typename Mat<T>::V8 pf = Mat<T>::pack(x);
 #pragma unroll
-        for (int d = 0; d < ND; ++d) o[d] = Tile<T>::mma32(Img::trans(vi, kb * 32 + st * 16, d * 32, ln), pf, o[d]);
+        for (int d = 0; d < ND; ++d) o[d] = Mat<T>::mma32(Img::trans(vi, kb * 32 + st * 16, d * 32, ln), pf, o[d]);
       }
+    }
   }
   l += __shfl_xor(l, 32, 64);
   if (qi >= a.Nq) return;
@@ -195,7 +197,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void s
 }
 
 template <typename T, int HDP>
-__global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void slide_dq(SlideArgs a) {
+__global__ __launch_bounds__(256, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) : HDP <= 64 ? 3 : 2) void slide_dq(SlideArgs a) {
   using KV = SlideKV<T, HDP>;
   using Img = typename KV::Img;
   constexpr int NS = HDP / 16, ND = HDP / 32;
@@ -212,7 +214,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void s
   KV kv{a, row<T>(a.k, b, 0, kvh), row<T>(a.v, b, 0, kvh), b, len, p_lo, p_hi, min(len, p_hi + 1) - 1, w, lane, smem, 0};
   if (tiles.n) kv.fetch(tiles.key0(0), 0);
 
-  typename Tile<T>::V8 qf[NS], dof[NS];
+  typename Mat<T>::V8 qf[NS], dof[NS];
   slide_frags<T, HDP>(qf, row<T>(a.q, b, qi, h), qi < a.Nq, a.hd, hh);
   slide_frags<T, HDP>(dof, row<T>(a.dout, b, qi, h), qi < a.Nq, a.hd, hh);
   const int64_t stat = ((int64_t)b * a.H + h) * a.Nq + qi;
@@ -223,33 +225,35 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void s
   const bool walk = tiles.n <= 4;
   float delta = 0.f;
   if (!walk) {
-    typename Tile<T>::V8 of[NS];
-    slide_frags<T, HDP>(of, row<T>(a.o, b, qi, h), qi < a.Nq, a.hd, hh);
+    const T *o = row<T>(a.o, b, qi, h), *d = row<T>(a.dout, b, qi, h);
 #pragma unroll
     for (int s = 0; s < NS; ++s)
+      if (qi < a.Nq && s * 16 + hh * 8 < a.hd) {
+        const typename Tile<T>::V8 x = Tile<T>::load(o + s * 16 + hh * 8), y = Tile<T>::load(d + s * 16 + hh * 8);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) delta = fmaf((float)of[s][e], (float)dof[s][e], delta);
+        for (int e = 0; e < 8; ++e) delta = fmaf((float)x[e], (float)y[e], delta);
+      }
     delta += __shfl_xor(delta, 32, 64);
   }
   f32x16 dq[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) dq[d] = tile_zero<f32x16>();
   // P and do v^T of 32 keys of a tile, zeros where the query does not see the key
-  auto scores = [&](const char* ki, const char* vi, int j0, int kb, bool full, f32x16& s, f32x16& dp) {
+  auto scores = [&](const char* ki, const char* vi, int j0, int kb, f32x16& s, f32x16& dp) {
+    const uint32_t hidden = (uint32_t)(kv.hid >> (32 * kb));
     s = dp = tile_zero<f32x16>();
 #pragma unroll
     for (int st = 0; st < NS; ++st) {
-      s = Tile<T>::mma32(Img::frag(ki, kb * 32, st, ln), qf[st], s);
-      dp = Tile<T>::mma32(Img::frag(vi, kb * 32, st, ln), dof[st], dp);
+      s = Mat<T>::mma32(Img::frag(ki, kb * 32, st, ln), qf[st], s);
+      dp = Mat<T>::mma32(Img::frag(vi, kb * 32, st, ln), dof[st], dp);
     }
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = tile_exp2(fmaf(s[i], c, -lse2));
-    if (!full) {
-      const uint32_t hid = (uint32_t)(kv.hid >> (32 * kb)) >> (4 * hh);
+    if (hidden || !slide_full(a, j0 + kb * 32, 32, pw_lo, pw_hi)) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int r = 8 * (i >> 2) + (i & 3);
-        const bool sees = slide_sees(a, p, j0 + kb * 32 + 4 * hh + r) & !(hid >> r & 1);
+        const bool sees = slide_sees(a, p, j0 + kb * 32 + 4 * hh + r) & !(hidden >> (4 * hh + r) & 1);
         s[i] = sees ? s[i] : 0.f;
         dp[i] = sees ? dp[i] : 0.f;
       }
@@ -261,12 +265,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void s
       const int j0 = tiles.key0(t);
       const char *ki = kv.arrive(j0, buf), *vi = ki + Img::bytes(64);
       kv.fetch(tiles.key0(t + 1 < tiles.n ? t + 1 : 0), buf ^ 1);
-      if (slide_none(a, j0, pw_lo, pw_hi)) continue;
-      const bool full = slide_full(a, j0, pw_lo, pw_hi, kv.hid);
 #pragma unroll 1
       for (int kb = 0; kb < 2; ++kb) {
+        if (slide_none(a, j0 + kb * 32, 32, pw_lo, pw_hi)) continue;
         f32x16 s, dp;
-        scores(ki, vi, j0, kb, full, s, dp);
+        scores(ki, vi, j0, kb, s, dp);
 #pragma unroll
         for (int i = 0; i < 16; ++i) delta = fmaf(s[i], dp[i], delta);
       }
@@ -277,19 +280,19 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void s
     const int j0 = tiles.key0(t);
     const char *ki = kv.arrive(j0, buf), *vi = ki + Img::bytes(64);
     if (t + 1 < tiles.n) kv.fetch(tiles.key0(t + 1), buf ^ 1);
-    if (slide_none(a, j0, pw_lo, pw_hi)) continue;
-    const bool full = slide_full(a, j0, pw_lo, pw_hi, kv.hid);
 #pragma unroll 1
     for (int kb = 0; kb < 2; ++kb) {
+      if (slide_none(a, j0 + kb * 32, 32, pw_lo, pw_hi)) continue;
       f32x16 s, dp;
-      scores(ki, vi, j0, kb, full, s, dp);
+      scores(ki, vi, j0, kb, s, dp);
 #pragma unroll
       for (int st = 0; st < 2; ++st) {
-        typename Tile<T>::V8 df;
+        float x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) df[e] = (T)(s[st * 8 + e] * (dp[st * 8 + e] - delta));
+        for (int e = 0; e < 8; ++e) x[e] = s[st * 8 + e] * (dp[st * 8 + e] - delta);
+        const typename Mat<T>::V8 df = Mat<T>::pack(x);
 #pragma unroll
-        for (int d = 0; d < ND; ++d) dq[d] = Tile<T>::mma32(Img::trans(ki, kb * 32 + st * 16, d * 32, ln), df, dq[d]);
+        for (int d = 0; d < ND; ++d) dq[d] = Mat<T>::mma32(Img::trans(ki, kb * 32 + st * 16, d * 32, ln), df, dq[d]);
       }
     }
   }
@@ -337,7 +340,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void s
     ld = stat[(int64_t)h * a.Nq + min(q0 + lane, qb - 1)];
   };
   if (all) fetch(0, 0);
-  typename Tile<T>::V8 kf[NS], vf[NS];
+  typename Mat<T>::V8 kf[NS], vf[NS];
   slide_frags<T, HDP>(kf, row<T>(a.k, b, j, kvh), key_ok, a.hd, hh);
   slide_frags<T, HDP>(vf, row<T>(a.v, b, j, kvh), key_ok, a.hd, hh);
   const bool hidden = __builtin_amdgcn_ballot_w64(!key_ok) != 0;
@@ -352,17 +355,17 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void s
     if (w < 2) Ls[(t & 1) * 128 + threadIdx.x] = q0 + lane >= qb ? (w ? 0.f : INFINITY) : (w ? ld : ld * kTileLog2e);
     __syncthreads();
     if (t + 1 < all) fetch(t + 1, (t + 1) & 1);
-    // no query of this tile sees a key of this wave
-    if (p0 + QT - 1 < jw || (jw >= a.sinks && p0 - (jw + 31) >= a.window)) continue;
-    const bool full = !hidden && q0 + QT <= qb && jw + 31 <= p0 && (jw + 32 <= a.sinks || p0 + QT - 1 - jw < a.window);
 #pragma unroll 1
     for (int qt = 0; qt < 2; ++qt) {
+      const int pq = p0 + qt * 32;
+      if (slide_none(a, jw, 32, pq, pq + 31)) continue;
+      const bool full = !hidden && q0 + qt * 32 + 32 <= qb && slide_full(a, jw, 32, pq, pq + 31);
       if constexpr (sizeof(T) == 2) ln.forget();
       f32x16 s = tile_zero<f32x16>(), dp = tile_zero<f32x16>();
 #pragma unroll
       for (int st = 0; st < NS; ++st) {
-        s = Tile<T>::mma32(Img::frag(qi, qt * 32, st, ln), kf[st], s);
-        dp = Tile<T>::mma32(Img::frag(di, qt * 32, st, ln), vf[st], dp);
+        s = Mat<T>::mma32(Img::frag(qi, qt * 32, st, ln), kf[st], s);
+        dp = Mat<T>::mma32(Img::frag(di, qt * 32, st, ln), vf[st], dp);
       }
 #pragma unroll
       for (int i4 = 0; i4 < 4; ++i4) {
@@ -387,13 +390,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void s
       }
 #pragma unroll
       for (int st = 0; st < 2; ++st) {
-        typename Tile<T>::V8 pf, df;
+        float x[8], y[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) { pf[e] = (T)s[st * 8 + e]; df[e] = (T)dp[st * 8 + e]; }
+        for (int e = 0; e < 8; ++e) { x[e] = s[st * 8 + e]; y[e] = dp[st * 8 + e]; }
+        const typename Mat<T>::V8 pf = Mat<T>::pack(x), df = Mat<T>::pack(y);
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
-          dv[d] = Tile<T>::mma32(Img::trans(di, qt * 32 + st * 16, d * 32, ln), pf, dv[d]);
-          dk[d] = Tile<T>::mma32(Img::trans(qi, qt * 32 + st * 16, d * 32, ln), df, dk[d]);
+          dv[d] = Mat<T>::mma32(Img::trans(di, qt * 32 + st * 16, d * 32, ln), pf, dv[d]);
+          dk[d] = Mat<T>::mma32(Img::trans(qi, qt * 32 + st * 16, d * 32, ln), df, dk[d]);
         }
       }
     }

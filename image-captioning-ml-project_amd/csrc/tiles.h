@@ -2,8 +2,8 @@
 //
 // A fragment is 8 values per lane.  In a 32x32 product lane l holds row (A) or column (B) l & 31 and
 // the contraction slots (h = l >> 5, e = 0..7) of a 16-deep step; in a 16x16 product row / column
-// l & 15 and slots (g = l >> 4, e) of a 32-deep step.  bf16 runs one instruction per step; fp32 runs
-// eight 2-deep (4-deep) ones, the e-th over slots (., e), so both types share every index below.
+// l & 15 and slots (g = l >> 4, e) of a 32-deep step.  bf16 runs one instruction per step; the fp32 form of
+// the latter runs eight 4-deep ones, the e-th over slots (., e), so both types share every index below.
 // Accumulators: 32x32: lane column l & 31, register i row 8 (i >> 2) + 4 h + (i & 3);
 // 16x16: lane column l & 15, register i row 4 g + i.
 #pragma once
@@ -36,17 +36,57 @@ template <> struct Tile<float> {
     const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
     return (V8){a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
   }
-  __device__ __forceinline__ static f32x16 mma32(V8 a, V8 b, f32x16 c) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
-    return c;
-  }
   __device__ __forceinline__ static f32x4 mma16(V8 a, V8 b, f32x4 c) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
     return c;
   }
   __device__ __forceinline__ static void store4(float* p, f32x4 v) { *(f32x4*)p = v; }
+};
+
+// The operands of the attention products.  bf16 values are fragments as they are.  An fp32 value goes through
+// the bf16 unit as three bf16 parts, x = h + m + l to 2^-26 of it, and a product as the six part products
+// above 2^-26: 6 x 32 clocks for a 32x32x16 step, where the fp32 instructions take 8 x 64.
+struct Split8 {
+  bf16x8 h, m, l;
+};
+template <typename T> struct Mat;
+template <> struct Mat<bf16> {
+  using V8 = bf16x8;
+  __device__ __forceinline__ static V8 pack(const float (&x)[8]) {
+    V8 r;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r[e] = (bf16)x[e];
+    return r;
+  }
+  __device__ __forceinline__ static V8 from(bf16x8 x) { return x; }
+  __device__ __forceinline__ static f32x16 mma32(const V8& a, const V8& b, f32x16 c) { return Tile<bf16>::mma32(a, b, c); }
+};
+template <> struct Mat<float> {
+  using V8 = Split8;
+  __device__ __forceinline__ static V8 pack(const float (&x)[8]) {
+    V8 r;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      r.h[e] = (bf16)x[e];
+      const float y = x[e] - (float)r.h[e];
+      r.m[e] = (bf16)y;
+      r.l[e] = (bf16)(y - (float)r.m[e]);
+    }
+    return r;
+  }
+  __device__ __forceinline__ static V8 from(f32x8 x) {
+    const float y[8] = {x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]};
+    return pack(y);
+  }
+  __device__ __forceinline__ static f32x16 mma32(const V8& a, const V8& b, f32x16 c) {
+    c = Tile<bf16>::mma32(a.h, b.l, c);
+    c = Tile<bf16>::mma32(a.l, b.h, c);
+    c = Tile<bf16>::mma32(a.m, b.m, c);
+    c = Tile<bf16>::mma32(a.h, b.m, c);
+    c = Tile<bf16>::mma32(a.m, b.h, c);
+    return Tile<bf16>::mma32(a.h, b.h, c);
+  }
 };
 
 template <typename T> __device__ __forceinline__ typename Tile<T>::V8 tile_zero8() {
@@ -127,20 +167,21 @@ template <typename T, int HDP> struct TileImg {
   static constexpr bool POW2 = (RB & (RB - 1)) == 0;
   // A / B fragment of a 32x32 product: row r0 + (l & 31), columns 16 s + 8 h (r0 a multiple of 32).  Chunks
   // 2 s (fp32: 4 s) beside the mask: an exclusive or, where rows are not a power of two of its masked bits.
-  __device__ __forceinline__ static typename Tile<T>::V8 frag(const char* img, int r0, int s, const Lane& l) {
+  __device__ __forceinline__ static typename Mat<T>::V8 frag(const char* img, int r0, int s, const Lane& l) {
     if constexpr (sizeof(T) == 2) {
       const int o = POW2 ? l.f ^ (s * 32) : (l.f ^ ((s & 1) * 32)) + (s >> 1) * 64;
       return *(const bf16x8*)(img + r0 * RB + o);
     } else {
       const int o = POW2 ? l.f ^ (s * 64) : (l.f ^ ((s & 1) * 64)) + (s >> 1) * 128;
       const f32x4 x = *(const f32x4*)(img + r0 * RB + o), y = *(const f32x4*)(img + r0 * RB + (o ^ 16));
-      return (f32x8){x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+      const float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+      return Mat<float>::pack(v);
     }
   }
   // A fragment of the transpose for a 32x32 product: lane column c0 + (l & 31), slot (h, e) = row
   // r0 + 8 (e >> 2) + 4 h + (e & 3) -- the order in which eight accumulator registers of a 32x32
   // product hold their rows (r0 a multiple of 16, c0 of 32).
-  __device__ __forceinline__ static typename Tile<T>::V8 trans(const char* img, int r0, int c0, const Lane& l) {
+  __device__ __forceinline__ static typename Mat<T>::V8 trans(const char* img, int r0, int c0, const Lane& l) {
     if constexpr (sizeof(T) == 2) {
       const char *a = img + r0 * RB + (POW2 ? l.ta ^ (c0 * 2) : l.ta + c0 * 2), *b = img + r0 * RB + (POW2 ? l.tb ^ (c0 * 2) : l.tb + c0 * 2);
       const bf16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, a));
@@ -148,13 +189,13 @@ template <typename T, int HDP> struct TileImg {
       return (bf16x8){x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
     } else {
       const int d = c0 + l.tb;
-      f32x8 v;
+      float v[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int r = 8 * (e >> 2) + 4 * l.ta + (e & 3);
         v[e] = *(const float*)(img + (r0 + r) * RB + (((d / 4) ^ swz(r)) << 4) + (d & 3) * 4);
       }
-      return v;
+      return Mat<float>::pack(v);
     }
   }
 };

@@ -58,6 +58,10 @@ __device__ __forceinline__ void slide_frags(typename Mat<T>::V8 (&f)[HDP / 16], 
     f[s] = Mat<T>::from(x);
   }
 }
+template <typename V, int N> __device__ __forceinline__ void slide_settle(V (&f)[N]) {
+#pragma unroll
+  for (int s = 0; s < N; ++s) tile_settle(f[s]);
+}
 template <typename T, int HDP>
 __device__ __forceinline__ void slide_store(T* dst, const f32x16 (&acc)[HDP / 32], float f, int hd, int h) {
 #pragma unroll
@@ -102,6 +106,21 @@ template <typename T, int HDP> struct SlideKV {
   }
 };
 
+// n products whose LDS operands are requested D ahead: the order is written down, as the compiler would
+// request each operand right before its use and wait for it
+template <int D, int N, typename L, typename M> __device__ __forceinline__ void slide_pipe(L load, M mul) {
+  decltype(load(0)) f[D];
+#pragma unroll
+  for (int i = 0; i < D && i < N; ++i) f[i] = load(i);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    __builtin_amdgcn_sched_barrier(0);
+    mul(i, f[i % D]);
+    if (i + D < N) f[i % D] = load(i + D);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+}
+
 // whether queries at positions p_lo..p_hi see none, or all, of the keys j0 .. j0 + n - 1
 __device__ __forceinline__ bool slide_none(const SlideArgs& a, int j0, int n, int p_lo, int p_hi) {
   return j0 > p_hi || (j0 >= a.sinks && p_lo - (j0 + n - 1) >= a.window);
@@ -116,7 +135,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) : HDP <= 
   using Img = typename KV::Img;
   constexpr int NS = HDP / 16, ND = HDP / 32;
   extern __shared__ __align__(16) char smem[];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, hh = lane >> 5;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hh = lane >> 5;
   const SlideBlock at(a);
   const int b = at.b, kvh = at.kvh, G = a.H / a.Hk, h = kvh * G + at.rest % G, len = slide_len(a, b), off = len - a.Nq;
   const int q0 = ((a.Nq + 127) / 128 - 1 - at.rest / G) * 128, qw = q0 + w * 32, qi = qw + (lane & 31), p = off + qi;
@@ -136,18 +155,18 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) : HDP <= 
   // mc: the exponent that the sums are relative to, the running maximum of c s or up to 8 below it (so
   // that o is rescaled when the maximum has grown 2^8-fold, not with every step of it)
   float mc = -INFINITY, l = 0.f;
+  slide_settle(qf);
   for (int t = 0; t < tiles.n; ++t) {
     const int j0 = tiles.key0(t);
     const char *ki = kv.arrive(j0, t & 1), *vi = ki + Img::bytes(64);
     if (t + 1 < tiles.n) kv.fetch(tiles.key0(t + 1), (t + 1) & 1);
     if (slide_none(a, j0, 64, pw_lo, pw_hi)) continue;
-    f32x16 s[2];
+    f32x16 s[2] = {tile_zero<f32x16>(), tile_zero<f32x16>()};
+    slide_pipe<4, 2 * NS>([&](int i) { return Img::frag(ki, (i & 1) * 32, i >> 1, ln); },
+                  [&](int i, const auto& k) { s[i & 1] = Mat<T>::mma32(k, qf[i >> 1], s[i & 1]); });
+    typename Mat<T>::V8 vf[2][ND];  // V^T fragments of a 16-key step, requested a step ahead
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      s[kb] = tile_zero<f32x16>();
-#pragma unroll
-      for (int st = 0; st < NS; ++st) s[kb] = Mat<T>::mma32(Img::frag(ki, kb * 32, st, ln), qf[st], s[kb]);
-    }
+    for (int d = 0; d < ND; ++d) vf[0][d] = Img::trans(vi, 0, d * 32, ln);
     if (kv.hid || !slide_full(a, j0, 64, pw_lo, pw_hi)) {
       const uint32_t hid[2] = {(uint32_t)kv.hid >> (4 * hh), (uint32_t)(kv.hid >> 32) >> (4 * hh)};
 #pragma unroll
@@ -174,19 +193,21 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) : HDP <= 
     }
     const float ms = mc == -INFINITY ? 0.f : mc;
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
+    for (int u = 0; u < 4; ++u) {  // 16 keys each
+      __builtin_amdgcn_sched_barrier(0);
+      if (u < 3)
 #pragma unroll
-      for (int st = 0; st < 2; ++st) {
-        float x[8];
+        for (int d = 0; d < ND; ++d) vf[(u + 1) & 1][d] = Img::trans(vi, (u + 1) * 16, d * 32, ln);
+      __builtin_amdgcn_sched_barrier(0);
+      float x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          x[e] = tile_exp2(fmaf(s[kb][st * 8 + e], c, -ms));
-          l += x[e];
-        }
-        const typename Mat<T>::V8 pf = Mat<T>::pack(x);
-#pragma unroll
-        for (int d = 0; d < ND; ++d) o[d] = Mat<T>::mma32(Img::trans(vi, kb * 32 + st * 16, d * 32, ln), pf, o[d]);
+      for (int e = 0; e < 8; ++e) {
+        x[e] = tile_exp2(fmaf(s[u >> 1][(u & 1) * 8 + e], c, -ms));
+        l += x[e];
       }
+      const typename Mat<T>::V8 pf = Mat<T>::pack(x);
+#pragma unroll
+      for (int d = 0; d < ND; ++d) o[d] = Mat<T>::mma32(vf[u & 1][d], pf, o[d]);
     }
   }
   l += __shfl_xor(l, 32, 64);
@@ -202,7 +223,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) : HDP <= 
   using Img = typename KV::Img;
   constexpr int NS = HDP / 16, ND = HDP / 32;
   extern __shared__ __align__(16) char smem[];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, hh = lane >> 5;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hh = lane >> 5;
   const SlideBlock at(a);
   const int b = at.b, kvh = at.kvh, G = a.H / a.Hk, h = kvh * G + at.rest % G, len = slide_len(a, b), off = len - a.Nq;
   const int q0 = ((a.Nq + 127) / 128 - 1 - at.rest / G) * 128, qw = q0 + w * 32, qi = qw + (lane & 31), p = off + qi;
@@ -238,6 +259,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) : HDP <= 
   f32x16 dq[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) dq[d] = tile_zero<f32x16>();
+  slide_settle(qf);
+  slide_settle(dof);
   // P and do v^T of 32 keys of a tile, zeros where the query does not see the key
   auto scores = [&](const char* ki, const char* vi, int j0, int kb, f32x16& s, f32x16& dp) {
     const uint32_t hidden = (uint32_t)(kv.hid >> (32 * kb));
@@ -310,7 +333,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void s
   constexpr int QT = 64, NS = HDP / 16, ND = HDP / 32, BUF = 2 * Img::bytes(QT);
   extern __shared__ __align__(16) char smem[];
   float* Ls = (float*)(smem + 2 * BUF);  // per buffer: lse (base 2) and D of 64 queries
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, hh = lane >> 5;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hh = lane >> 5;
   const SlideBlock at(a);
   const int b = at.b, kvh = at.kvh, G = a.H / a.Hk, len = slide_len(a, b), off = len - a.Nq;
   const int tiles = (a.Nk + kSlideKeys - 1) / kSlideKeys;
@@ -335,9 +358,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void s
   auto fetch = [&](int t, int buf) {
     const int h = kvh * G + t / nq, q0 = qa + t % nq * QT;
     char* img = smem + buf * BUF;
+    ld = stat[(int64_t)h * a.Nq + min(q0 + lane, qb - 1)];
     Img::template dma<QT, 4>(img, row<T>(a.q, b, 0, h), a.q.rs, q0, qb - 1, a.hd, w, lane);
     Img::template dma<QT, 4>(img + Img::bytes(QT), row<T>(a.dout, b, 0, h), a.dout.rs, q0, qb - 1, a.hd, w, lane);
-    ld = stat[(int64_t)h * a.Nq + min(q0 + lane, qb - 1)];
   };
   if (all) fetch(0, 0);
   typename Mat<T>::V8 kf[NS], vf[NS];
@@ -347,6 +370,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void s
   f32x16 dk[ND], dv[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) dk[d] = dv[d] = tile_zero<f32x16>();
+  slide_settle(kf);
+  slide_settle(vf);
   for (int t = 0; t < all; ++t) {
     const char *qi = smem + (t & 1) * BUF, *di = qi + Img::bytes(QT);
     const float* ls = Ls + (t & 1) * 128;
@@ -451,8 +476,10 @@ static int slide_check(const char* who, int dtype, int B, int H, int Hk, int Nq,
   CAPK_CHECK_ARG(scale > 0.f && scale < INFINITY, "%s: scale must be positive", who);
   const int ea = dtype == CAPK_BF16 ? 8 : 4;
   for (int i = 0; i < n; ++i)
-    CAPK_CHECK_ARG(v[i].p && (uintptr_t)v[i].p % 16 == 0 && v[i].bs % ea == 0 && v[i].rs % ea == 0 && v[i].hs % ea == 0,
-                   "%s: operand %d must be 16-B aligned with strides that keep it so", who, i);
+    CAPK_CHECK_ARG(v[i].p && (uintptr_t)v[i].p % 16 == 0 && v[i].bs % ea == 0 && v[i].rs % ea == 0 && v[i].hs % ea == 0 &&
+                       v[i].rs >= 0 && v[i].rs < (1 << 22),
+                   "%s: operand %d must be 16-B aligned with strides that keep it so, and tokens less than 2^22 elements apart",
+                   who, i);
   return CAPK_OK;
 }
 

@@ -89,6 +89,11 @@ template <> struct Mat<float> {
   }
 };
 
+// Fragments loaded before a loop: waited for here.  Otherwise the compiler waits at their first use, inside
+// the loop and in every turn of it, and with them for the copies that are meant to stay in flight.
+__device__ __forceinline__ void tile_settle(bf16x8& f) { asm volatile("" : "+v"(f)); }
+__device__ __forceinline__ void tile_settle(Split8& f) { asm volatile("" : "+v"(f.h), "+v"(f.m), "+v"(f.l)); }
+
 template <typename T> __device__ __forceinline__ typename Tile<T>::V8 tile_zero8() {
   typename Tile<T>::V8 z;
 #pragma unroll
@@ -121,23 +126,35 @@ template <typename T, int HDP> struct TileImg {
   static constexpr int bytes(int rows) { return rows * RB; }
 
   // Copies rows r0 .. r0 + ROWS - 1 of `src` (row stride rs) into the image, 1 KiB per wave and
-  // instruction; rows past `last` repeat it, columns past hd repeat column 0.  Arrives with vmcnt(0).
+  // instruction; rows past `last` repeat it, columns past hd repeat column 0.  src, img, w and the rows are
+  // the same for the whole wave; 64 rows span less than 2^31 bytes.  The image is there after the issuing
+  // waves waited for vmcnt(0) and met at a barrier.  Written as assembly (it has no destination register):
+  // for the builtin the compiler assumes that any transposed LDS read may touch the copy in flight, and
+  // waits for it there -- in the middle of the tile that the copy is meant to overlap.
   template <int ROWS, int WAVES>
   __device__ __forceinline__ static void dma(char* img, const T* src, int64_t rs, int r0, int last, int hd, int w, int lane) {
     static_assert(ROWS * RB % (1024 * WAVES) == 0, "whole pieces for every wave");
+    constexpr int N = ROWS * RB / 1024 / WAVES;
     constexpr int STEP = 1024 * WAVES / RB;  // rows from one piece of a wave to its next
-    const int o = w * 1024 + lane * 16, r = o / RB, c = (o % RB / 16) ^ swz(r), col = c * PER < hd ? c * PER : 0;
+    constexpr bool SAME = 1024 * WAVES % RB == 0 && STEP % 16 == 0;  // same columns in every piece of a lane
+    const uint32_t lds = (uint32_t)(uintptr_t)LDS_PTR(char, img) + w * 1024, rsb = (uint32_t)(rs * (int)sizeof(T));
+    const char* base = (const char*)(src + (int64_t)r0 * rs);
+    const int left = last - r0;
 #pragma unroll
-    for (int i = 0; i < ROWS * RB / 1024 / WAVES; ++i) {
-      int ri = r + i * STEP, ci = col;
-      if constexpr (1024 * WAVES % RB != 0 || STEP % 16 != 0) {  // the mask changes from piece to piece
-        const int oi = o + i * 1024 * WAVES;
-        ri = oi / RB;
-        ci = ((oi % RB / 16) ^ swz(ri)) * PER;
-        ci = ci < hd ? ci : 0;
+    for (int i = 0; i < N; ++i) {
+      const int o = (SAME ? 0 : i * 1024 * WAVES) + w * 1024 + lane * 16, r = o / RB, c = ((o % RB / 16) ^ swz(r)) * PER;
+      const uint32_t col = (c < hd ? c : 0) * (uint32_t)sizeof(T);
+      uint32_t off = r * rsb + col;
+      const char* at = base;
+      if (SAME) at += (int64_t)(i * STEP) * rsb;
+      if (left < ROWS - 1) {  // the last rows: clamped one by one
+        at = base;
+        off = min(r + (SAME ? i * STEP : 0), left) * rsb + col;
       }
-      __builtin_amdgcn_global_load_lds((const void*)(src + (int64_t)min(r0 + ri, last) * rs + ci),
-                                       (__attribute__((address_space(3))) void*)(img + (i * WAVES + w) * 1024), 16, 0, 0);
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                   :
+                   : "s"(lds + i * WAVES * 1024), "v"(off), "s"(at)
+                   : "memory", "m0");
     }
   }
   // zeros in the rows whose bit of `rows` is set (all 256 threads)

@@ -90,9 +90,11 @@ template <typename T, int HDP> struct SlideKV {
     Img::template dma<KT, 4>(img + Img::bytes(KT), v, a.v.rs, j0, last, a.hd, w, lane);
   }
   // waits for the tile; keys that no query of the workgroup sees become zeros (they may hold anything)
-  __device__ __forceinline__ const char* arrive(int j0, int buf) {
+  // GROUPS = 2: workgroup barriers meet both groups, so both always take two, also without a tile (any = false)
+  template <int GROUPS = 1>
+  __device__ __forceinline__ const char* arrive(int j0, int buf, bool any = true) {
     char* img = smem + buf * BUF;
-    const int j = j0 + lane;
+    const int j = any ? j0 + lane : p_hi;
     hid = __builtin_amdgcn_ballot_w64(j >= len || (a.pad && a.pad[(int64_t)b * a.Nk + j]));
     const uint64_t out = hid | __builtin_amdgcn_ballot_w64(j > p_hi || (j >= a.sinks && p_lo - j >= a.window));
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -100,8 +102,8 @@ template <typename T, int HDP> struct SlideKV {
     if (out) {
       Img::clear(img, out);
       Img::clear(img + Img::bytes(KT), out);
-      __syncthreads();
     }
+    if (GROUPS == 2 || out) __syncthreads();
     return img;
   }
 };
@@ -129,13 +131,15 @@ __device__ __forceinline__ bool slide_full(const SlideArgs& a, int j0, int n, in
   return j0 + n - 1 <= p_lo && (j0 + n <= a.sinks || p_hi - j0 < a.window);
 }
 
-template <typename T, int HDP>
-__global__ __launch_bounds__(256, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) : HDP <= 96 ? 3 : 2) void slide_fwd(SlideArgs a) {
+// GROUPS = 2: a second group of 4 waves, with images of its own, takes every other tile of the same queries.
+template <typename T, int HDP, int GROUPS>
+__global__ __launch_bounds__(256 * GROUPS, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) : GROUPS == 2 || HDP > 96 ? 2 : 3) void slide_fwd(SlideArgs a) {
   using KV = SlideKV<T, HDP>;
   using Img = typename KV::Img;
   constexpr int NS = HDP / 16, ND = HDP / 32;
   extern __shared__ __align__(16) char smem[];
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hh = lane >> 5;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6 & 3), hh = lane >> 5;
+  const int grp = GROUPS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
   const SlideBlock at(a);
   const int b = at.b, kvh = at.kvh, G = a.H / a.Hk, h = kvh * G + at.rest % G, len = slide_len(a, b), off = len - a.Nq;
   const int q0 = ((a.Nq + 127) / 128 - 1 - at.rest / G) * 128, qw = q0 + w * 32, qi = qw + (lane & 31), p = off + qi;
@@ -144,8 +148,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) : HDP <= 
   const float c = a.scale * kTileLog2e;
   typename Img::Lane ln(lane);
   const SlideTiles<64> tiles(a.window, a.sinks, p_lo, p_hi, len);
-  KV kv{a, row<T>(a.k, b, 0, kvh), row<T>(a.v, b, 0, kvh), b, len, p_lo, p_hi, min(len, p_hi + 1) - 1, w, lane, smem, 0};
-  if (tiles.n) kv.fetch(tiles.key0(0), 0);
+  KV kv{a, row<T>(a.k, b, 0, kvh), row<T>(a.v, b, 0, kvh), b, len, p_lo, p_hi, min(len, p_hi + 1) - 1, w, lane, smem + grp * 2 * KV::BUF, 0};
+  if (grp < tiles.n) kv.fetch(tiles.key0(grp), 0);
 
   typename Mat<T>::V8 qf[NS];
   slide_frags<T, HDP>(qf, row<T>(a.q, b, qi, h), qi < a.Nq, a.hd, hh);
@@ -156,10 +160,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) : HDP <= 
   // that o is rescaled when the maximum has grown 2^8-fold, not with every step of it)
   float mc = -INFINITY, l = 0.f;
   slide_settle(qf);
-  for (int t = 0; t < tiles.n; ++t) {
-    const int j0 = tiles.key0(t);
-    const char *ki = kv.arrive(j0, t & 1), *vi = ki + Img::bytes(64);
-    if (t + 1 < tiles.n) kv.fetch(tiles.key0(t + 1), (t + 1) & 1);
+  for (int u = 0; u * GROUPS < tiles.n; ++u) {  // (as many turns, and barriers, in both groups)
+    const int t = u * GROUPS + grp, j0 = tiles.key0(t);
+    const char *ki = kv.template arrive<GROUPS>(j0, u & 1, t < tiles.n), *vi = ki + Img::bytes(64);
+    if (t >= tiles.n) continue;
+    if (t + GROUPS < tiles.n) kv.fetch(tiles.key0(t + GROUPS), (u + 1) & 1);
     if (slide_none(a, j0, 64, pw_lo, pw_hi)) continue;
     f32x16 s[2] = {tile_zero<f32x16>(), tile_zero<f32x16>()};
     slide_pipe<4, 2 * NS>([&](int i) { return Img::frag(ki, (i & 1) * 32, i >> 1, ln); },
@@ -211,6 +216,27 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) : HDP <= 
     }
   }
   l += __shfl_xor(l, 32, 64);
+  if constexpr (GROUPS == 2) {  // the groups' partial softmaxes joined: registers of the second through LDS
+    __syncthreads();
+    float* x = (float*)smem + (threadIdx.x & 255);
+    if (grp == 1) {
+      x[0] = mc;
+      x[256] = l;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[(2 + d * 16 + i) * 256] = o[d][i];
+    }
+    __syncthreads();
+    if (grp == 1) return;
+    const float m1 = x[0], mn = fmaxf(mc, m1), f0 = mn == -INFINITY ? 0.f : tile_exp2(mc - mn), f1 = mn == -INFINITY ? 0.f : tile_exp2(m1 - mn);
+    mc = mn;
+    l = l * f0 + x[256] * f1;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[d][i] = o[d][i] * f0 + x[(2 + d * 16 + i) * 256] * f1;
+  }
   if (qi >= a.Nq) return;
   slide_store<T, HDP>(row<T>(a.o, b, qi, h), o, l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l), a.hd, hh);
   if (a.lse && hh == 0)
@@ -455,12 +481,13 @@ __global__ __launch_bounds__(256) void slide_dkv_sum(SlideArgs a) {
 }
 
 template <typename K>
-static int slide_launch(K kernel, dim3 grid, size_t shm, hipStream_t st, const SlideArgs& a, const char* name) {
+static int slide_launch(K kernel, dim3 grid, size_t shm, hipStream_t st, const SlideArgs& a, const char* name,
+                        int threads = 256) {
   if (shm > 65536) {
     hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)shm);
     if (e != hipSuccess) return hip_status(e, name);
   }
-  hipLaunchKernelGGL(kernel, grid, dim3(256), shm, st, a);
+  hipLaunchKernelGGL(kernel, grid, dim3(threads), shm, st, a);
   CAPK_LAUNCH_CHECK(name);
   return CAPK_OK;
 }
@@ -554,10 +581,16 @@ extern "C" int capk_sliding_attention_fwd(int dtype, int B, int H, int Hk, int N
   if (slide_few(Nq)) return step_launch(dtype, slide_step(a), ws, ws_bytes, S(stream));
   const int hdp = slide_hdp(hd);
   const dim3 grid(cdiv(Nq, 128) * H * B);
+  // up to one workgroup per CU: a second group of waves shares its tiles (117 to 82 us at 256 workgroups of
+  // 66 tiles, heads of 128); fp32 images of wider heads leave no room for it
+  const bool two = grid.x <= 256;
   SLIDE_HD(hdp, {
+    constexpr int B16 = SlideKV<bf16, HDP>::BUF, B32 = SlideKV<float, HDP>::BUF, G32 = HDP <= 64 ? 2 : 1;
     if (dtype == CAPK_BF16)
-      return slide_launch(slide_fwd<bf16, HDP>, grid, 2 * SlideKV<bf16, HDP>::BUF, S(stream), a, "slide_fwd");
-    return slide_launch(slide_fwd<float, HDP>, grid, 2 * SlideKV<float, HDP>::BUF, S(stream), a, "slide_fwd");
+      return two ? slide_launch(slide_fwd<bf16, HDP, 2>, grid, 4 * B16, S(stream), a, "slide_fwd", 512)
+                 : slide_launch(slide_fwd<bf16, HDP, 1>, grid, 2 * B16, S(stream), a, "slide_fwd");
+    return two && G32 == 2 ? slide_launch(slide_fwd<float, HDP, G32>, grid, 2 * G32 * B32, S(stream), a, "slide_fwd", 256 * G32)
+                           : slide_launch(slide_fwd<float, HDP, 1>, grid, 2 * B32, S(stream), a, "slide_fwd");
   });
 }
 

@@ -59,6 +59,7 @@ template <> struct Mat<bf16> {
     for (int e = 0; e < 8; ++e) r[e] = (bf16)x[e];
     return r;
   }
+  __device__ __forceinline__ static void set(V8& r, int e, float x) { r[e] = (bf16)x; }
   __device__ __forceinline__ static V8 from(bf16x8 x) { return x; }
   __device__ __forceinline__ static f32x16 mma32(const V8& a, const V8& b, f32x16 c) { return Tile<bf16>::mma32(a, b, c); }
 };
@@ -67,13 +68,14 @@ template <> struct Mat<float> {
   __device__ __forceinline__ static V8 pack(const float (&x)[8]) {
     V8 r;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      r.h[e] = (bf16)x[e];
-      const float y = x[e] - (float)r.h[e];
-      r.m[e] = (bf16)y;
-      r.l[e] = (bf16)(y - (float)r.m[e]);
-    }
+    for (int e = 0; e < 8; ++e) set(r, e, x[e]);
     return r;
+  }
+  __device__ __forceinline__ static void set(V8& r, int e, float x) {
+    r.h[e] = (bf16)x;
+    const float y = x - (float)r.h[e];
+    r.m[e] = (bf16)y;
+    r.l[e] = (bf16)(y - (float)r.m[e]);
   }
   __device__ __forceinline__ static V8 from(f32x8 x) {
     const float y[8] = {x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]};
@@ -154,12 +156,12 @@ template <typename T, int HDP> struct TileImg {
       asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                    :
                    : "s"(lds + i * WAVES * 1024), "v"(off), "s"(at)
-                   : "memory", "m0");
+                   : "memory");
     }
   }
-  // zeros in the rows whose bit of `rows` is set (all 256 threads)
+  // zeros in the rows whose bit of `rows` is set (256 threads)
   __device__ __forceinline__ static void clear(char* img, uint64_t rows) {
-    for (int o = threadIdx.x * 16; o < 64 * RB; o += 256 * 16)
+    for (int o = (threadIdx.x & 255) * 16; o < 64 * RB; o += 256 * 16)
       if (rows >> (o / RB) & 1) *(f32x4*)(img + o) = (f32x4){0.f, 0.f, 0.f, 0.f};
   }
   // Byte offsets of a lane's reads: of a row fragment, and (bf16) of the two halves of a transposed one.

@@ -8,6 +8,7 @@ eager-PyTorch fallback: a missing library or a non-GPU tensor raises.
 
 import ctypes
 import contextlib
+import functools
 import os
 import threading
 import weakref
@@ -1266,9 +1267,20 @@ def _launch(dev, name, *args):
     if at != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
             return _launch(dev, name, *args)
-    rc = getattr(_lib.load(), name)(*args, torch._C._cuda_getCurrentRawStream(at))
+    rc = _entry(name)(*args, torch._C._cuda_getCurrentRawStream(at))
     if rc:
         check(rc, name)
+
+
+@functools.lru_cache(maxsize=None)
+def _entry(name):
+    return getattr(_lib.load(), name)
+
+
+@functools.lru_cache(maxsize=4096)
+def _ws_bytes(name, *sizes):
+    """A workspace query's answer (it depends on the sizes alone)."""
+    return _entry(name)(*sizes)
 
 
 def _same(what, first, *rest, dtype=True):
@@ -1338,16 +1350,19 @@ def axis_rope(q, k, pos, freq, axis, *, interleaved=False, inverse=False, out_q=
 
 
 def _sliding_args(what, q, k, v, window, sinks, key_pad, kv_len):
-    _same(what, q, k, v)
-    code = dtype_code(q)
+    dev, dt = q.device, q.dtype
+    if not (dev == k.device == v.device and dt == k.dtype == v.dtype and dev.type == "cuda"):
+        _same(what, q, k, v)
     views = _view4(what, q) + _view4(what, k) + _view4(what, v)
     B, Nq, H, hd = q.shape
-    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != hd:
+    kB, Nk, Hk, khd = k.shape
+    if kB != B or khd != hd or v.shape != k.shape:
         raise ValueError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
-    Nk, Hk = k.shape[1], k.shape[2]
-    key_pad = _index(f"{what}: key_pad", key_pad, (B, Nk), torch.uint8, q.device)
-    kv_len = _index(f"{what}: kv_len", kv_len, (B,), torch.int32, q.device)
-    return code, (B, H, Hk, Nq, Nk, hd), (int(window), int(sinks)), views, key_pad, kv_len
+    if key_pad is not None:
+        key_pad = _index(f"{what}: key_pad", key_pad, (B, Nk), torch.uint8, dev)
+    if kv_len is not None:
+        kv_len = _index(f"{what}: kv_len", kv_len, (B,), torch.int32, dev)
+    return dtype_code(q), (B, H, Hk, Nq, Nk, hd), (int(window), int(sinks)), views, key_pad, kv_len
 
 
 def sliding_attention_fwd(q, k, v, window, sinks, scale, key_pad=None, kv_len=None, *, out=None, want_lse=True):
@@ -1361,7 +1376,7 @@ def sliding_attention_fwd(q, k, v, window, sinks, scale, key_pad=None, kv_len=No
         if out.shape != q.shape:
             raise ValueError(f"{what}: out {tuple(out.shape)} for q {tuple(q.shape)}")
     lse = torch.empty(q.shape[0], q.shape[2], q.shape[1], dtype=torch.float32, device=q.device) if want_lse else None
-    wsb = lib().capk_sliding_attention_fwd_workspace(code, *dims, *ws_args)
+    wsb = _ws_bytes("capk_sliding_attention_fwd_workspace", code, *dims, *ws_args)
     ws = _ws(wsb, q.device)
     _launch(q.device, "capk_sliding_attention_fwd", code, *dims, float(scale), *ws_args, *views, _p(key_pad), _p(kv_len),
             *_view4(what, out), _p(lse), _p(ws), wsb)
@@ -1378,7 +1393,7 @@ def sliding_attention_bwd(q, k, v, o, do, lse, window, sinks, scale, key_pad=Non
             tuple(lse.shape) != (q.shape[0], q.shape[2], q.shape[1]):
         raise ValueError(f"{what}: o, do like q and a contiguous fp32 lse [B, H, Nq]")
     dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
-    wsb = lib().capk_sliding_attention_bwd_workspace(*dims, *ws_args)
+    wsb = _ws_bytes("capk_sliding_attention_bwd_workspace", *dims, *ws_args)
     ws = _ws(wsb, q.device)
     _launch(q.device, "capk_sliding_attention_bwd", code, *dims, float(scale), *ws_args, *views, _p(key_pad), _p(kv_len),
             *_view4(what, o), *_view4(what, do), _p(lse), *_view4(what, dq), *_view4(what, dk), *_view4(what, dv),
@@ -1450,7 +1465,7 @@ def kv4_attention(q, codes, scales, table, kv_len, window, sinks, scale, *, lse=
     if kv_len is None:
         raise ValueError(f"{what}: kv_len is needed")
     o = q.new_empty(q.shape)
-    wsb = lib().capk_kv4_attention_workspace(code, B, H, Hk, Nq, hd, int(window), int(sinks), page, table.shape[1])
+    wsb = _ws_bytes("capk_kv4_attention_workspace", code, B, H, Hk, Nq, hd, int(window), int(sinks), page, table.shape[1])
     ws = _ws(wsb, q.device)
     _launch(q.device, "capk_kv4_attention", code, B, H, Hk, Nq, hd, float(scale), int(window), int(sinks), *qv,
             codes.data_ptr(), scales.data_ptr(), pages, page, *targs, _p(kv_len), *_view4(what, o), _p(lse), _p(ws), wsb)
@@ -1477,7 +1492,7 @@ def verify_drafts(target, ids, u, draft=None, *, draft_len=None, temperature=1.0
     u = u.contiguous()
     accepted = torch.empty(B, dtype=torch.int32, device=dev)
     tokens = torch.empty(B, K + 1, dtype=torch.int64, device=dev)
-    wsb = lib().capk_verify_drafts_workspace(B, K, V)
+    wsb = _ws_bytes("capk_verify_drafts_workspace", B, K, V)
     ws = _ws(wsb, dev)
     dargs = (None, 0, 0) if draft is None or not K else (draft.data_ptr(), draft.stride(0), draft.stride(1))
     _launch(dev, "capk_verify_drafts", code, B, K, V, target.data_ptr(), target.stride(0), target.stride(1), *dargs,

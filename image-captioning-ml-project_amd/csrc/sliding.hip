@@ -74,39 +74,81 @@ __device__ __forceinline__ void slide_store(T* dst, const f32x16 (&acc)[HDP / 32
     }
 }
 
-// A tile of 64 keys of a workgroup's queries, in the double-buffered images (K, V): the next tile is on its
-// way from memory while this one is computed.
-template <typename T, int HDP> struct SlideKV {
-  using Img = TileImg<T, HDP>;
-  static constexpr int KT = 64, BUF = 2 * Img::bytes(KT);
-  const SlideArgs& a;
-  const T *k, *v;
-  int b, len, p_lo, p_hi, last, w, lane;
+// Tiles of 64 rows of two matrices (K and V, or Q and dO) on their way into LDS images, by 4 waves.
+// bf16: copied straight to LDS, into the one pair of images while the other is read.
+template <typename T, int HDP> struct SlidePair {
+  using Img = TileImg<bf16, HDP>;
+  static constexpr int IMG = Img::bytes(64), LDS = 4 * IMG;
+  const T *x, *y;
+  int64_t xrs, yrs;
+  int hd, w, lane;
   char* smem;
-  uint64_t hid;  // keys past the length or padded
-  __device__ __forceinline__ void fetch(int j0, int buf) const {
-    char* img = smem + buf * BUF;
-    Img::template dma<KT, 4>(img, k, a.k.rs, j0, last, a.hd, w, lane);
-    Img::template dma<KT, 4>(img + Img::bytes(KT), v, a.v.rs, j0, last, a.hd, w, lane);
+  __device__ __forceinline__ void fetch(int r0, int last, int buf) {  // rows past `last` repeat it
+    Img::template dma<64, 4>(smem + buf * 2 * IMG, x, xrs, r0, last, hd, w, lane);
+    Img::template dma<64, 4>(smem + buf * 2 * IMG + IMG, y, yrs, r0, last, hd, w, lane);
   }
-  // waits for the tile; keys that no query of the workgroup sees become zeros (they may hold anything)
-  // GROUPS = 2: workgroup barriers meet both groups, so both always take two, also without a tile (any = false)
-  template <int GROUPS = 1>
-  __device__ __forceinline__ const char* arrive(int j0, int buf, bool any = true) {
-    char* img = smem + buf * BUF;
-    const int j = any ? j0 + lane : p_hi;
-    hid = __builtin_amdgcn_ballot_w64(j >= len || (a.pad && a.pad[(int64_t)b * a.Nk + j]));
-    const uint64_t out = hid | __builtin_amdgcn_ballot_w64(j > p_hi || (j >= a.sinks && p_lo - j >= a.window));
+  // Waits for the tile, and for the readers of the one before; rows with a bit in `out` become zeros (they
+  // may hold anything).  GROUPS = 2: the barriers meet two groups of waves with tiles of their own, so the
+  // second is taken in any case.
+  template <int GROUPS = 1> __device__ __forceinline__ void land(int buf, uint64_t out) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (out) {
-      Img::clear(img, out);
-      Img::clear(img + Img::bytes(KT), out);
+      Img::clear(smem + buf * 2 * IMG, out);
+      Img::clear(smem + buf * 2 * IMG + IMG, out);
     }
     if (GROUPS == 2 || out) __syncthreads();
-    return img;
   }
+  __device__ __forceinline__ const char* first(int buf) const { return smem + buf * 2 * IMG; }
+  __device__ __forceinline__ const char* second(int buf) const { return smem + buf * 2 * IMG + IMG; }
 };
+// fp32: through registers, split into the parts of the one pair of images when its readers are done.
+template <int HDP> struct SlidePair<float, HDP> {
+  using Img = TileImg<float, HDP>;
+  static constexpr int IMG = Img::bytes(64), LDS = 2 * IMG, C = HDP / 8, N = C / 4;  // chunks of 8: per row, per thread
+  const float *x, *y;
+  int64_t xrs, yrs;
+  int hd, w, lane;
+  char* smem;
+  f32x8 rx[N], ry[N];
+  __device__ __forceinline__ void fetch(int r0, int last, int) {
+    const int t = threadIdx.x & 255;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int o = i * 256 + t, c = o % C * 8, col = c < hd ? c : 0;
+      const int64_t r = min(r0 + o / C, last);
+      rx[i] = Tile<float>::load(x + r * xrs + col);
+      ry[i] = Tile<float>::load(y + r * yrs + col);
+    }
+  }
+  template <int GROUPS = 1> __device__ __forceinline__ void land(int, uint64_t out) {
+    __syncthreads();
+    const int t = threadIdx.x & 255;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int o = i * 256 + t, r = o / C, at = r * TileImg<bf16, HDP>::RB + ((o % C ^ TileImg<bf16, HDP>::swz(r)) << 4);
+      if (out >> r & 1) rx[i] = ry[i] = tile_zero8<float>();
+      const Split8 a = Mat<float>::from(rx[i]), b = Mat<float>::from(ry[i]);
+      *(bf16x8*)(smem + at) = a.h;
+      *(bf16x8*)(smem + at + Img::PART) = a.m;
+      *(bf16x8*)(smem + at + 2 * Img::PART) = a.l;
+      *(bf16x8*)(smem + at + IMG) = b.h;
+      *(bf16x8*)(smem + at + IMG + Img::PART) = b.m;
+      *(bf16x8*)(smem + at + IMG + 2 * Img::PART) = b.l;
+    }
+    __syncthreads();
+  }
+  __device__ __forceinline__ const char* first(int) const { return smem; }
+  __device__ __forceinline__ const char* second(int) const { return smem + IMG; }
+};
+
+// One bit per key of the tile at j0: past the length or padded; seen by no query at p_lo..p_hi.
+__device__ __forceinline__ uint64_t slide_hidden(const SlideArgs& a, int b, int j, int len) {
+  return __builtin_amdgcn_ballot_w64(j >= len || (a.pad && a.pad[(int64_t)b * a.Nk + j]));
+}
+__device__ __forceinline__ uint64_t slide_unseen(const SlideArgs& a, int j, int p_lo, int p_hi) {
+  return __builtin_amdgcn_ballot_w64((j > p_hi) | ((j >= a.sinks) & (p_lo - j >= a.window)));
+}
 
 // n products whose LDS operands are requested D ahead: the order is written down, as the compiler would
 // request each operand right before its use and wait for it
@@ -134,7 +176,7 @@ __device__ __forceinline__ bool slide_full(const SlideArgs& a, int j0, int n, in
 // GROUPS = 2: a second group of 4 waves, with images of its own, takes every other tile of the same queries.
 template <typename T, int HDP, int GROUPS>
 __global__ __launch_bounds__(256 * GROUPS, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) : GROUPS == 2 || HDP > 96 ? 2 : 3) void slide_fwd(SlideArgs a) {
-  using KV = SlideKV<T, HDP>;
+  using KV = SlidePair<T, HDP>;
   using Img = typename KV::Img;
   constexpr int NS = HDP / 16, ND = HDP / 32;
   extern __shared__ __align__(16) char smem[];
@@ -148,8 +190,9 @@ __global__ __launch_bounds__(256 * GROUPS, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) 
   const float c = a.scale * kTileLog2e;
   typename Img::Lane ln(lane);
   const SlideTiles<64> tiles(a.window, a.sinks, p_lo, p_hi, len);
-  KV kv{a, row<T>(a.k, b, 0, kvh), row<T>(a.v, b, 0, kvh), b, len, p_lo, p_hi, min(len, p_hi + 1) - 1, w, lane, smem + grp * 2 * KV::BUF, 0};
-  if (grp < tiles.n) kv.fetch(tiles.key0(grp), 0);
+  const int last = min(len, p_hi + 1) - 1;
+  KV kv{row<T>(a.k, b, 0, kvh), row<T>(a.v, b, 0, kvh), a.k.rs, a.v.rs, a.hd, w, lane, smem + grp * KV::LDS};
+  if (grp < tiles.n) kv.fetch(tiles.key0(grp), last, 0);
 
   typename Mat<T>::V8 qf[NS];
   slide_frags<T, HDP>(qf, row<T>(a.q, b, qi, h), qi < a.Nq, a.hd, hh);
@@ -162,9 +205,12 @@ __global__ __launch_bounds__(256 * GROUPS, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) 
   slide_settle(qf);
   for (int u = 0; u * GROUPS < tiles.n; ++u) {  // (as many turns, and barriers, in both groups)
     const int t = u * GROUPS + grp, j0 = tiles.key0(t);
-    const char *ki = kv.template arrive<GROUPS>(j0, u & 1, t < tiles.n), *vi = ki + Img::bytes(64);
+    const int j = t < tiles.n ? j0 + lane : p_hi;
+    const uint64_t hid = slide_hidden(a, b, j, len);
+    kv.template land<GROUPS>(u & 1, hid | slide_unseen(a, j, p_lo, p_hi));
     if (t >= tiles.n) continue;
-    if (t + GROUPS < tiles.n) kv.fetch(tiles.key0(t + GROUPS), (u + 1) & 1);
+    const char *ki = kv.first(u & 1), *vi = kv.second(u & 1);
+    if (t + GROUPS < tiles.n) kv.fetch(tiles.key0(t + GROUPS), last, (u + 1) & 1);
     if (slide_none(a, j0, 64, pw_lo, pw_hi)) continue;
     f32x16 s[2] = {tile_zero<f32x16>(), tile_zero<f32x16>()};
     slide_pipe<4, 2 * NS>([&](int i) { return Img::frag(ki, (i & 1) * 32, i >> 1, ln); },
@@ -172,14 +218,14 @@ __global__ __launch_bounds__(256 * GROUPS, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) 
     typename Mat<T>::V8 vf[2][ND];  // V^T fragments of a 16-key step, requested a step ahead
 #pragma unroll
     for (int d = 0; d < ND; ++d) vf[0][d] = Img::trans(vi, 0, d * 32, ln);
-    if (kv.hid || !slide_full(a, j0, 64, pw_lo, pw_hi)) {
-      const uint32_t hid[2] = {(uint32_t)kv.hid >> (4 * hh), (uint32_t)(kv.hid >> 32) >> (4 * hh)};
+    if (hid || !slide_full(a, j0, 64, pw_lo, pw_hi)) {
+      const uint32_t hl[2] = {(uint32_t)hid >> (4 * hh), (uint32_t)(hid >> 32) >> (4 * hh)};
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int r = 8 * (i >> 2) + (i & 3);
-          const bool sees = slide_sees(a, p, j0 + kb * 32 + 4 * hh + r) & !(hid[kb] >> r & 1);
+          const bool sees = slide_sees(a, p, j0 + kb * 32 + 4 * hh + r) & !(hl[kb] >> r & 1);
           s[kb][i] = sees ? s[kb][i] : -INFINITY;
         }
     }
@@ -245,7 +291,7 @@ __global__ __launch_bounds__(256 * GROUPS, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) 
 
 template <typename T, int HDP>
 __global__ __launch_bounds__(256, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) : HDP <= 64 ? 3 : 2) void slide_dq(SlideArgs a) {
-  using KV = SlideKV<T, HDP>;
+  using KV = SlidePair<T, HDP>;
   using Img = typename KV::Img;
   constexpr int NS = HDP / 16, ND = HDP / 32;
   extern __shared__ __align__(16) char smem[];
@@ -258,8 +304,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) : HDP <= 
   const float c = a.scale * kTileLog2e;
   typename Img::Lane ln(lane);
   const SlideTiles<64> tiles(a.window, a.sinks, p_lo, p_hi, len);
-  KV kv{a, row<T>(a.k, b, 0, kvh), row<T>(a.v, b, 0, kvh), b, len, p_lo, p_hi, min(len, p_hi + 1) - 1, w, lane, smem, 0};
-  if (tiles.n) kv.fetch(tiles.key0(0), 0);
+  const int last = min(len, p_hi + 1) - 1;
+  KV kv{row<T>(a.k, b, 0, kvh), row<T>(a.v, b, 0, kvh), a.k.rs, a.v.rs, a.hd, w, lane, smem};
+  if (tiles.n) kv.fetch(tiles.key0(0), last, 0);
 
   typename Mat<T>::V8 qf[NS], dof[NS];
   slide_frags<T, HDP>(qf, row<T>(a.q, b, qi, h), qi < a.Nq, a.hd, hh);
@@ -288,8 +335,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) : HDP <= 
   slide_settle(qf);
   slide_settle(dof);
   // P and do v^T of 32 keys of a tile, zeros where the query does not see the key
-  auto scores = [&](const char* ki, const char* vi, int j0, int kb, f32x16& s, f32x16& dp) {
-    const uint32_t hidden = (uint32_t)(kv.hid >> (32 * kb));
+  auto scores = [&](const char* ki, const char* vi, int j0, int kb, uint64_t hid, f32x16& s, f32x16& dp) {
+    const uint32_t hidden = (uint32_t)(hid >> (32 * kb));
     s = dp = tile_zero<f32x16>();
 #pragma unroll
     for (int st = 0; st < NS; ++st) {
@@ -312,13 +359,15 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) : HDP <= 
   if (walk) {
     for (int t = 0; t < tiles.n; ++t, buf ^= 1) {
       const int j0 = tiles.key0(t);
-      const char *ki = kv.arrive(j0, buf), *vi = ki + Img::bytes(64);
-      kv.fetch(tiles.key0(t + 1 < tiles.n ? t + 1 : 0), buf ^ 1);
+      const uint64_t hid = slide_hidden(a, b, j0 + lane, len);
+      kv.land(buf, hid | slide_unseen(a, j0 + lane, p_lo, p_hi));
+      const char *ki = kv.first(buf), *vi = kv.second(buf);
+      kv.fetch(tiles.key0(t + 1 < tiles.n ? t + 1 : 0), last, buf ^ 1);
 #pragma unroll 1
       for (int kb = 0; kb < 2; ++kb) {
         if (slide_none(a, j0 + kb * 32, 32, pw_lo, pw_hi)) continue;
         f32x16 s, dp;
-        scores(ki, vi, j0, kb, s, dp);
+        scores(ki, vi, j0, kb, hid, s, dp);
 #pragma unroll
         for (int i = 0; i < 16; ++i) delta = fmaf(s[i], dp[i], delta);
       }
@@ -327,13 +376,15 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) : HDP <= 
   }
   for (int t = 0; t < tiles.n; ++t, buf ^= 1) {
     const int j0 = tiles.key0(t);
-    const char *ki = kv.arrive(j0, buf), *vi = ki + Img::bytes(64);
-    if (t + 1 < tiles.n) kv.fetch(tiles.key0(t + 1), buf ^ 1);
+    const uint64_t hid = slide_hidden(a, b, j0 + lane, len);
+    kv.land(buf, hid | slide_unseen(a, j0 + lane, p_lo, p_hi));
+    const char *ki = kv.first(buf), *vi = kv.second(buf);
+    if (t + 1 < tiles.n) kv.fetch(tiles.key0(t + 1), last, buf ^ 1);
 #pragma unroll 1
     for (int kb = 0; kb < 2; ++kb) {
       if (slide_none(a, j0 + kb * 32, 32, pw_lo, pw_hi)) continue;
       f32x16 s, dp;
-      scores(ki, vi, j0, kb, s, dp);
+      scores(ki, vi, j0, kb, hid, s, dp);
 #pragma unroll
       for (int st = 0; st < 2; ++st) {
         float x[8];
@@ -355,10 +406,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) : HDP <= 
 constexpr int kSlideKeys = 128;
 template <typename T, int HDP>
 __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void slide_dkv(SlideArgs a) {
-  using Img = TileImg<T, HDP>;
-  constexpr int QT = 64, NS = HDP / 16, ND = HDP / 32, BUF = 2 * Img::bytes(QT);
+  using Pair = SlidePair<T, HDP>;
+  using Img = typename Pair::Img;
+  constexpr int QT = 64, NS = HDP / 16, ND = HDP / 32;
   extern __shared__ __align__(16) char smem[];
-  float* Ls = (float*)(smem + 2 * BUF);  // per buffer: lse (base 2) and D of 64 queries
+  float* Ls = (float*)(smem + Pair::LDS);  // per buffer: lse (base 2) and D of 64 queries
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hh = lane >> 5;
   const SlideBlock at(a);
   const int b = at.b, kvh = at.kvh, G = a.H / a.Hk, len = slide_len(a, b), off = len - a.Nq;
@@ -381,12 +433,13 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void s
   // the tile of 64 queries t: head kvh G + t / nq, queries qa + 64 (t % nq)
   const float* stat = (threadIdx.x & 64 ? a.delta : a.lse) + (int64_t)b * a.H * a.Nq;
   float ld = 0.f;  // threads 0..63 carry lse, 64..127 D (unconditional loads: nothing waits for them here)
+  Pair qd{nullptr, nullptr, a.q.rs, a.dout.rs, a.hd, w, lane, smem};
   auto fetch = [&](int t, int buf) {
     const int h = kvh * G + t / nq, q0 = qa + t % nq * QT;
-    char* img = smem + buf * BUF;
     ld = stat[(int64_t)h * a.Nq + min(q0 + lane, qb - 1)];
-    Img::template dma<QT, 4>(img, row<T>(a.q, b, 0, h), a.q.rs, q0, qb - 1, a.hd, w, lane);
-    Img::template dma<QT, 4>(img + Img::bytes(QT), row<T>(a.dout, b, 0, h), a.dout.rs, q0, qb - 1, a.hd, w, lane);
+    qd.x = row<T>(a.q, b, 0, h);
+    qd.y = row<T>(a.dout, b, 0, h);
+    qd.fetch(q0, qb - 1, buf);
   };
   if (all) fetch(0, 0);
   typename Mat<T>::V8 kf[NS], vf[NS];
@@ -399,19 +452,18 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void s
   slide_settle(kf);
   slide_settle(vf);
   for (int t = 0; t < all; ++t) {
-    const char *qi = smem + (t & 1) * BUF, *di = qi + Img::bytes(QT);
     const float* ls = Ls + (t & 1) * 128;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     const int q0 = qa + t % nq * QT, p0 = off + q0;
     if (w < 2) Ls[(t & 1) * 128 + threadIdx.x] = q0 + lane >= qb ? (w ? 0.f : INFINITY) : (w ? ld : ld * kTileLog2e);
-    __syncthreads();
+    qd.land(t & 1, 0);
+    const char *qi = qd.first(t & 1), *di = qd.second(t & 1);
     if (t + 1 < all) fetch(t + 1, (t + 1) & 1);
 #pragma unroll 1
     for (int qt = 0; qt < 2; ++qt) {
       const int pq = p0 + qt * 32;
       if (slide_none(a, jw, 32, pq, pq + 31)) continue;
       const bool full = !hidden && q0 + qt * 32 + 32 <= qb && slide_full(a, jw, 32, pq, pq + 31);
-      if constexpr (sizeof(T) == 2) ln.forget();
+      if constexpr (sizeof(T) == 2 || HDP > 96) ln.forget();
       f32x16 s = tile_zero<f32x16>(), dp = tile_zero<f32x16>();
 #pragma unroll
       for (int st = 0; st < NS; ++st) {
@@ -476,6 +528,7 @@ __global__ __launch_bounds__(256) void slide_dkv_sum(SlideArgs a) {
   const float* src = a.part + (((int64_t)blockIdx.z * a.Hk + blockIdx.y) * a.sink_tiles + tile) * (a.far_chunks + 1) * 2 *
                                   kSlideKeys * a.hd + (int64_t)which * kSlideKeys * a.hd + e;
   f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
   for (int c = j < a.sinks ? 0 : a.far_chunks; c <= a.far_chunks; ++c) s += *(const f32x4*)(src + (int64_t)c * 2 * kSlideKeys * a.hd);
   Tile<T>::store4(row<T>(which ? a.dv : a.dk, blockIdx.z, j, blockIdx.y) + e % a.hd, s);
 }
@@ -585,12 +638,12 @@ extern "C" int capk_sliding_attention_fwd(int dtype, int B, int H, int Hk, int N
   // 66 tiles, heads of 128); fp32 images of wider heads leave no room for it
   const bool two = grid.x <= 256;
   SLIDE_HD(hdp, {
-    constexpr int B16 = SlideKV<bf16, HDP>::BUF, B32 = SlideKV<float, HDP>::BUF, G32 = HDP <= 64 ? 2 : 1;
+    constexpr int L16 = SlidePair<bf16, HDP>::LDS, L32 = SlidePair<float, HDP>::LDS, G32 = HDP <= 64 ? 2 : 1;
     if (dtype == CAPK_BF16)
-      return two ? slide_launch(slide_fwd<bf16, HDP, 2>, grid, 4 * B16, S(stream), a, "slide_fwd", 512)
-                 : slide_launch(slide_fwd<bf16, HDP, 1>, grid, 2 * B16, S(stream), a, "slide_fwd");
-    return two && G32 == 2 ? slide_launch(slide_fwd<float, HDP, G32>, grid, 2 * G32 * B32, S(stream), a, "slide_fwd", 256 * G32)
-                           : slide_launch(slide_fwd<float, HDP, 1>, grid, 2 * B32, S(stream), a, "slide_fwd");
+      return two ? slide_launch(slide_fwd<bf16, HDP, 2>, grid, 2 * L16, S(stream), a, "slide_fwd", 512)
+                 : slide_launch(slide_fwd<bf16, HDP, 1>, grid, L16, S(stream), a, "slide_fwd");
+    return two && G32 == 2 ? slide_launch(slide_fwd<float, HDP, G32>, grid, G32 * L32, S(stream), a, "slide_fwd", 256 * G32)
+                           : slide_launch(slide_fwd<float, HDP, 1>, grid, L32, S(stream), a, "slide_fwd");
   });
 }
 
@@ -632,11 +685,11 @@ extern "C" int capk_sliding_attention_bwd(int dtype, int B, int H, int Hk, int N
   hipStream_t st = S(stream);
   SLIDE_HD(hdp, {
     if (dtype == CAPK_BF16) {
-      const size_t shm = 2 * SlideKV<bf16, HDP>::BUF;
+      const size_t shm = SlidePair<bf16, HDP>::LDS;
       if ((rc = slide_launch(slide_dq<bf16, HDP>, gq, shm, st, a, "slide_dq"))) return rc;
       if ((rc = slide_launch(slide_dkv<bf16, HDP>, gk, shm + 1024, st, a, "slide_dkv"))) return rc;
     } else {
-      const size_t shm = 2 * SlideKV<float, HDP>::BUF;
+      const size_t shm = SlidePair<float, HDP>::LDS;
       if ((rc = slide_launch(slide_dq<float, HDP>, gq, shm, st, a, "slide_dq"))) return rc;
       if ((rc = slide_launch(slide_dkv<float, HDP>, gk, shm + 1024, st, a, "slide_dkv"))) return rc;
     }

@@ -113,17 +113,14 @@ template <typename V> __device__ __forceinline__ V tile_zero() {
 // c ^ swz(r).  The masks put the 16 lanes that a b128 read serves together ({0-3, 12-15, 20-27} and so on:
 // one chunk of 16 rows) and the 32 lanes of a transposed b64 read (four chunks of 4 rows) on distinct
 // banks, and leave whole 1-KiB pieces contiguous, as the copy straight from memory needs them.
-template <typename T, int HDP> struct TileImg {
-  static constexpr int RB = HDP * (int)sizeof(T), PER = 16 / (int)sizeof(T);  // bytes of a row, elements of a chunk
+template <typename T, int HDP> struct TileImg;
+template <int HDP> struct TileImg<bf16, HDP> {
+  using T = bf16;
+  static constexpr int RB = HDP * 2, PER = 8;  // bytes of a row, elements of a chunk
   __device__ __forceinline__ static int swz(int r) {
-    if constexpr (sizeof(T) == 2) {
-      if constexpr (HDP == 128) return (r & 3) << 2 | ((r >> 2) & 3);
-      else if constexpr (HDP == 64) return ((r >> 1) & 1) << 2 | ((r >> 2) & 3);
-      else return (r >> 2) & 3;
-    } else {
-      if constexpr (RB % 256 == 0) return r & 15;
-      else return (r >> 1) & 7;
-    }
+    if constexpr (HDP == 128) return (r & 3) << 2 | ((r >> 2) & 3);
+    else if constexpr (HDP == 64) return ((r >> 1) & 1) << 2 | ((r >> 2) & 3);
+    else return (r >> 2) & 3;
   }
   static constexpr int bytes(int rows) { return rows * RB; }
 
@@ -164,58 +161,47 @@ template <typename T, int HDP> struct TileImg {
     for (int o = (threadIdx.x & 255) * 16; o < 64 * RB; o += 256 * 16)
       if (rows >> (o / RB) & 1) *(f32x4*)(img + o) = (f32x4){0.f, 0.f, 0.f, 0.f};
   }
-  // Byte offsets of a lane's reads: of a row fragment, and (bf16) of the two halves of a transposed one.
+  // Byte offsets of a lane's reads: of a row fragment, and of the two halves of a transposed one.
   struct Lane {
     int f, ta, tb;
     __device__ __forceinline__ explicit Lane(int lane) {
       const int r = lane & 31, h = lane >> 5, i16 = lane & 15;
-      f = r * RB + ((h * 8 / PER ^ swz(r)) << 4);
-      if constexpr (sizeof(T) == 2) {
-        const int q = 4 * h + (i16 >> 2), c = 2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1);
-        ta = q * RB + ((c ^ swz(q)) << 4) + (i16 & 1) * 8;
-        tb = (q + 8) * RB + ((c ^ swz(q + 8)) << 4) + (i16 & 1) * 8;
-      } else {
-        ta = h;
-        tb = r;
-      }
+      f = r * RB + ((h ^ swz(r)) << 4);
+      const int q = 4 * h + (i16 >> 2), c = 2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1);
+      ta = q * RB + ((c ^ swz(q)) << 4) + (i16 & 1) * 8;
+      tb = (q + 8) * RB + ((c ^ swz(q + 8)) << 4) + (i16 & 1) * 8;
     }
     // Makes the offsets opaque: what derives from them is computed again (an instruction each) where the
     // loop would otherwise hold it in registers that it does not have.
     __device__ __forceinline__ void forget() { asm volatile("" : "+v"(f), "+v"(ta), "+v"(tb)); }
   };
   static constexpr bool POW2 = (RB & (RB - 1)) == 0;
-  // A / B fragment of a 32x32 product: row r0 + (l & 31), columns 16 s + 8 h (r0 a multiple of 32).  Chunks
-  // 2 s (fp32: 4 s) beside the mask: an exclusive or, where rows are not a power of two of its masked bits.
-  __device__ __forceinline__ static typename Mat<T>::V8 frag(const char* img, int r0, int s, const Lane& l) {
-    if constexpr (sizeof(T) == 2) {
-      const int o = POW2 ? l.f ^ (s * 32) : (l.f ^ ((s & 1) * 32)) + (s >> 1) * 64;
-      return *(const bf16x8*)(img + r0 * RB + o);
-    } else {
-      const int o = POW2 ? l.f ^ (s * 64) : (l.f ^ ((s & 1) * 64)) + (s >> 1) * 128;
-      const f32x4 x = *(const f32x4*)(img + r0 * RB + o), y = *(const f32x4*)(img + r0 * RB + (o ^ 16));
-      const float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-      return Mat<float>::pack(v);
-    }
+  // A / B fragment of a 32x32 product: row r0 + (l & 31), columns 16 s + 8 h (r0 a multiple of 32).  Chunk
+  // 2 s beside the mask: an exclusive or, where rows are not a power of two of its masked bits.
+  __device__ __forceinline__ static bf16x8 frag(const char* img, int r0, int s, const Lane& l) {
+    return *(const bf16x8*)(img + r0 * RB + (POW2 ? l.f ^ (s * 32) : (l.f ^ ((s & 1) * 32)) + (s >> 1) * 64));
   }
   // A fragment of the transpose for a 32x32 product: lane column c0 + (l & 31), slot (h, e) = row
   // r0 + 8 (e >> 2) + 4 h + (e & 3) -- the order in which eight accumulator registers of a 32x32
   // product hold their rows (r0 a multiple of 16, c0 of 32).
-  __device__ __forceinline__ static typename Mat<T>::V8 trans(const char* img, int r0, int c0, const Lane& l) {
-    if constexpr (sizeof(T) == 2) {
-      const char *a = img + r0 * RB + (POW2 ? l.ta ^ (c0 * 2) : l.ta + c0 * 2), *b = img + r0 * RB + (POW2 ? l.tb ^ (c0 * 2) : l.tb + c0 * 2);
-      const bf16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, a));
-      const bf16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, b));
-      return (bf16x8){x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-    } else {
-      const int d = c0 + l.tb;
-      float v[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int r = 8 * (e >> 2) + 4 * l.ta + (e & 3);
-        v[e] = *(const float*)(img + (r0 + r) * RB + (((d / 4) ^ swz(r)) << 4) + (d & 3) * 4);
-      }
-      return Mat<float>::pack(v);
-    }
+  __device__ __forceinline__ static bf16x8 trans(const char* img, int r0, int c0, const Lane& l) {
+    const char *a = img + r0 * RB + (POW2 ? l.ta ^ (c0 * 2) : l.ta + c0 * 2), *b = img + r0 * RB + (POW2 ? l.tb ^ (c0 * 2) : l.tb + c0 * 2);
+    const bf16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, a));
+    const bf16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, b));
+    return (bf16x8){x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+  }
+};
+// The image of 64 rows of an fp32 matrix: its three bf16 parts one after the other, split once for all waves.
+template <int HDP> struct TileImg<float, HDP> {
+  using I = TileImg<bf16, HDP>;
+  using Lane = typename I::Lane;
+  static constexpr int PART = I::bytes(64);
+  static constexpr int bytes(int rows) { return 3 * I::bytes(rows); }
+  __device__ __forceinline__ static Split8 frag(const char* img, int r0, int s, const Lane& l) {
+    return {I::frag(img, r0, s, l), I::frag(img + PART, r0, s, l), I::frag(img + 2 * PART, r0, s, l)};
+  }
+  __device__ __forceinline__ static Split8 trans(const char* img, int r0, int c0, const Lane& l) {
+    return {I::trans(img, r0, c0, l), I::trans(img + PART, r0, c0, l), I::trans(img + 2 * PART, r0, c0, l)};
   }
 };
 // A fragment of the transpose of a row-major LDS image (row stride st) for a 16x16 product over 32 rows:

@@ -338,11 +338,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) : HDP <= 
   auto scores = [&](const char* ki, const char* vi, int j0, int kb, uint64_t hid, f32x16& s, f32x16& dp) {
     const uint32_t hidden = (uint32_t)(hid >> (32 * kb));
     s = dp = tile_zero<f32x16>();
-#pragma unroll
-    for (int st = 0; st < NS; ++st) {
-      s = Mat<T>::mma32(Img::frag(ki, kb * 32, st, ln), qf[st], s);
-      dp = Mat<T>::mma32(Img::frag(vi, kb * 32, st, ln), dof[st], dp);
-    }
+    slide_pipe<(sizeof(T) == 2 ? 4 : 2), 2 * NS>([&](int i) { return Img::frag(i & 1 ? vi : ki, kb * 32, i >> 1, ln); },
+                          [&](int i, const auto& f) {
+                            if (i & 1) dp = Mat<T>::mma32(f, dof[i >> 1], dp);
+                            else s = Mat<T>::mma32(f, qf[i >> 1], s);
+                          });
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = tile_exp2(fmaf(s[i], c, -lse2));
     if (hidden || !slide_full(a, j0 + kb * 32, 32, pw_lo, pw_hi)) {
@@ -385,15 +385,16 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) : HDP <= 
       if (slide_none(a, j0 + kb * 32, 32, pw_lo, pw_hi)) continue;
       f32x16 s, dp;
       scores(ki, vi, j0, kb, hid, s, dp);
+      typename Mat<T>::V8 df[2];
 #pragma unroll
       for (int st = 0; st < 2; ++st) {
         float x[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = s[st * 8 + e] * (dp[st * 8 + e] - delta);
-        const typename Mat<T>::V8 df = Mat<T>::pack(x);
-#pragma unroll
-        for (int d = 0; d < ND; ++d) dq[d] = Mat<T>::mma32(Img::trans(ki, kb * 32 + st * 16, d * 32, ln), df, dq[d]);
+        df[st] = Mat<T>::pack(x);
       }
+      slide_pipe<(sizeof(T) == 2 ? 4 : 2), 2 * ND>([&](int i) { return Img::trans(ki, kb * 32 + i / ND * 16, i % ND * 32, ln); },
+                            [&](int i, const auto& f) { dq[i % ND] = Mat<T>::mma32(f, df[i / ND], dq[i % ND]); });
     }
   }
   if (qi >= a.Nq) return;
@@ -465,11 +466,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void s
       const bool full = !hidden && q0 + qt * 32 + 32 <= qb && slide_full(a, jw, 32, pq, pq + 31);
       if constexpr (sizeof(T) == 2 || HDP > 96) ln.forget();
       f32x16 s = tile_zero<f32x16>(), dp = tile_zero<f32x16>();
-#pragma unroll
-      for (int st = 0; st < NS; ++st) {
-        s = Mat<T>::mma32(Img::frag(qi, qt * 32, st, ln), kf[st], s);
-        dp = Mat<T>::mma32(Img::frag(di, qt * 32, st, ln), vf[st], dp);
-      }
+      slide_pipe<2, 2 * NS>([&](int i) { return Img::frag(i & 1 ? di : qi, qt * 32, i >> 1, ln); },
+                            [&](int i, const auto& f) {
+                              if (i & 1) dp = Mat<T>::mma32(f, vf[i >> 1], dp);
+                              else s = Mat<T>::mma32(f, kf[i >> 1], s);
+                            });
 #pragma unroll
       for (int i4 = 0; i4 < 4; ++i4) {
         const int r = qt * 32 + 8 * i4 + 4 * hh;
@@ -491,18 +492,21 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void s
           dp[i] = sees ? dp[i] : 0.f;
         }
       }
+      typename Mat<T>::V8 pf[2], df[2];
 #pragma unroll
       for (int st = 0; st < 2; ++st) {
         float x[8], y[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) { x[e] = s[st * 8 + e]; y[e] = dp[st * 8 + e]; }
-        const typename Mat<T>::V8 pf = Mat<T>::pack(x), df = Mat<T>::pack(y);
-#pragma unroll
-        for (int d = 0; d < ND; ++d) {
-          dv[d] = Mat<T>::mma32(Img::trans(di, qt * 32 + st * 16, d * 32, ln), pf, dv[d]);
-          dk[d] = Mat<T>::mma32(Img::trans(qi, qt * 32 + st * 16, d * 32, ln), df, dk[d]);
-        }
+        pf[st] = Mat<T>::pack(x);
+        df[st] = Mat<T>::pack(y);
       }
+      slide_pipe<2, 4 * ND>([&](int i) { return Img::trans(i & 1 ? qi : di, qt * 32 + i / (2 * ND) * 16, (i >> 1) % ND * 32, ln); },
+                            [&](int i, const auto& f) {
+                              const int d = (i >> 1) % ND, st = i / (2 * ND);
+                              if (i & 1) dk[d] = Mat<T>::mma32(f, df[st], dk[d]);
+                              else dv[d] = Mat<T>::mma32(f, pf[st], dv[d]);
+                            });
     }
   }
   if (far && j >= a.sinks) return;

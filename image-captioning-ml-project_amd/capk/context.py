@@ -29,12 +29,13 @@ def axis_frequencies(sections, theta=10000.0, device="cuda"):
 
 
 def _rows(t):
-    """`t` itself where its rows start 16-B aligned with unit element stride, else a contiguous copy."""
+    """`t` itself where its rows start 16-B aligned with unit element stride, and its tokens less than 2^22
+    elements apart, else a contiguous copy."""
     if t is None or t.dim() != 4:
         return t
     n, s, d = 16 // t.element_size(), t.stride(), t.shape
     if (t.data_ptr() % 16 == 0 and (s[3] == 1 or d[3] == 1) and (s[0] % n == 0 or d[0] == 1)
-            and (s[1] % n == 0 or d[1] == 1) and (s[2] % n == 0 or d[2] == 1)):
+            and ((s[1] % n == 0 and s[1] < 1 << 22) or d[1] == 1) and (s[2] % n == 0 or d[2] == 1)):
         return t
     return t.contiguous()
 
@@ -95,7 +96,7 @@ def sliding_attention(q, k, v, *, window=0, sinks=0, scale=None, key_pad=None, k
     if q.dim() == 4 and k.dim() == 4 and not (q.numel() and k.numel()):  # nothing to attend, or to
         if q.dtype != k.dtype or q.dtype != v.dtype or k.shape != v.shape or q.shape[0] != k.shape[0]:
             raise ValueError(f"sliding_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
-        return q * 0
+        return q.masked_fill(torch.ones_like(q, dtype=torch.bool), 0)  # (zeros, of q's graph)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _SlidingAttention.apply(q, k, v, window, sinks, scale, key_pad, kv_len)
     return ops.sliding_attention_fwd(_rows(q), _rows(k), _rows(v), window, sinks, scale, key_pad, kv_len,
@@ -105,7 +106,8 @@ def sliding_attention(q, k, v, *, window=0, sinks=0, scale=None, key_pad=None, k
 class KV4Cache:
     """Pages of keys and values in 4 bits: codes [pages, 2, heads, page, hd/2] and scales [pages, 2, heads, page,
     hd/32] (uint8).  The caller keeps the page tables (int [B, pages of a sequence]) and lengths, as one table
-    serves every layer's cache; a page may stand in several tables (shared prefixes, beams)."""
+    serves every layer's cache; a page may stand in several tables (shared prefixes, beams) as long as
+    no call appends to the same slot twice."""
 
     def __init__(self, codes, scales):
         self.codes, self.scales = codes, scales

@@ -1298,7 +1298,8 @@ def _same(what, first, *rest, dtype=True):
 
 
 def _index(what, t, shape, dtype, dev):
-    """`t` as a contiguous index / flag tensor of `dtype`, after checks of shape, kind and device."""
+    """`t` as a contiguous index / flag tensor of `dtype` (its values have to fit), after checks of shape, kind
+    and device."""
     if t is None:
         return None
     if t.device != dev:
@@ -1359,6 +1360,8 @@ def _sliding_args(what, q, k, v, window, sinks, key_pad, kv_len):
     if kB != B or khd != hd or v.shape != k.shape:
         raise ValueError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
     if key_pad is not None:
+        if key_pad.dtype not in (torch.bool, torch.uint8) and not key_pad.dtype.is_floating_point:
+            key_pad = key_pad != 0
         key_pad = _index(f"{what}: key_pad", key_pad, (B, Nk), torch.uint8, dev)
     if kv_len is not None:
         kv_len = _index(f"{what}: kv_len", kv_len, (B,), torch.int32, dev)
@@ -1485,6 +1488,8 @@ def verify_drafts(target, ids, u, draft=None, *, draft_len=None, temperature=1.0
         if t is not None and (t.dim() != 3 or tuple(t.shape[:2]) != (B, n) or not 1 <= V <= t.shape[2] or
                               (t.stride(2) != 1 and t.shape[2] > 1)):
             raise ValueError(f"{what}: logits [{B}, {n}, >= {V}] with unit stride in the last, got {tuple(t.shape)}")
+    if ids is None:
+        raise ValueError(f"{what}: ids are needed")
     ids = _index(f"{what}: ids", ids, (B, K), torch.int64, dev)
     draft_len = _index(f"{what}: draft_len", draft_len, (B,), torch.int32, dev)
     if u.dtype != torch.float32 or tuple(u.shape) != (B, K + 1) or u.device != dev:

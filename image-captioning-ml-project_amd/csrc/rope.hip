@@ -180,7 +180,7 @@ extern "C" int capk_axis_rope(int dtype, int B, int N, int hd, int pairs, int in
   // tokens per workgroup: enough workgroups for every CU first, then up to 8 to share the launch
   const int64_t all = (int64_t)B * N;
   a.tokens = (int)(all / 2048 < 1 ? 1 : all / 2048 > 8 ? 8 : all / 2048);
-  CAPK_CHECK_ARG(all / a.tokens < (1 << 30) && Hq + (int64_t)Hk <= 1024, "capk_axis_rope: too many tokens or heads");
+  CAPK_CHECK_ARG(all / a.tokens < (1 << 24) - 1 && Hq + (int64_t)Hk <= 1024, "capk_axis_rope: too many tokens or heads");
   const int per = pairs / V + (hd - 2 * pairs) / V, heads = Hq + Hk;
   a.per_mul = (uint32_t)(((1ull << 32) + per - 1) / per);
   a.heads_mul = (uint32_t)(((1ull << 32) + heads - 1) / heads);

@@ -328,6 +328,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) : HDP <= 
         for (int e = 0; e < 8; ++e) delta = fmaf((float)x[e], (float)y[e], delta);
       }
     delta += __shfl_xor(delta, 32, 64);
+    if (lse2 == -INFINITY) delta = 0.f;  // (it sees nothing, and its do may be anything)
   }
   f32x16 dq[ND];
 #pragma unroll
@@ -556,7 +557,7 @@ static int slide_check(const char* who, int dtype, int B, int H, int Hk, int Nq,
   CAPK_CHECK_ARG(Hk >= 1 && H >= Hk && H % Hk == 0 && H <= 65535, "%s: %d query heads over %d key heads", who, H, Hk);
   CAPK_CHECK_ARG(hd >= 8 && hd % 8 == 0 && hd <= 128, "%s: hd=%d must be a multiple of 8, <= 128", who, hd);
   CAPK_CHECK_ARG(window >= 0 && sinks >= 0, "%s: window and sinks must not be negative", who);
-  CAPK_CHECK_ARG((int64_t)B * H * (cdiv(Nq, 128) + 2 * (int64_t)cdiv(Nk, 128)) < (1 << 30), "%s: too many tiles", who);
+  CAPK_CHECK_ARG((int64_t)B * H * (cdiv(Nq, 128) + 2 * (int64_t)cdiv(Nk, 128)) < (1 << 24), "%s: too many tiles", who);
   CAPK_CHECK_ARG(scale > 0.f && scale < INFINITY, "%s: scale must be positive", who);
   const int ea = dtype == CAPK_BF16 ? 8 : 4;
   for (int i = 0; i < n; ++i)
@@ -581,8 +582,7 @@ static SlideArgs slide_args(int B, int H, int Hk, int Nq, int Nk, int hd, float 
 // The far queries of the sink tiles.  An item's length is its 64-query tiles; the launch runs about
 // `slots` workgroups at a time.  Where even the longest item (a sink tile with every query) is within
 // a slot's share of the whole, each sink tile has one owner; else its far queries go in chunks of a
-// quarter of that share (at least 256 queries, at most an ordinary tile's).  Measured at N = 16384,
-// window 1024, 4 sinks, 4 key heads: see slide_dkv.
+// quarter of that share (at least 256 queries), so the partial sums stay below 2^29 bytes.
 static void slide_far(SlideArgs& a) {
   const int64_t slots = 512, G = a.H / a.Hk;
   a.sink_tiles = cdiv(a.sinks, kSlideKeys);
@@ -594,8 +594,6 @@ static void slide_far(SlideArgs& a) {
   const int64_t share = a.B * (int64_t)a.Hk * (cdiv(a.Nk, kSlideKeys) * near + a.sink_tiles * far) / slots;
   if (near + far <= share) return;
   int64_t n = share / 4 / G * 64;
-  const int64_t top = (a.window + kSlideKeys + 63) / 64 * 64;
-  if (n > top) n = top;
   if (n < 256) n = 256;
   a.far_rows = (int)n;
   a.far_chunks = cdiv(rows, n);

@@ -117,8 +117,8 @@ template <typename T, int HDP> struct StepTile<true, T, HDP> {
   }
   __device__ __forceinline__ static float scale(const uint8_t* c, int t, int g) {
     // run t lies in the block of the first run or in that of the last
-    if constexpr (HDP == 96) return __uint_as_float((uint32_t)(elem(t, g) / 32 != elem(0, g) / 32 ? c[1] : c[0]) << 23);
-    else return __uint_as_float((uint32_t)c[0] << 23);
+    if constexpr (HDP == 96) return kv4_scale(elem(t, g) / 32 != elem(0, g) / 32 ? c[1] : c[0]);
+    else return kv4_scale(c[0]);
   }
   __device__ __forceinline__ bf16x8 kf(int s, int t, int g) const { return step_fp4(k[s][t], scale(ks[s], t, g)); }
   __device__ __forceinline__ bf16x8 vf(int s, int t, int g) const { return step_fp4(v[s][t], scale(vs[s], t, g)); }

@@ -28,7 +28,6 @@ struct VerArgs {
   int64_t u_bs;
   const int32_t* draft_len;
   double scale64;  // 64 log2(e) / T
-  float reach;     // 1500 T
   int32_t* accepted;
   int64_t* tokens;
   int64_t tok_bs;
@@ -46,8 +45,9 @@ template <typename T> __device__ __forceinline__ const T* ver_row(const VerArgs&
 }
 // e^((x - m) / T) in 64 bits: with t = 64 log2(e) (x - m) / T = 64 e + j + f, 2^e times 2^(j / 64) from a
 // table times the series of 2^(f / 64), |f| <= 1/2, whose fifth term is below 4e-14.  (A series for
-// |f| <= 1/2 of a whole octave takes eleven terms: 36 us over 64 x 8 rows of 50257.)  Logits below
-// m - 1500 T, -inf among them, have no mass, nor has NaN or a row whose m is -inf.
+// |f| <= 1/2 of a whole octave takes eleven terms: 36 us over 64 x 8 rows of 50257.)  x - m is exact
+// enough at any size of either, so t is too, however small T; below 2^-3000 there is no mass, nor has
+// -inf, NaN or a row whose m is -inf.
 __device__ const double kVerPow[64] = {  // 2^(j / 64)
     1.0, 1.0108892860517005, 1.0218971486541166, 1.0330248790212284,
     1.0442737824274138, 1.0556451783605572, 1.0671404006768237, 1.0787607977571199,
@@ -74,16 +74,13 @@ struct VerTable {
   }
 };
 struct VerExp {
-  double scale, top;  // 64 log2(e) / T, that times m
-  float low;          // 2^t is 0 from here down
+  double scale, top;  // 64 log2(e) / T, m
   const VerTable& tab;
   __device__ __forceinline__ VerExp(const VerArgs& a, const VerTable& tb, float m)
-      : scale(a.scale64), top((double)m * a.scale64), low(m - a.reach), tab(tb) {
-    if (m == -INFINITY) scale = 0.0, top = 64 * 3000.0, low = 0.f;
-  }
+      : scale(a.scale64), top(m == -INFINITY ? INFINITY : (double)m), tab(tb) {}
   __device__ __forceinline__ double operator()(float x) const {
     constexpr double round = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to whole numbers, in the low bits
-    const double t = fma((double)fmaxf(x, low), scale, -top), u = t + round, f = t - (u - round);
+    const double t = fmax(((double)x - top) * scale, -64 * 3000.0), u = t + round, f = t - (u - round);
     const int i = __double2loint(u);
     constexpr double c1 = 0.69314718055994530942 / 64, c2 = c1 * c1 / 2, c3 = c2 * c1 / 3, c4 = c3 * c1 / 4;
     return __builtin_ldexp(fma(f, fma(f, fma(f, fma(f, c4, c3), c2), c1), 1.0) * tab.at[i & 63], i >> 6);
@@ -371,7 +368,7 @@ extern "C" int capk_verify_drafts(int dtype, int B, int K, int V, const void* ta
   CAPK_CHECK_ARG(dtype == CAPK_F32 || dtype == CAPK_BF16, "capk_verify_drafts: dtype");
   CAPK_CHECK_ARG(B >= 0 && K >= 0 && K <= 1024 && V >= 1 && (int64_t)B * (2 * K + 1) <= 65535 && V <= (1 << 28),
                  "capk_verify_drafts: need 0 <= K <= 1024, V >= 1 and B (2 K + 1) <= 65535 (B %d, K %d, V %d)", B, K, V);
-  CAPK_CHECK_ARG(temperature > 0.0 && temperature < (double)INFINITY, "capk_verify_drafts: temperature must be positive");
+  CAPK_CHECK_ARG(temperature >= 1e-300 && temperature < (double)INFINITY, "capk_verify_drafts: temperature must be positive");
   if (B == 0) return CAPK_OK;
   CAPK_CHECK_ARG(target && (K == 0 || ids) && u && accepted && tokens, "capk_verify_drafts: null pointer");
   const size_t need = capk_verify_drafts_workspace(B, K, V);
@@ -383,7 +380,6 @@ extern "C" int capk_verify_drafts(int dtype, int B, int K, int V, const void* ta
   a.draft = K ? draft : nullptr; a.d_bs = d_bs; a.d_rs = d_rs;
   a.ids = ids; a.ids_bs = ids_bs; a.u = u; a.u_bs = u_bs; a.draft_len = draft_len;
   a.scale64 = 64 * 1.4426950408889634074 / temperature;
-  a.reach = (float)(1500.0 * temperature);
   a.accepted = accepted; a.tokens = tokens; a.tok_bs = tok_bs;
   const size_t rows = (size_t)B * (2 * (size_t)K + 1) * a.chunks;
   a.zs = (double*)ws;

@@ -672,7 +672,8 @@ int capk_rowscale_add(int dtype, int rows, int cols, const void* x, int64_t ldx,
  *   freq fp64, axis uint8 < axes): (x1, x2) -> (x1 cos - x2 sin, x1 sin + x2 cos), angles in
  *   64 bits.  interleaved = 0: pair i = elements i, i + pairs; 1: 2i, 2i + 1.  Elements from
  *   2*pairs on are copied.  inverse = 1 turns back (the gradient).  q and k (Hk = 0: none) in one
- *   launch; y may be x.  Any alignment (whole vectors where it allows).  hd <= 512, Hq + Hk <= 1024. */
+ *   launch; y may be x.  Any alignment (whole vectors where it allows).  hd <= 512, Hq + Hk <= 1024.
+ *   axis entries past the last axis count as the last. */
 int capk_axis_rope(int dtype, int B, int N, int hd, int pairs, int interleaved, int inverse, int axes,
                    const int32_t* pos, int64_t pos_as, int64_t pos_bs, const double* freq, const uint8_t* axis,
                    int Hq, const void* q, int64_t q_bs, int64_t q_rs, int64_t q_hs, void* qo, int64_t qo_bs,
@@ -683,10 +684,12 @@ int capk_axis_rope(int dtype, int B, int N, int hd, int pairs, int interleaved, 
  *   j < sinks or p - j < window (window 0: every j <= p), less those with key_pad[b*Nk + j] != 0.
  *   H query heads share Hk key heads (head h reads h / (H / Hk)).  o = softmax(scale q k^T) v,
  *   lse (fp32 [B, H, Nq], optional forward) its log denominator; a query that sees nothing has
- *   o = 0, lse = -inf.  Keys hidden from every query of a call are never used: NaN there is
- *   harmless.  Nq <= 16 runs the decoding-step kernel (split over the keys, partial results in ws).
- *   Backward: dq, dk, dv (all of them written), deterministic.  hd % 8 == 0, hd <= 128.
- *   Lengths up to 2^28; no dropout. */
+ *   o = 0, lse = -inf (rows before position 0 may hold anything, in q and in the backward's dout).
+ *   Keys hidden from every query of a call are never used: NaN there is harmless; a value that is
+ *   not finite may reach any query of its sequence and head.  Nq <= 16 runs the decoding-step kernel
+ *   (split over the keys, partial results in ws).  Backward: dq, dk, dv (all of them written),
+ *   deterministic.  hd % 8 == 0, hd <= 128; scale positive and finite; lengths up to 2^28, B <=
+ *   65535; tokens less than 2^22 elements apart (0 <= rs); no dropout. */
 size_t capk_sliding_attention_fwd_workspace(int dtype, int B, int H, int Hk, int Nq, int Nk, int hd, int window,
                                             int sinks);
 int capk_sliding_attention_fwd(int dtype, int B, int H, int Hk, int Nq, int Nk, int hd, float scale, int window,
@@ -714,7 +717,8 @@ int capk_sliding_attention_bwd(int dtype, int B, int H, int Hk, int Nq, int Nk, 
  *   else is left as it was.  Two sequences must not write the same page slot in one call.
  * capk_kv4_read: the values of tokens start[b] + i, i < n (zeros where there is no page).
  * capk_kv4_attention: capk_sliding_attention_fwd over the cache for Nq <= 64 queries; keys without a
- *   page are hidden.  kv_len is clamped to [0, table_cols * page]. */
+ *   page are hidden.  kv_len is clamped to [0, table_cols * page].
+ * All three: B <= 65535, Hk <= 32767, n and table_cols * page <= 2^28, page <= 4096. */
 int capk_kv4_append(int dtype, int B, int n, int Hk, int hd, const void* k, int64_t k_bs, int64_t k_rs, int64_t k_hs,
                     const void* v, int64_t v_bs, int64_t v_rs, int64_t v_hs, void* codes, void* scales, int pages,
                     int page, const int32_t* table, int64_t table_ld, int table_cols, const int32_t* start,
@@ -735,7 +739,9 @@ int capk_kv4_attention(int dtype, int B, int H, int Hk, int Nq, int hd, float sc
  *   accepted[b] = n of them, and one more token is drawn with u[b][K] by inverse CDF from
  *   max(p_n - q_n, 0) after a refusal (from p_n where that leaves nothing), from p_n after draft_len
  *   acceptances: the first token whose cumulative mass exceeds u times the whole.  tokens[b][0..K]
- *   = the accepted ids, the drawn token, -1.  64-bit sums.  u in [0, 1) fp32 [B][K + 1]. */
+ *   = the accepted ids, the drawn token, -1.  64-bit sums.  u in [0, 1) fp32 [B][K + 1]; K <= 1024,
+ *   B (2K + 1) <= 65535, temperature >= 1e-300.  A logit of -inf or NaN has no mass; a row without
+ *   any draws token 0. */
 size_t capk_verify_drafts_workspace(int B, int K, int V);
 int capk_verify_drafts(int dtype, int B, int K, int V, const void* target, int64_t t_bs, int64_t t_rs,
                        const void* draft, int64_t d_bs, int64_t d_rs, const int64_t* ids, int64_t ids_bs,

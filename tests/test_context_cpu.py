@@ -99,3 +99,32 @@ def test_python_entry_points_need_a_gpu():
                 dict(pages=1, heads=1, head_dim=64, page=17)):
         with pytest.raises(ValueError):
             context.KV4Cache.empty(device="cpu", **bad)
+
+
+def test_scale_stride_and_size_limits():
+    L = _lib()
+
+    def fwd(scale=1.0, rs=128, Nq=40, Nk=50, B=1, H=2):
+        return L.capk_sliding_attention_fwd(1, B, H, 2, Nq, Nk, 64, scale, 8, 2, P, 0, 128, 64, P, 0, rs, 64, P, 0, 128, 64, None,
+                                            None, P, 0, 128, 64, None, None, 0, None)
+
+    for bad in (0.0, -1.0, float("inf"), float("nan")):
+        assert fwd(scale=bad) == EINVAL
+        assert L.capk_kv4_attention(1, 1, 4, 2, 1, 64, bad, 0, 0, P, 0, 256, 64, P, P, 8, 64, P, 4, 4, P, P, 0, 256, 64, None, P,
+                                    1 << 30, None) == EINVAL
+    assert fwd(rs=1 << 22) == EINVAL and fwd(rs=-128) == EINVAL
+    assert fwd(B=65535, H=65534, Nq=1 << 20) == EINVAL  # more workgroups than a launch has
+    for kw in (dict(hd=514), dict(Hq=1000, Hk=25), dict(B=1 << 20, N=1 << 20)):
+        assert _rope(L, **kw) == EINVAL, kw
+    assert L.capk_verify_drafts(0, 1, 1, 9, P, 0, 0, None, 0, 0, P, 0, P, 0, None, 1e-310, P, P, 2, P, 1 << 20, None) == EINVAL
+
+
+def test_backward_workspace_stays_small():
+    """Partial sums of the far queries, for few and many keys that stay visible."""
+    L = _lib()
+    for N, Hk, G, hd in ((16384, 4, 1, 128), (16384, 1, 8, 128), (65536, 2, 4, 64), (4096, 8, 2, 128)):
+        for window in (1, 128, 2000):
+            for sinks in (1, 4, 200, 2048, N // 2, N):
+                for B in (1, 4):
+                    size = L.capk_sliding_attention_bwd_workspace(B, Hk * G, Hk, N, N, hd, window, sinks)
+                    assert size <= B * Hk * G * N * 4 + (1 << 29), (N, Hk, G, hd, window, sinks, B)

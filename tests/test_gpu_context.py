@@ -701,3 +701,127 @@ def test_refusals():
                  lambda: context.verify_drafts(logits, ids.float(), u)):
         with pytest.raises((CapkError, ValueError)):
             call()
+
+
+# --------------------------------------------------------------------------- rarely used calls ---
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("hd", [64, 96])
+def test_kv4_attention_over_non_finite_blocks(dtype, hd):
+    """A visible block that stands for NaN makes its heads' queries NaN (all elements for a key, the block's for
+    a value), and nothing else."""
+    from capk import context
+    B, n, Hk = 2, 90, 3
+    cache, table = context.KV4Cache.empty(12, Hk, hd, 16), _table(B, 6, 12, seed=3)
+    k, v = (_rand(B, n, Hk, hd, seed=201 + i) for i in (0, 1))
+    k[0, 70, 0, 40], v[0, 71, 1, 33] = math.nan, math.inf
+    k[1, 3], v[1, 4] = math.nan, math.nan  # (hidden by the window)
+    zero = torch.zeros(B, dtype=torch.int32, device="cuda")
+    cache.append(k, v, table, zero)
+    q = _rand(B, 1, 2 * Hk, hd, seed=203, dtype=DT[dtype])
+    o = cache.attend(q, table, zero + n, window=40, sinks=2)[:, 0]
+    assert torch.isnan(o[0, :2]).all() and torch.isfinite(o[1]).all() and torch.isfinite(o[0, 4:]).all()
+    assert torch.isnan(o[0, 2:4, 32:64]).all() and torch.isfinite(o[0, 2:4, :32]).all() and torch.isfinite(o[0, 2:4, 64:]).all()
+
+
+@pytest.mark.parametrize("size", [1.0, 2.0 ** 60])
+@pytest.mark.parametrize("t", [1e-3, 2.0 ** -40, 1e-30, 1e12])
+def test_verify_drafts_temperatures(t, size):
+    """Temperatures down to an arg max and up to a flat row, at logits of any size (in steps of 2^-6 of them, so that
+    no two probabilities but equal ones are near each other)."""
+    from capk import context
+    B, K, V = 4, 3, 1000
+    target, draft = ((torch.round(_rand(B, n, V, seed=211 + n) * 64) / 64 * size) for n in (K + 1, K))
+    ids = target[:, :K].argmax(-1)
+    ids[1, 1] = 5
+    u = torch.rand(B, K + 1, device="cuda", generator=torch.Generator("cuda").manual_seed(212))
+    for d in (draft, None):
+        n, tok = context.verify_drafts(target, ids, u, d, temperature=t)
+        rn, rt = _verify_ref(target, ids, u, d, None, t)
+        assert n.cpu().numpy().tolist() == rn.tolist() and tok.cpu().numpy().tolist() == rt.tolist()
+
+
+def test_sliding_attention_layouts_that_are_copied():
+    """Tokens 2^22 elements apart, an integer key_pad of any non-zero values, and no keys at all."""
+    from capk import context
+    wide = torch.zeros(20, (1 << 22) // 64, 64, dtype=torch.bfloat16, device="cuda")
+    wide[:, :4] = _rand(20, 4, 64, seed=221, dtype=torch.bfloat16)
+    q = wide[:, :4].unsqueeze(0)
+    assert q.stride(1) == 1 << 22
+    pad = torch.zeros(1, 20, dtype=torch.int64, device="cuda")
+    pad[0, 3] = 256
+    o = context.sliding_attention(q, q, q, window=7, sinks=1, key_pad=pad)
+    assert torch.equal(o, context.sliding_attention(*[q.contiguous()] * 3, window=7, sinks=1, key_pad=pad != 0))
+    q = torch.full((2, 3, 4, 64), math.inf, device="cuda", requires_grad=True)
+    o = context.sliding_attention(q, q[:, :0], q[:, :0])
+    o.sum().backward()
+    assert o.shape == q.shape and not o.any() and not q.grad.any()
+
+
+def test_sliding_attention_unseeing_rows_with_any_gradient():
+    """Rows before their sequence's first key: whatever their q and do hold, they give zeros and change nothing."""
+    from capk import ops
+    B, N, H, hd = 1, 700, 2, 64
+    q, k, v, do = (_rand(B, N, H, hd, seed=231 + i, dtype=torch.bfloat16) for i in range(4))
+    kv_len = torch.tensor([600], dtype=torch.int32, device="cuda")  # rows 0..99 stand before position 0
+    args = (0, 0, hd ** -0.5, None, kv_len)
+    o, lse = ops.sliding_attention_fwd(q, k, v, *args)
+    ref = ops.sliding_attention_bwd(q, k, v, o, do, lse, *args)
+    q[:, :100], do[:, :100] = math.nan, math.nan
+    o2, lse2 = ops.sliding_attention_fwd(q, k, v, *args)
+    got = ops.sliding_attention_bwd(q, k, v, o2, do, lse2, *args)
+    assert torch.equal(o, o2) and torch.equal(lse, lse2) and not o[:, :100].any() and not got[0][:, :100].any()
+    assert all(torch.equal(a, b) for a, b in zip(ref, got))
+
+
+def test_one_tensor_for_all_operands():
+    """q, k and v the same leaf: its gradient is the sum of the three."""
+    from capk import context
+    x = _rand(2, 150, 2, 32, seed=241).requires_grad_()
+    do = _rand(2, 150, 2, 32, seed=242)
+    context.sliding_attention(x, x, x, window=20, sinks=3).backward(do)
+    leaves = [x.detach().clone().requires_grad_() for _ in range(3)]
+    context.sliding_attention(*leaves, window=20, sinks=3).backward(do)
+    three = [t.grad for t in leaves]
+    # two additions in either order: a step of 2^-24 each, of sums no larger than the magnitudes'
+    bound = 4 * F * sum(g.double().abs() for g in three)
+    _close(x.grad, sum(g.double() for g in three), bound)
+
+
+def test_calls_on_two_streams_and_graphs_that_take_turns():
+    """Steps with split keys at once on two streams, and two captured graphs replayed in turn, each with workspaces of
+    its own: every result equals the call alone."""
+    from capk import context
+    n, Hk, hd = 4000, 2, 128
+    sets, alone = [], []
+    for i in range(2):
+        cache, table = context.KV4Cache.empty(64, Hk, hd, 64), torch.randperm(64, device="cuda").int().view(1, 64)
+        k, v = (_rand(1, n, Hk, hd, seed=251 + 3 * i + j) for j in (0, 1))
+        cache.append(k, v, table, torch.zeros(1, dtype=torch.int32, device="cuda"))
+        q = _rand(1, 4, 8, hd, seed=253 + 3 * i, dtype=torch.bfloat16)
+        sets.append((q, k.bfloat16(), v.bfloat16(), cache, table, torch.tensor([n], dtype=torch.int32, device="cuda")))
+
+    def call(s):
+        q, k, v, cache, table, length = s
+        return cache.attend(q, table, length), context.sliding_attention(q, k, v, window=3000, sinks=4)
+
+    alone = [[t.clone() for t in call(s)] for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = []
+    for r in range(6):
+        with torch.cuda.stream(streams[r % 2]):
+            got.append(call(sets[r % 2]))
+    torch.cuda.synchronize()
+    for r, g in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(g, alone[r % 2])), r
+    graphs, outs = [], []
+    for s in sets:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(call(s))
+    for r in range(6):
+        graphs[r % 2].replay()
+        call(sets[(r + 1) % 2])
+    torch.cuda.synchronize()
+    for o, a in zip(outs, alone):
+        assert all(torch.equal(x, y) for x, y in zip(o, a))

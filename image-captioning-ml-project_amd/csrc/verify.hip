@@ -9,7 +9,8 @@
 // Three launches: (maximum, sum of exp) of every row in chunks; acceptance and the mass of the row to draw
 // from in chunks; the draw within its chunk.  (Drawing in the last workgroup of the second launch was
 // slower, 27 for 10 us alone and 80 for 22 us at 64 sequences: its fences write the L2 back.)
-// Bound: HBM (each logit once, and the chosen rows again) beside a 64-bit exp per logit.
+// Bound: a 64-bit exp per logit, about 26 vector instructions, of which the first launch runs nine tenths of
+// the time (25 us over 8 of 64 x 15 rows of 50257 bf16 logits in the mean, 2 TB/s; the second 13, the third 8).
 #include "common.h"
 
 namespace capk {
@@ -68,10 +69,9 @@ __device__ const double kVerPow[64] = {  // 2^(j / 64)
 };
 struct VerTable {
   double at[64];
-  __device__ __forceinline__ void fill() {
-    if (threadIdx.x < 64) at[threadIdx.x] = kVerPow[threadIdx.x];
-    __syncthreads();
-  }
+  // requested before a kernel's own loads, stored once those are on their way; a barrier has to follow
+  __device__ __forceinline__ static double load() { return kVerPow[threadIdx.x & 63]; }
+  __device__ __forceinline__ void store(double x) { if (threadIdx.x < 64) at[threadIdx.x] = x; }
 };
 struct VerExp {
   double scale, top;  // 64 log2(e) / T, m
@@ -118,26 +118,26 @@ __global__ __launch_bounds__(256) void verify_rows(VerArgs a) {
   const int rows = a.draft ? 2 * a.K + 1 : a.K + 1, b = blockIdx.y / rows, i = blockIdx.y % rows, c = blockIdx.x;
   const int len = ver_len(a, b);
   if (i <= a.K ? i > len : i - a.K - 1 >= len) return;  // never asked for
-  tab.fill();
+  const double pow = VerTable::load();
   const T* x = ver_row<T>(a, b, i);
-  if (c == 0 && threadIdx.x == 255 && i != a.K) {
-    const int64_t id = a.ids[b * a.ids_bs + (i < a.K ? i : i - a.K - 1)];
-    a.lx[(int64_t)b * (2 * a.K + 1) + i] = id >= 0 && id < a.V ? to_f32(x[id]) : -INFINITY;
-  }
   const int head = min(a.V, (int)((AL - ((uintptr_t)x & (AL - 1))) & (AL - 1)) / (int)sizeof(T));
   const int v0 = head + c * ver_chunk<RUN>();
   float r[RUN], first = -INFINITY, m = -INFINITY;
   if (c == 0 && (int)threadIdx.x < head) m = first = to_f32(x[threadIdx.x]);
+  if (v0 + ver_chunk<RUN>() <= a.V) {
+    vec y[NV];
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int v = v0 + (k * 256 + threadIdx.x) * PER;
-    if (v + PER <= a.V) {
-      const vec y = *(const vec*)(x + v);
+    for (int k = 0; k < NV; ++k) y[k] = *(const vec*)(x + v0 + (k * 256 + threadIdx.x) * PER);
+    tab.store(pow);
 #pragma unroll
-      for (int e = 0; e < PER; ++e) r[k * PER + e] = (float)y[e];
-    } else {
+    for (int k = 0; k < RUN; ++k) r[k] = (float)y[k / PER][k % PER];
+  } else {
+    tab.store(pow);
 #pragma unroll
-      for (int e = 0; e < PER; ++e) r[k * PER + e] = v + e < a.V ? to_f32(x[v + e]) : -INFINITY;
+    for (int k = 0; k < RUN; ++k) {
+      const int v = v0 + (k / PER * 256 + (int)threadIdx.x) * PER + k % PER;
+      const float z = to_f32(x[min(v, a.V - 1)]);
+      r[k] = v < a.V ? z : -INFINITY;
     }
   }
 #pragma unroll
@@ -156,6 +156,10 @@ __global__ __launch_bounds__(256) void verify_rows(VerArgs a) {
     a.ms[at] = m;
     a.zs[at] = z;
   }
+  if (c == 0 && threadIdx.x == 255 && i != a.K) {
+    const int64_t id = a.ids[b * a.ids_bs + (i < a.K ? i : i - a.K - 1)];
+    a.lx[(int64_t)b * (2 * a.K + 1) + i] = id >= 0 && id < a.V ? to_f32(x[id]) : -INFINITY;
+  }
 }
 
 struct VerPick {
@@ -165,41 +169,68 @@ struct VerPick {
   int64_t id;
 };
 // How many drafts are accepted, and the statistics of the row to draw from (whole workgroup).  What it
-// reads does not depend on what it reads, so it pays memory's latency once.
-__device__ __forceinline__ VerPick ver_pick(const VerArgs& a, const VerTable& tab, int b, double* zs, float* ms) {
+// reads does not depend on what it reads and is requested at once (of the drafts past 256, later), so it
+// pays memory's latency once.  Fills the table.
+struct VerDraft {
+  float xp, xq, u;
+  int64_t id;
+  __device__ __forceinline__ void load(const VerArgs& a, int b, int i) {
+    const float* lx = a.lx + (int64_t)b * (2 * a.K + 1);
+    xp = lx[i];
+    xq = a.draft ? lx[a.K + 1 + i] : 0.f;
+    id = a.ids[b * a.ids_bs + i];
+    u = a.u[b * a.u_bs + i];
+  }
+};
+struct VerStats {  // lane l of a row's 16: chunks l, l + 16, .. of the first 64
+  float m[4];
+  double z[4];
+  __device__ __forceinline__ void load(const VerArgs& a, int64_t at, int l) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int c = l + 16 * k, cc = min(c, a.chunks - 1);
+      m[k] = a.ms[at + cc];
+      z[k] = a.zs[at + cc];
+      if (c >= a.chunks) m[k] = -INFINITY, z[k] = 0.0;
+    }
+  }
+};
+__device__ __forceinline__ VerPick ver_pick(const VerArgs& a, VerTable& tab, int b, double* zs, float* ms) {
   __shared__ int first;
   VerPick p;
+  const double pow = VerTable::load();
   p.len = ver_len(a, b);
   const int rows = a.draft ? 2 * a.K + 1 : a.K + 1, l = threadIdx.x & 15;
+  const int64_t at0 = (int64_t)b * (2 * a.K + 1) * a.chunks;
+  VerDraft mine{};
+  if (a.K > 0) mine.load(a, b, min((int)threadIdx.x, a.K - 1));
+  VerStats st;
+  st.load(a, at0 + (int64_t)min((int)threadIdx.x >> 4, rows - 1) * a.chunks, l);
+  tab.store(pow);
   if (threadIdx.x == 0) first = p.len;
+  __syncthreads();
   for (int i = threadIdx.x >> 4; i < rows; i += 16) {  // 16 lanes per row
-    const int64_t at = ((int64_t)b * (2 * a.K + 1) + i) * a.chunks;
-    float m = -INFINITY, mc = -INFINITY;
-    double z = 0.0;
-    if (a.chunks <= 16) {
-      if (l < a.chunks) { m = mc = a.ms[at + l]; z = a.zs[at + l]; }
-    } else {
-      for (int c = l; c < a.chunks; c += 16) m = fmaxf(m, a.ms[at + c]);
-    }
+    const int64_t at = at0 + (int64_t)i * a.chunks;
+    if (i >= 16) st.load(a, at, l);
+    float m = fmaxf(fmaxf(st.m[0], st.m[1]), fmaxf(st.m[2], st.m[3]));
+    for (int c = l + 64; c < a.chunks; c += 16) m = fmaxf(m, a.ms[at + c]);
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 16));
     const VerExp mass(a, tab, m);
-    if (a.chunks <= 16) z *= mass(mc);
-    else
-      for (int c = l; c < a.chunks; c += 16) z += a.zs[at + c] * mass(a.ms[at + c]);
+    double z = 0.0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) z += st.z[k] * mass(st.m[k]);
+    for (int c = l + 64; c < a.chunks; c += 16) z += a.zs[at + c] * mass(a.ms[at + c]);
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) z += __shfl_xor(z, o, 16);
     if (l == 0) { ms[i] = m; zs[i] = z; }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < a.K; i += 256) {
-    const float *lx = a.lx + (int64_t)b * (2 * a.K + 1), xp = lx[i], xq = a.draft ? lx[a.K + 1 + i] : 0.f;
-    const int64_t id = a.ids[b * a.ids_bs + i];
-    const double u = a.u[b * a.u_bs + i];
-    if (i >= p.len) break;
-    const double q = a.draft ? VerExp(a, tab, ms[a.K + 1 + i])(xq) / zs[a.K + 1 + i] : 1.0;
+  for (int i = threadIdx.x; i < p.len; i += 256) {
+    if (i >= 256) mine.load(a, b, i);
+    const double q = a.draft ? VerExp(a, tab, ms[a.K + 1 + i])(mine.xq) / zs[a.K + 1 + i] : 1.0;
     // the smallest refused index: the same in every order
-    if (id < 0 || id >= a.V || !(u * q < VerExp(a, tab, ms[i])(xp) / zs[i])) atomicMin(&first, i);
+    if (mine.id < 0 || mine.id >= a.V || !(mine.u * q < VerExp(a, tab, ms[i])(mine.xp) / zs[i])) atomicMin(&first, i);
   }
   __syncthreads();
   p.n = first;
@@ -232,25 +263,26 @@ template <typename T, int RUN>
 __global__ __launch_bounds__(256) void verify_mass(VerArgs a) {
   __shared__ VerTable tab;
   extern __shared__ double zs[];  // [rows] sums, [rows] maxima
-  tab.fill();
   const int b = blockIdx.y, v0 = blockIdx.x * ver_chunk<RUN>();
   const VerPick p = ver_pick(a, tab, b, zs, (float*)(zs + 2 * a.K + 1));
   if (blockIdx.x == 0 && threadIdx.x == 0) a.pick[b] = p;
   const bool two = a.draft && p.n < p.len;
   const T *tr = ver_row<T>(a, b, p.n), *dr = two ? ver_row<T>(a, b, a.K + 1 + p.n) : tr;
   const VerMass mass(a, tab, p);
-  float t[RUN], d[RUN];
+  T t[RUN], d[RUN];  // (loads without a condition: behind one each would be waited for)
 #pragma unroll
   for (int k = 0; k < RUN; ++k) {
-    const int v = v0 + k * 256 + threadIdx.x;
-    t[k] = v < a.V ? to_f32(tr[v]) : -INFINITY;
-    d[k] = v < a.V ? to_f32(dr[v]) : -INFINITY;
+    const int v = min(v0 + k * 256 + (int)threadIdx.x, a.V - 1);
+    t[k] = tr[v];
+    d[k] = dr[v];
   }
   double r = 0.0, w = 0.0;
 #pragma unroll
   for (int k = 0; k < RUN; ++k) {
+    const int v = v0 + k * 256 + threadIdx.x;
     double y;
-    r += mass(t[k], d[k], v0 + k * 256 + threadIdx.x, y);
+    const double x = mass(v < a.V ? to_f32(t[k]) : -INFINITY, to_f32(d[k]), v, y);
+    r += x;
     w += y;
   }
   r = ver_block_sum(r);
@@ -269,6 +301,7 @@ __global__ __launch_bounds__(1024) void verify_draw(VerArgs a) {
   __shared__ int best, last;
   __shared__ double ws[16];
   const int b = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const double pow = VerTable::load();
   const VerPick p = a.pick[b];
   const double u = a.u[b * a.u_bs + a.K];
   const int64_t my_id = (int)threadIdx.x < a.K ? a.ids[b * a.ids_bs + threadIdx.x] : -1;  // (K <= 1024)
@@ -300,19 +333,21 @@ __global__ __launch_bounds__(1024) void verify_draw(VerArgs a) {
   // the same within the chunk
   const T *tr = ver_row<T>(a, b, p.n), *dr = a.draft && p.n < p.len ? ver_row<T>(a, b, a.K + 1 + p.n) : tr;
   const int v0 = pick * ver_chunk<RUN>() + threadIdx.x * PER;
-  float xt[PER], xd[PER];
+  T xt[PER], xd[PER];
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
-    xt[k] = v0 + k < a.V ? to_f32(tr[v0 + k]) : -INFINITY;
-    xd[k] = v0 + k < a.V ? to_f32(dr[v0 + k]) : -INFINITY;
+    const int v = min(v0 + k, a.V - 1);
+    xt[k] = tr[v];
+    xd[k] = dr[v];
   }
-  tab.fill();
+  tab.store(pow);
+  __syncthreads();
   const VerMass mass(a, tab, p);
   double run[PER], mine = 0.0;
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
     double y;
-    run[k] = mass(xt[k], xd[k], v0 + k, y);
+    run[k] = mass(v0 + k < a.V ? to_f32(xt[k]) : -INFINITY, to_f32(xd[k]), v0 + k, y);
     if (whole) run[k] = y;
     mine += run[k];
   }

@@ -49,8 +49,20 @@ struct SlideBlock {
   }
 };
 
+// Fragments of a row, zeros where !ok or past hd.  The loads are of a valid row in any case and without
+// conditions: behind one each would be waited for.
 template <typename T, int HDP>
 __device__ __forceinline__ void slide_frags(typename Mat<T>::V8 (&f)[HDP / 16], const T* src, bool ok, int hd, int h) {
+  typename Tile<T>::V8 x[HDP / 16];
+#pragma unroll
+  for (int s = 0; s < HDP / 16; ++s) x[s] = Tile<T>::load(src + (s * 16 + h * 8 < hd ? s * 16 + h * 8 : 0));
+#pragma unroll
+  for (int s = 0; s < HDP / 16; ++s) f[s] = Mat<T>::from(ok && s * 16 + h * 8 < hd ? x[s] : tile_zero8<T>());
+}
+// The same with conditional loads (src is read only where ok): in slide_dkv, whose registers are all taken, the
+// unconditional form is allocated worse (306 us for 299 at 16384 tokens).
+template <typename T, int HDP>
+__device__ __forceinline__ void slide_frags_if(typename Mat<T>::V8 (&f)[HDP / 16], const T* src, bool ok, int hd, int h) {
 #pragma unroll
   for (int s = 0; s < HDP / 16; ++s) {
     typename Tile<T>::V8 x = tile_zero8<T>();
@@ -185,6 +197,7 @@ __global__ __launch_bounds__(256 * GROUPS, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) 
   const SlideBlock at(a);
   const int b = at.b, kvh = at.kvh, G = a.H / a.Hk, h = kvh * G + at.rest % G, len = slide_len(a, b), off = len - a.Nq;
   const int q0 = ((a.Nq + 127) / 128 - 1 - at.rest / G) * 128, qw = q0 + w * 32, qi = qw + (lane & 31), p = off + qi;
+  const int qr = min(qi, a.Nq - 1);  // a row to load
   const int p_lo = off + q0, p_hi = off + min(q0 + 127, a.Nq - 1);
   const int pw_lo = off + qw, pw_hi = off + qw + 31;
   const float c = a.scale * kTileLog2e;
@@ -195,7 +208,7 @@ __global__ __launch_bounds__(256 * GROUPS, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) 
   if (grp < tiles.n) kv.fetch(tiles.key0(grp), last, 0);
 
   typename Mat<T>::V8 qf[NS];
-  slide_frags<T, HDP>(qf, row<T>(a.q, b, qi, h), qi < a.Nq, a.hd, hh);
+  slide_frags<T, HDP>(qf, row<T>(a.q, b, qr, h), qi < a.Nq, a.hd, hh);
   f32x16 o[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) o[d] = tile_zero<f32x16>();
@@ -299,6 +312,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) : HDP <= 
   const SlideBlock at(a);
   const int b = at.b, kvh = at.kvh, G = a.H / a.Hk, h = kvh * G + at.rest % G, len = slide_len(a, b), off = len - a.Nq;
   const int q0 = ((a.Nq + 127) / 128 - 1 - at.rest / G) * 128, qw = q0 + w * 32, qi = qw + (lane & 31), p = off + qi;
+  const int qr = min(qi, a.Nq - 1);  // a row to load
   const int p_lo = off + q0, p_hi = off + min(q0 + 127, a.Nq - 1);
   const int pw_lo = off + qw, pw_hi = off + qw + 31;
   const float c = a.scale * kTileLog2e;
@@ -309,24 +323,31 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) : HDP <= 
   if (tiles.n) kv.fetch(tiles.key0(0), last, 0);
 
   typename Mat<T>::V8 qf[NS], dof[NS];
-  slide_frags<T, HDP>(qf, row<T>(a.q, b, qi, h), qi < a.Nq, a.hd, hh);
-  slide_frags<T, HDP>(dof, row<T>(a.dout, b, qi, h), qi < a.Nq, a.hd, hh);
+  slide_frags<T, HDP>(qf, row<T>(a.q, b, qr, h), qi < a.Nq, a.hd, hh);
+  slide_frags<T, HDP>(dof, row<T>(a.dout, b, qr, h), qi < a.Nq, a.hd, hh);
   const int64_t stat = ((int64_t)b * a.H + h) * a.Nq + qi;
-  const float lse2 = qi < a.Nq ? a.lse[stat] * kTileLog2e : INFINITY;
+  const float lse = a.lse[stat - qi + qr], lse2 = qi < a.Nq ? lse * kTileLog2e : INFINITY;
   // D from the saved output costs a pass over one row, but inherits that output's rounding, which weighs
   // where few keys share a row.  With at most 4 tiles of keys D is summed from P (do v^T) itself, in a
   // walk of its own.
   const bool walk = tiles.n <= 4;
   float delta = 0.f;
   if (!walk) {
-    const T *o = row<T>(a.o, b, qi, h), *d = row<T>(a.dout, b, qi, h);
+    const T *o = row<T>(a.o, b, qr, h), *d = row<T>(a.dout, b, qr, h);
+    typename Tile<T>::V8 x[NS], y[NS];
 #pragma unroll
-    for (int s = 0; s < NS; ++s)
-      if (qi < a.Nq && s * 16 + hh * 8 < a.hd) {
-        const typename Tile<T>::V8 x = Tile<T>::load(o + s * 16 + hh * 8), y = Tile<T>::load(d + s * 16 + hh * 8);
+    for (int s = 0; s < NS; ++s) {
+      const int at = s * 16 + hh * 8 < a.hd ? s * 16 + hh * 8 : 0;
+      x[s] = Tile<T>::load(o + at);
+      y[s] = Tile<T>::load(d + at);
+    }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) delta = fmaf((float)x[e], (float)y[e], delta);
-      }
+    for (int s = 0; s < NS; ++s) {
+      float f = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f = fmaf((float)x[s][e], (float)y[s][e], f);
+      if (s * 16 + hh * 8 < a.hd) delta += f;
+    }
     delta += __shfl_xor(delta, 32, 64);
     if (lse2 == -INFINITY) delta = 0.f;  // (it sees nothing, and its do may be anything)
   }
@@ -445,8 +466,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void s
   };
   if (all) fetch(0, 0);
   typename Mat<T>::V8 kf[NS], vf[NS];
-  slide_frags<T, HDP>(kf, row<T>(a.k, b, j, kvh), key_ok, a.hd, hh);
-  slide_frags<T, HDP>(vf, row<T>(a.v, b, j, kvh), key_ok, a.hd, hh);
+  slide_frags_if<T, HDP>(kf, row<T>(a.k, b, j, kvh), key_ok, a.hd, hh);
+  slide_frags_if<T, HDP>(vf, row<T>(a.v, b, j, kvh), key_ok, a.hd, hh);
   const bool hidden = __builtin_amdgcn_ballot_w64(!key_ok) != 0;
   f32x16 dk[ND], dv[ND];
 #pragma unroll

@@ -245,7 +245,7 @@ __global__ __launch_bounds__(256 * GROUPS, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) 
     float mt = -INFINITY;
 #pragma unroll
     for (int i = 0; i < 16; ++i) mt = fmaxf(fmaxf(mt, s[0][i]), s[1][i]);
-    mt = fmaxf(mt, __shfl_xor(mt, 32, 64)) * c;
+    mt = tile_max32(mt) * c;
     if (__builtin_amdgcn_ballot_w64(mt > mc + 8.f)) {
       const float mn = fmaxf(mc, mt), alpha = mn == -INFINITY ? 1.f : tile_exp2(mc - mn);
       mc = mn;
@@ -274,7 +274,7 @@ __global__ __launch_bounds__(256 * GROUPS, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) 
       for (int d = 0; d < ND; ++d) o[d] = Mat<T>::mma32(vf[u & 1][d], pf, o[d]);
     }
   }
-  l += __shfl_xor(l, 32, 64);
+  l = tile_sum32(l);
   if constexpr (GROUPS == 2) {  // the groups' partial softmaxes joined: registers of the second through LDS
     __syncthreads();
     float* x = (float*)smem + (threadIdx.x & 255);
@@ -348,7 +348,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) : HDP <= 
       for (int e = 0; e < 8; ++e) f = fmaf((float)x[s][e], (float)y[s][e], f);
       if (s * 16 + hh * 8 < a.hd) delta += f;
     }
-    delta += __shfl_xor(delta, 32, 64);
+    delta = tile_sum32(delta);
     if (lse2 == -INFINITY) delta = 0.f;  // (it sees nothing, and its do may be anything)
   }
   f32x16 dq[ND];
@@ -394,7 +394,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) : HDP <= 
         for (int i = 0; i < 16; ++i) delta = fmaf(s[i], dp[i], delta);
       }
     }
-    delta += __shfl_xor(delta, 32, 64);
+    delta = tile_sum32(delta);
   }
   for (int t = 0; t < tiles.n; ++t, buf ^= 1) {
     const int j0 = tiles.key0(t);

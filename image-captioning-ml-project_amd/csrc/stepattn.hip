@@ -246,8 +246,7 @@ __global__ __launch_bounds__(256, (step_waves<KV4, T, HDP, NRT>())) void step_at
       float mt = x[0];
 #pragma unroll
       for (int e = 1; e < 8; ++e) mt = fmaxf(mt, x[e]);
-      mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
-      mt = fmaxf(mt, __shfl_xor(mt, 32, 64)) * c;
+      mt = tile_max32(tile_max16(mt)) * c;
       if (__builtin_amdgcn_ballot_w64(mt > m[rt] + 8.f)) {
         const float mn = fmaxf(m[rt], mt), alpha = mn == -INFINITY ? 1.f : tile_exp2(m[rt] - mn);
         m[rt] = mn;
@@ -286,9 +285,7 @@ __global__ __launch_bounds__(256, (step_waves<KV4, T, HDP, NRT>())) void step_at
   float* ms = os + 4 * 16 * OST;          // [4][16] maximum, [4][16] sum
 #pragma unroll
   for (int rt = 0; rt < NRT; ++rt) {
-    float lt = l[rt];
-    lt += __shfl_xor(lt, 16, 64);
-    lt += __shfl_xor(lt, 32, 64);
+    const float lt = tile_sum32(tile_sum16(l[rt]));
     __syncthreads();
 #pragma unroll
     for (int d = 0; d < ND; ++d) *(f32x4*)(os + (w * 16 + (lane & 15)) * OST + d * 16 + 4 * g) = o[rt][d];

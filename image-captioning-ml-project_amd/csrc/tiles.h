@@ -223,5 +223,19 @@ __device__ __forceinline__ f32x8 tile_trans16(const float* img, int st, int r0, 
 }
 // v_exp_f32: 2^x; the arguments below are <= 0 or -inf (-> 0)
 __device__ __forceinline__ float tile_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+// Sum / maximum with the lane 16 (32) away: a swap of the rows' odd and even (upper and lower) halves between two
+// copies, in registers (through LDS, as shuffles go, it is 100 cycles and more in the path of every tile).
+__device__ __forceinline__ f32x2 tile_swap16(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return (f32x2){__uint_as_float(r[0]), __uint_as_float(r[1])};
+}
+__device__ __forceinline__ f32x2 tile_swap32(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return (f32x2){__uint_as_float(r[0]), __uint_as_float(r[1])};
+}
+__device__ __forceinline__ float tile_max16(float x) { const f32x2 r = tile_swap16(x); return fmaxf(r[0], r[1]); }
+__device__ __forceinline__ float tile_max32(float x) { const f32x2 r = tile_swap32(x); return fmaxf(r[0], r[1]); }
+__device__ __forceinline__ float tile_sum16(float x) { const f32x2 r = tile_swap16(x); return r[0] + r[1]; }
+__device__ __forceinline__ float tile_sum32(float x) { const f32x2 r = tile_swap32(x); return r[0] + r[1]; }
 
 }  // namespace capk

@@ -53,7 +53,7 @@ template <typename T, int HDP> struct StepTile<false, T, HDP> {
   typename Tile<T>::V8 k[2][NS], v[2][NS];
   uint32_t hid;
   __device__ __forceinline__ static int elem(int t, int g) { return 32 * t + 8 * g; }
-  __device__ __forceinline__ void load(const StepArgs& a, int b, int kvh, int j0, int last, int lo, int, int, int lane) {
+  __device__ __forceinline__ void load(const StepArgs& a, int b, int kvh, int j0, int last, int lo, uint32_t, int, int lane) {
     hid = 0;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
@@ -84,23 +84,30 @@ template <typename T, int HDP> struct StepTile<true, T, HDP> {
   uint8_t ks[2][HDP == 96 ? 2 : 1], vs[2][HDP == 96 ? 2 : 1];  // scale codes of the first (and the last) run
   uint32_t hid;
   __device__ __forceinline__ static int elem(int t, int g) { return g * (HDP / 4) + 8 * t; }
-  // pages: the page of every 16 keys of the next tiles, one per lane; `at` is this tile's first
-  __device__ __forceinline__ void load(const StepArgs& a, int b, int kvh, int j0, int last, int lo, int pages, int at, int lane) {
+  // 16 keys from a multiple of 16 on lie in one page: the sixteenth of the row (of all pages' key rows) where they
+  // start, ~0 without a page
+  __device__ __forceinline__ static uint32_t piece(const StepArgs& a, int b, int kvh, int j) {
+    const int at = j / a.page, pg = a.table[(int64_t)b * a.table_ld + at];
+    const int64_t r = ((int64_t)pg * 2 * a.Hk + kvh) * (a.page / 16) + (j - at * a.page) / 16;
+    return pg < 0 || pg >= a.pages ? ~0u : (uint32_t)r;  // (2^32 sixteenths are more than memory holds)
+  }
+  // pieces: those of the next tiles, one per lane; `at` is this tile's first
+  __device__ __forceinline__ void load(const StepArgs& a, int b, int kvh, int j0, int last, int lo, uint32_t pieces, int at, int lane) {
     hid = 0;
     const int g = lane >> 4, e0 = elem(0, g) / 32, e1 = elem(NS - 1, g) / 32;
+    const int64_t to_v = (int64_t)a.Hk * (a.page / 16);
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const int js = j0 + 16 * s, j = js + (lane & 15);
-      const int pg = __builtin_amdgcn_readlane(pages, at + s);  // 16 keys from a multiple of 16 lie in one page
-      const bool page_ok = pg >= 0 && pg < a.pages;
-      const bool ok = (j < last) & ((j < a.sinks) | (j >= lo)) & page_ok;
+      const int j = j0 + 16 * s + (lane & 15);
+      const uint32_t pc = __builtin_amdgcn_readlane(pieces, at + s);
+      const bool ok = (j < last) & ((j < a.sinks) | (j >= lo)) & (pc != ~0u);
       hid |= (uint32_t)(~__builtin_amdgcn_ballot_w64(ok) & 0xffff) << (16 * s);
-      const int64_t kr = ((int64_t)(page_ok ? pg : 0) * 2 * a.Hk + kvh) * a.page + js % a.page, vr = kr + (int64_t)a.Hk * a.page;
+      const int64_t kr = pc == ~0u ? 0 : pc, vr = kr + to_v;
       const uint32_t o = (lane & 15) * (HDP / 2) + g * (HDP / 8), so = (lane & 15) * NB;
-      const uint32_t *kc = (const uint32_t*)(a.codes + kr * (HDP / 2) + o), *vc = (const uint32_t*)(a.codes + vr * (HDP / 2) + o);
+      const uint32_t *kc = (const uint32_t*)(a.codes + kr * (8 * HDP) + o), *vc = (const uint32_t*)(a.codes + vr * (8 * HDP) + o);
 #pragma unroll
       for (int t = 0; t < NS; ++t) { k[s][t] = kc[t]; v[s][t] = vc[t]; }
-      const uint8_t *kss = a.scales + kr * NB + so, *vss = a.scales + vr * NB + so;
+      const uint8_t *kss = a.scales + kr * (16 * NB) + so, *vss = a.scales + vr * (16 * NB) + so;
       ks[s][0] = kss[e0];
       vs[s][0] = vss[e0];
       if constexpr (HDP == 96) {
@@ -147,7 +154,7 @@ __global__ __launch_bounds__(256, (step_waves<KV4, T, HDP, NRT>())) void step_at
   constexpr int NS = HDP / 32, ND = HDP / 16, PARTS = Ty::PARTS, IST = HDP + 16, OST = HDP + 4;
   constexpr int KT = 32, GROUP = 32;  // keys of a tile; tiles whose pages a wave holds at a time
   extern __shared__ __align__(16) char smem[];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
   const int b = blockIdx.z, kvh = blockIdx.y % a.Hk, r0 = blockIdx.y / a.Hk * 16 * NRT, R = a.Nq * (a.H / a.Hk);
   const int len = a.len ? min(max(a.len[b], 0), a.cap) : a.cap, off = len - a.Nq;
   const float c = a.scale * kTileLog2e;
@@ -161,19 +168,23 @@ __global__ __launch_bounds__(256, (step_waves<KV4, T, HDP, NRT>())) void step_at
   // tiles in flight: 4-bit ones are small, and three of them cover the latency of memory
   constexpr int RING = KV4 ? 3 : 2;
   St ring[RING];
-  int pages = -1;  // the pages of the GROUP tiles from ta + i GROUP on, one 16-key piece per lane
+  uint32_t pieces = ~0u;  // where the GROUP tiles from ta + i GROUP on lie, one 16-key piece per lane
+  // Every turn fetches a tile (behind the last one, that again, from the caches): with a tile left out now and then
+  // the compiler, which has to count loads on every path, would wait for all of them.
   auto fetch = [&](St& st, int t) {
     if constexpr (KV4) {
-      if ((t - ta) % GROUP == 0) {
+      if ((t - ta) % GROUP == 0 && t < tb) {
         const int tt = t + lane / 2, j = tt < tb ? tiles.key0(tt) + lane % 2 * 16 : len;
-        pages = j < len ? a.table[(int64_t)b * a.table_ld + j / a.page] : -1;
+        pieces = j < len ? St::piece(a, b, kvh, j) : ~0u;
       }
     }
-    st.load(a, b, kvh, tiles.key0(t), len, lo, pages, (t - ta) % GROUP * 2, lane);
+    t = min(t, tb - 1);
+    st.load(a, b, kvh, tiles.key0(t), len, lo, pieces, (t - ta) % GROUP * 2, lane);
   };
+  if (ta < tb) {
 #pragma unroll
-  for (int i = 0; i + 1 < RING; ++i)
-    if (ta + i < tb) fetch(ring[i], ta + i);
+    for (int i = 0; i + 1 < RING; ++i) fetch(ring[i], ta + i);
+  }
 
   F qf[NRT][NS][PARTS];
   int pos[NRT];
@@ -276,7 +287,7 @@ __global__ __launch_bounds__(256, (step_waves<KV4, T, HDP, NRT>())) void step_at
 #pragma unroll
     for (int i = 0; i < RING; ++i) {
       if (t + i >= tb) break;
-      if (t + i + RING - 1 < tb) fetch(ring[(i + RING - 1) % RING], t + i + RING - 1);
+      fetch(ring[(i + RING - 1) % RING], t + i + RING - 1);
       compute(ring[i], t + i);
     }
   }

@@ -231,7 +231,18 @@ __global__ __launch_bounds__(256 * GROUPS, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) 
     typename Mat<T>::V8 vf[2][ND];  // V^T fragments of a 16-key step, requested a step ahead
 #pragma unroll
     for (int d = 0; d < ND; ++d) vf[0][d] = Img::trans(vi, 0, d * 32, ln);
-    if (hid || !slide_full(a, j0, 64, pw_lo, pw_hi)) {
+    // most masked tiles: three instructions per score, not eight (at 96, where three waves share a SIMD, the second
+    // form of the mask spills: 97 us for 65 over 16 x 1024 tokens)
+    if (HDP != 96 && !hid && j0 >= a.sinks) {
+      if (!slide_full(a, j0, 64, pw_lo, pw_hi)) {
+        const int d = p - j0 - 4 * hh;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            s[kb][i] = (unsigned)(d - (kb * 32 + 8 * (i >> 2) + (i & 3))) < (unsigned)a.window ? s[kb][i] : -INFINITY;
+      }
+    } else if (hid || !slide_full(a, j0, 64, pw_lo, pw_hi)) {
       const uint32_t hl[2] = {(uint32_t)hid >> (4 * hh), (uint32_t)(hid >> 32) >> (4 * hh)};
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)

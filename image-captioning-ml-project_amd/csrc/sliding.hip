@@ -7,13 +7,22 @@
 //
 // Forward: a workgroup owns 128 queries of a head (4 waves x 32), walks the key tiles that hold sinks
 // and then those of its window, and keeps a running maximum and sum (one pass).  S^T = K Q^T puts one
-// query on each lane, so the row statistics need one shuffle, and P^T, already in B-operand order, is
-// multiplied by V^T fragments read transposed from LDS.
+// query on each lane, so the row statistics need one swap, and P^T, already in B-operand order, is
+// multiplied by V^T fragments read transposed from LDS.  A tile's 16 + 16 products of 32 cycles (hd 128)
+// stand beside about 1100 cycles of softmax and 1000 of LDS reads (each wave reads the whole tile for its 32
+// queries), so no unit is saturated: 187 us for 16384 tokens, window 1024, 16 heads of 128 (146 GFLOP, 780
+// TF/s of the 1600 that a large product reaches); 64 queries per wave would halve the LDS reads, but its 128
+// sums then travel between the two halves of the register file every tile (700 us).
 // Backward: D = rowsum(do * o); P = exp(s - lse); dS = P (do v^T - D) scale.  One kernel owns queries
 // (dQ^T += K^T dS^T), one owns keys and walks their queries over all heads of the group
-// (dV^T += dO^T P, dK^T += Q^T dS): every sum has one owner, so results do not depend on timing.  Keys
+// (dV^T += dO^T P, dK^T += Q^T dS): every sum has one owner, so results do not depend on timing.  S and dP are
+// computed in both (seven products for five): one kernel for all would add dQ through atomics.  The same
+// tokens: dQ 233 us (940 TF/s), dK and dV 300 us (970), bound by LDS reads as the forward is.  Keys
 // that stay visible are seen by all later queries: those far queries are cut into chunks with owners
-// of their own, whose 32-bit partial sums one more kernel adds in a fixed order.
+// of their own, whose 32-bit partial sums one more kernel adds in a fixed order (7 us).
+//
+// fp32: three bf16 parts per value and six part products per product (tiles.h), at 16 times the rate of the fp32
+// matrix instructions.
 #include "sliding.h"
 
 namespace capk {

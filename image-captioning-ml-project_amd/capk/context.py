@@ -44,24 +44,32 @@ def _unit(t):
     return t if t is None or t.dim() != 4 or t.stride(3) == 1 else t.contiguous()
 
 
+# (The backward passes run in the engine's thread, on a cold core: what can be checked, converted and looked up is,
+# in the forward.)
 class _AxisRope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, pos, freq, axis, interleaved):
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(pos, freq, axis)
-        ctx.interleaved = interleaved
-        return ops.axis_rope(_unit(q), _unit(k), pos, freq, axis, interleaved=interleaved)
+        q, k = _unit(q), _unit(k)
+        sizes, *table = ops._axis_rope_args(q, k, pos, freq, axis)
+        out_q, out_k = q.new_empty(q.shape), None if k is None else k.new_empty(k.shape)
+        ops._axis_rope_run(sizes, *table, q, k, out_q, out_k, int(interleaved), 0)
+        ctx.save_for_backward(*table)
+        ctx.rule = (sizes, int(interleaved))
+        return out_q, out_k
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gq, gk):
-        pos, freq, axis = ctx.saved_tensors
-        kw = dict(interleaved=ctx.interleaved, inverse=True)
-        if gq is None:
-            dq, dk = None, None if gk is None else ops.axis_rope(_unit(gk), None, pos, freq, axis, **kw)[0]
-        else:
-            dq, dk = ops.axis_rope(_unit(gq), _unit(gk), pos, freq, axis, **kw)
-        return dq, dk, None, None, None, None
+        sizes, interleaved = ctx.rule
+        if gq is None and gk is None:
+            return None, None, None, None, None, None
+        g = [_unit(x) for x in (gq, gk)]
+        d = [None if x is None else x.new_empty(x.shape) for x in g]
+        first = 0 if gq is not None else 1
+        second = 1 if first == 0 else 0
+        ops._axis_rope_run(sizes, *ctx.saved_tensors, g[first], g[second], d[first], d[second], interleaved, 1)
+        return d[0], d[1], None, None, None, None
 
 
 def axis_rope(q, k, pos, freq, axis, *, interleaved=False):
@@ -75,16 +83,18 @@ class _SlidingAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, window, sinks, scale, key_pad, kv_len):
         q, k, v = _rows(q), _rows(k), _rows(v)
-        o, lse = ops.sliding_attention_fwd(q, k, v, window, sinks, scale, key_pad, kv_len)
+        args = ops._sliding_args("sliding_attention", q, k, v, window, sinks, key_pad, kv_len)
+        o, lse = ops._sliding_fwd_run(*args, q, scale, q.new_empty(q.shape), True)
+        code, dims, rule, _, key_pad, kv_len = args
         ctx.save_for_backward(q, k, v, o, lse, key_pad, kv_len)
-        ctx.rule = (window, sinks, scale)
+        ctx.rule = ((code, *dims), rule, scale)
         return o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
         q, k, v, o, lse, key_pad, kv_len = ctx.saved_tensors
-        dq, dk, dv = ops.sliding_attention_bwd(q, k, v, o, _rows(do), lse, *ctx.rule, key_pad, kv_len)
+        dq, dk, dv = ops._sliding_bwd_run(*ctx.rule, q, k, v, o, _rows(do), lse, key_pad, kv_len)
         return dq, dk, dv, None, None, None, None, None
 
 

@@ -1321,32 +1321,46 @@ def _view4(what, t):
     return t.data_ptr(), s[0] if shape[0] > 1 else 0, s[1] if shape[1] > 1 else 0, s[2] if shape[2] > 1 else 0
 
 
+def _axis_rope_args(q, k, pos, freq, axis):
+    """(sizes, pos, freq, axis) of a rotation of q and k after all checks; the tensors in the kernel's types."""
+    _same("axis_rope", q, k)
+    code = dtype_code(q)
+    if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3])):
+        raise ValueError(f"axis_rope: q {tuple(q.shape)}, k {None if k is None else tuple(k.shape)}: need [B, N, heads, hd]")
+    B, N, H, hd = q.shape
+    if pos.dim() not in (2, 3) or tuple(pos.shape[1:]) not in ((B, N), (N,)) or not pos.shape[0]:
+        raise ValueError(f"axis_rope: positions [axes, {B}, {N}] or [axes, {N}], got {tuple(pos.shape)}")
+    if freq.dtype != torch.float64 or freq.dim() != 1 or freq.device != q.device:
+        raise ValueError("axis_rope: frequencies must be fp64 [pairs] on the operands' device")
+    pos = _index("axis_rope: positions", pos, pos.shape, torch.int32, q.device)
+    axis = _index("axis_rope: axis", axis, (freq.shape[0],), torch.uint8, q.device)
+    return (code, B, N, hd, freq.shape[0]), pos, freq.contiguous(), axis
+
+
+def _axis_rope_run(sizes, pos, freq, axis, q, k, out_q, out_k, interleaved, inverse):
+    what = "axis_rope"
+    if k is None:
+        Hk, kv = 0, (None, 0, 0, 0) * 2
+    else:
+        Hk, kv = k.shape[2], _view4(what, k) + _view4(what, out_k)
+    _launch(q.device, "capk_axis_rope", *sizes, interleaved, inverse, pos.shape[0], pos.data_ptr(), pos.stride(0),
+            pos.stride(1) if pos.dim() == 3 else 0, freq.data_ptr(), axis.data_ptr(), q.shape[2], *_view4(what, q),
+            *_view4(what, out_q), Hk, *kv)
+
+
 def axis_rope(q, k, pos, freq, axis, *, interleaved=False, inverse=False, out_q=None, out_k=None):
     """Rotary positions over several axes (capk_axis_rope) of q [B, N, H, hd] and k [B, N, Hk, hd] (or
     None); pos int [axes, B, N] or [axes, N], freq fp64 [pairs], axis [pairs].  out_q / out_k may be q / k."""
-    what = "axis_rope"
+    args = _axis_rope_args(q, k, pos, freq, axis)
+    for x, out in ((q, out_q), (k, out_k)):
+        if out is not None:
+            _same("axis_rope", q, out)
+            if x is None or out.shape != x.shape:
+                raise ValueError(f"axis_rope: an output {tuple(out.shape)} for {None if x is None else tuple(x.shape)}")
     out_q = q.new_empty(q.shape) if out_q is None else out_q
     if k is not None and out_k is None:
         out_k = k.new_empty(k.shape)
-    _same(what, q, k, out_q, out_k)
-    code = dtype_code(q)
-    qv, qov = _view4(what, q), _view4(what, out_q)
-    B, N, H, hd = q.shape
-    if out_q.shape != q.shape or (k is not None and (k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != hd
-                                                     or out_k.shape != k.shape)):
-        raise ValueError(f"axis_rope: q {tuple(q.shape)}, k {None if k is None else tuple(k.shape)} and the outputs differ")
-    if pos.dim() not in (2, 3) or tuple(pos.shape[1:]) not in ((B, N), (N,)) or not pos.shape[0]:
-        raise ValueError(f"axis_rope: positions [axes, {B}, {N}] or [axes, {N}], got {tuple(pos.shape)}")
-    pairs = freq.shape[0]
-    pos = _index("axis_rope: positions", pos, pos.shape, torch.int32, q.device)
-    axis = _index("axis_rope: axis", axis, (pairs,), torch.uint8, q.device)
-    if freq.dtype != torch.float64 or freq.dim() != 1 or freq.device != q.device:
-        raise ValueError("axis_rope: frequencies must be fp64 [pairs] on the operands' device")
-    freq = freq.contiguous()
-    kv, kov = (_view4(what, k), _view4(what, out_k)) if k is not None else ((None, 0, 0, 0), (None, 0, 0, 0))
-    _launch(q.device, "capk_axis_rope", code, B, N, hd, pairs, int(interleaved), int(inverse), pos.shape[0],
-            pos.data_ptr(), pos.stride(0), pos.stride(1) if pos.dim() == 3 else 0, freq.data_ptr(), axis.data_ptr(),
-            H, *qv, *qov, 0 if k is None else k.shape[2], *kv, *kov)
+    _axis_rope_run(*args, q, k, out_q, out_k, int(interleaved), int(inverse))
     return out_q, out_k
 
 
@@ -1368,40 +1382,51 @@ def _sliding_args(what, q, k, v, window, sinks, key_pad, kv_len):
     return dtype_code(q), (B, H, Hk, Nq, Nk, hd), (int(window), int(sinks)), views, key_pad, kv_len
 
 
+def _sliding_fwd_run(code, dims, rule, views, key_pad, kv_len, q, scale, out, want_lse):
+    dev = q.device
+    lse = torch.empty(q.shape[0], q.shape[2], q.shape[1], dtype=torch.float32, device=dev) if want_lse else None
+    wsb = _ws_bytes("capk_sliding_attention_fwd_workspace", code, *dims, *rule)
+    ws = _ws(wsb, dev)
+    _launch(dev, "capk_sliding_attention_fwd", code, *dims, scale, *rule, *views, _p(key_pad), _p(kv_len),
+            *_view4("sliding_attention_fwd", out), _p(lse), _p(ws), wsb)
+    return out, lse
+
+
 def sliding_attention_fwd(q, k, v, window, sinks, scale, key_pad=None, kv_len=None, *, out=None, want_lse=True):
     """(o, lse fp32 [B, H, Nq]) of capk_sliding_attention_fwd; q [B, Nq, H, hd], k / v [B, Nk, Hk, hd]."""
     what = "sliding_attention_fwd"
-    code, dims, ws_args, views, key_pad, kv_len = _sliding_args(what, q, k, v, window, sinks, key_pad, kv_len)
+    args = _sliding_args(what, q, k, v, window, sinks, key_pad, kv_len)
     if out is None:
         out = q.new_empty(q.shape)
     else:
         _same(what, q, out)
         if out.shape != q.shape:
             raise ValueError(f"{what}: out {tuple(out.shape)} for q {tuple(q.shape)}")
-    lse = torch.empty(q.shape[0], q.shape[2], q.shape[1], dtype=torch.float32, device=q.device) if want_lse else None
-    wsb = _ws_bytes("capk_sliding_attention_fwd_workspace", code, *dims, *ws_args)
-    ws = _ws(wsb, q.device)
-    _launch(q.device, "capk_sliding_attention_fwd", code, *dims, float(scale), *ws_args, *views, _p(key_pad), _p(kv_len),
-            *_view4(what, out), _p(lse), _p(ws), wsb)
-    return out, lse
+    return _sliding_fwd_run(*args, q, float(scale), out, want_lse)
+
+
+def _sliding_bwd_run(sizes, rule, scale, q, k, v, o, do, lse, key_pad, kv_len):
+    """The backward's launch, of operands that have been checked; sizes (dtype, B, H, Hk, Nq, Nk, hd), rule (window, sinks)."""
+    what, dev = "sliding_attention_bwd", q.device
+    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+    wsb = _ws_bytes("capk_sliding_attention_bwd_workspace", *sizes[1:], *rule)
+    ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
+    _launch(dev, "capk_sliding_attention_bwd", *sizes, scale, *rule, *_view4(what, q), *_view4(what, k), *_view4(what, v),
+            _p(key_pad), _p(kv_len), *_view4(what, o), *_view4(what, do), lse.data_ptr(), *_view4(what, dq), *_view4(what, dk),
+            *_view4(what, dv), ws.data_ptr(), wsb)
+    return dq, dk, dv
 
 
 def sliding_attention_bwd(q, k, v, o, do, lse, window, sinks, scale, key_pad=None, kv_len=None):
     """(dq, dk, dv) of capk_sliding_attention_bwd from the forward's o and lse."""
     what = "sliding_attention_bwd"
-    code, dims, ws_args, views, key_pad, kv_len = _sliding_args(what, q, k, v, window, sinks, key_pad, kv_len)
+    code, dims, rule, _, key_pad, kv_len = _sliding_args(what, q, k, v, window, sinks, key_pad, kv_len)
     _same(what, q, o, do)
     _same(what, q, lse, dtype=False)
     if o.shape != q.shape or do.shape != q.shape or lse.dtype != torch.float32 or not lse.is_contiguous() or \
             tuple(lse.shape) != (q.shape[0], q.shape[2], q.shape[1]):
         raise ValueError(f"{what}: o, do like q and a contiguous fp32 lse [B, H, Nq]")
-    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
-    wsb = _ws_bytes("capk_sliding_attention_bwd_workspace", *dims, *ws_args)
-    ws = _ws(wsb, q.device)
-    _launch(q.device, "capk_sliding_attention_bwd", code, *dims, float(scale), *ws_args, *views, _p(key_pad), _p(kv_len),
-            *_view4(what, o), *_view4(what, do), _p(lse), *_view4(what, dq), *_view4(what, dk), *_view4(what, dv),
-            _p(ws), wsb)
-    return dq, dk, dv
+    return _sliding_bwd_run((code, *dims), rule, float(scale), q, k, v, o, do, lse, key_pad, kv_len)
 
 
 def _kv4_pages(what, codes, scales, table, B, dev):

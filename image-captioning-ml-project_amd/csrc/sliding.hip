@@ -35,9 +35,22 @@ struct SlideArgs {
   const int32_t* len;   // [B]
   float* lse;           // [B, H, Nq]
   float* delta;         // [B, H, Nq]
-  float* part;          // far-query partial sums of dK and dV
-  int sink_tiles, far_chunks, far_rows;
+  float* part;          // partial sums of dK and dV
+  int sink_tiles, far_chunks, far_rows, near_chunks;
 };
+
+constexpr int kSlideKeys = 128;  // keys of a dK / dV workgroup
+// Partial sums [B, Hk][part][dK, dV][128][hd]: tiles with sinks have far_chunks + near_chunks parts, the others
+// (more than one near chunk) near_chunks.
+__host__ __device__ __forceinline__ int slide_parts(const SlideArgs& a) {
+  const int tiles = (a.Nk + kSlideKeys - 1) / kSlideKeys;
+  if (a.near_chunks > 1) return a.sink_tiles * a.far_chunks + tiles * a.near_chunks;
+  return a.far_chunks ? a.sink_tiles * (a.far_chunks + 1) : 0;
+}
+// the first of a tile's parts; a tile without sinks has no far ones
+__device__ __forceinline__ int slide_part(const SlideArgs& a, int tile) {
+  return tile * a.near_chunks + min(tile, a.sink_tiles) * a.far_chunks;
+}
 
 __device__ __forceinline__ int slide_len(const SlideArgs& a, int b) {
   return a.len ? min(max(a.len[b], 0), a.Nk) : a.Nk;
@@ -50,8 +63,8 @@ __device__ __forceinline__ bool slide_sees(const SlideArgs& a, int p, int j) {
 // multiple of 8 a key head's tiles run on one XCD and share its L2 (with 4, on two).  Long items first.
 struct SlideBlock {
   int b, kvh, rest;
-  __device__ __forceinline__ explicit SlideBlock(const SlideArgs& a) {
-    const int i = blockIdx.x, n = a.B * a.Hk;
+  __device__ __forceinline__ explicit SlideBlock(const SlideArgs& a, int i) {
+    const int n = a.B * a.Hk;
     kvh = i % n % a.Hk;
     b = i % n / a.Hk;
     rest = i / n;
@@ -68,8 +81,8 @@ __device__ __forceinline__ void slide_frags(typename Mat<T>::V8 (&f)[HDP / 16], 
 #pragma unroll
   for (int s = 0; s < HDP / 16; ++s) f[s] = Mat<T>::from(ok && s * 16 + h * 8 < hd ? x[s] : tile_zero8<T>());
 }
-// The same with conditional loads (src is read only where ok): in slide_dkv, whose registers are all taken, the
-// unconditional form is allocated worse (306 us for 299 at 16384 tokens).
+// The same with conditional loads (src is read only where ok): in slide_dkv of bf16, whose registers are all taken,
+// the unconditional form is allocated worse (306 us for 299 at 16384 tokens).
 template <typename T, int HDP>
 __device__ __forceinline__ void slide_frags_if(typename Mat<T>::V8 (&f)[HDP / 16], const T* src, bool ok, int hd, int h) {
 #pragma unroll
@@ -203,7 +216,7 @@ __global__ __launch_bounds__(256 * GROUPS, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) 
   extern __shared__ __align__(16) char smem[];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6 & 3), hh = lane >> 5;
   const int grp = GROUPS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
-  const SlideBlock at(a);
+  const SlideBlock at(a, blockIdx.x);
   const int b = at.b, kvh = at.kvh, G = a.H / a.Hk, h = kvh * G + at.rest % G, len = slide_len(a, b), off = len - a.Nq;
   const int q0 = ((a.Nq + 127) / 128 - 1 - at.rest / G) * 128, qw = q0 + w * 32, qi = qw + (lane & 31), p = off + qi;
   const int qr = min(qi, a.Nq - 1);  // a row to load
@@ -329,7 +342,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) : HDP <= 
   constexpr int NS = HDP / 16, ND = HDP / 32;
   extern __shared__ __align__(16) char smem[];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hh = lane >> 5;
-  const SlideBlock at(a);
+  const SlideBlock at(a, blockIdx.x);
   const int b = at.b, kvh = at.kvh, G = a.H / a.Hk, h = kvh * G + at.rest % G, len = slide_len(a, b), off = len - a.Nq;
   const int q0 = ((a.Nq + 127) / 128 - 1 - at.rest / G) * 128, qw = q0 + w * 32, qi = qw + (lane & 31), p = off + qi;
   const int qr = min(qi, a.Nq - 1);  // a row to load
@@ -444,10 +457,23 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? (HDP <= 64 ? 2 : 1) : HDP <= 
   slide_store<T, HDP>(row<T>(a.dq, b, qi, h), dq, a.scale, a.hd, hh);
 }
 
-// Keys [j0, j0 + 128) of a key head against queries [qa, qb) of its group; far = only the sinks among
-// the keys, at queries that no longer have them in their window.
-constexpr int kSlideKeys = 128;
-template <typename T, int HDP>
+// The key tile and chunk of an item of dK / dV: near chunks of every tile first, then the far ones.
+struct SlideChunk : SlideBlock {
+  bool far;
+  int tile, chunk;
+  __device__ __forceinline__ SlideChunk(const SlideArgs& a, int i, int near_chunks) : SlideBlock(a, i) {
+    const int near = (a.Nk + kSlideKeys - 1) / kSlideKeys * near_chunks;
+    far = rest >= near;
+    const int at = far ? rest - near : rest, cut = far ? a.far_chunks : near_chunks;
+    tile = at / cut;
+    chunk = at % cut;
+  }
+};
+
+// Keys [j0, j0 + 128) of a key head against queries [qa, qb) of its group, a chunk of their tiles; far = only the
+// sinks among the keys, at queries that no longer have them in their window.  CUT: more than one near chunk (a form
+// of its own: with it the other would hold a few registers in memory, 307 us for 300 at 16384 tokens).
+template <typename T, int HDP, bool CUT>
 __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void slide_dkv(SlideArgs a) {
   using Pair = SlidePair<T, HDP>;
   using Img = typename Pair::Img;
@@ -455,20 +481,25 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void s
   extern __shared__ __align__(16) char smem[];
   float* Ls = (float*)(smem + Pair::LDS);  // per buffer: lse (base 2) and D of 64 queries
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hh = lane >> 5;
-  const SlideBlock at(a);
+  const int cuts = CUT ? a.near_chunks : 1;
+  const SlideChunk at(a, blockIdx.x, cuts);
   const int b = at.b, kvh = at.kvh, G = a.H / a.Hk, len = slide_len(a, b), off = len - a.Nq;
-  const int tiles = (a.Nk + kSlideKeys - 1) / kSlideKeys;
-  const bool far = at.rest >= tiles;
-  const int tile = far ? (at.rest - tiles) / a.far_chunks : at.rest;
-  const int chunk = far ? (at.rest - tiles) % a.far_chunks : a.far_chunks;
+  const bool far = at.far;
+  const int tile = at.tile, chunk = at.chunk;
   const int j0 = tile * kSlideKeys, jw = j0 + w * 32, j = jw + (lane & 31);
   const bool key_ok = j < len && !(a.pad && a.pad[(int64_t)b * a.Nk + j]) && (!far || j < a.sinks);
   // positions of the queries: near p in [j0, near_end), far p >= near_end in chunks of far_rows (no
   // chunks: the owner of a tile with sinks walks all of them)
   const int64_t near_end = tile < a.sink_tiles && a.far_chunks == 0 ? (int64_t)1 << 40 : (int64_t)j0 + kSlideKeys - 1 + a.window;
   const int qn = (int)min((int64_t)a.Nq, max((int64_t)0, near_end - off));
-  const int qa = far ? qn + chunk * a.far_rows : max(0, j0 - off);
-  const int qb = far ? min(a.Nq, qa + a.far_rows) : (j0 < len ? qn : 0);
+  int qa = far ? qn + chunk * a.far_rows : max(0, j0 - off);
+  int qb = far ? min(a.Nq, qa + a.far_rows) : (j0 < len ? qn : 0);
+  if (CUT && !far) {  // a share of the range's tiles of 64
+    const int64_t n = qb > qa ? (qb - qa + QT - 1) / QT : 0;
+    const int lo = (int)(n * chunk / cuts), hi = (int)(n * (chunk + 1) / cuts);
+    qb = min(qb, qa + hi * QT);
+    qa += lo * QT;
+  }
   const float c = a.scale * kTileLog2e;
   typename Img::Lane ln(lane);
   const int nq = qb > qa ? (qb - qa + QT - 1) / QT : 0, all = nq * G;
@@ -484,10 +515,16 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void s
     qd.y = row<T>(a.dout, b, 0, h);
     qd.fetch(q0, qb - 1, buf);
   };
-  if (all) fetch(0, 0);
+  if (all > 0) fetch(0, 0);
   typename Mat<T>::V8 kf[NS], vf[NS];
-  slide_frags_if<T, HDP>(kf, row<T>(a.k, b, j, kvh), key_ok, a.hd, hh);
-  slide_frags_if<T, HDP>(vf, row<T>(a.v, b, j, kvh), key_ok, a.hd, hh);
+  if constexpr (sizeof(T) == 4) {
+    const int jr = min(j, a.Nk - 1);
+    slide_frags<T, HDP>(kf, row<T>(a.k, b, jr, kvh), key_ok, a.hd, hh);
+    slide_frags<T, HDP>(vf, row<T>(a.v, b, jr, kvh), key_ok, a.hd, hh);
+  } else {
+    slide_frags_if<T, HDP>(kf, row<T>(a.k, b, j, kvh), key_ok, a.hd, hh);
+    slide_frags_if<T, HDP>(vf, row<T>(a.v, b, j, kvh), key_ok, a.hd, hh);
+  }
   const bool hidden = __builtin_amdgcn_ballot_w64(!key_ok) != 0;
   f32x16 dk[ND], dv[ND];
 #pragma unroll
@@ -551,31 +588,38 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : HDP <= 64 ? 3 : 2) void s
                             });
     }
   }
-  if (far && j >= a.sinks) return;
-  if (tile < a.sink_tiles && a.far_chunks > 0) {  // [B, Hk, sink tile, chunk][dK, dV][128][hd]
-    float* dst = a.part + ((((int64_t)b * a.Hk + kvh) * a.sink_tiles + tile) * (a.far_chunks + 1) + chunk) * 2 *
-                              kSlideKeys * a.hd + (int64_t)(w * 32 + (lane & 31)) * a.hd;
+  SlideChunk to = at;
+  if constexpr (CUT) {  // (found again: the loop has no registers to keep it)
+    int item = blockIdx.x;
+    asm volatile("" : "+s"(item));
+    to = SlideChunk(a, item, cuts);
+  }
+  if (to.far && j >= a.sinks) return;
+  if (CUT || (to.tile < a.sink_tiles && a.far_chunks > 0)) {
+    const int part = slide_part(a, to.tile) + (to.far || to.tile >= a.sink_tiles ? to.chunk : a.far_chunks + to.chunk);
+    float* dst = a.part + (((int64_t)to.b * a.Hk + to.kvh) * slide_parts(a) + part) * 2 * kSlideKeys * a.hd +
+                 (int64_t)(w * 32 + (lane & 31)) * a.hd;
     slide_store<float, HDP>(dst, dk, a.scale, a.hd, hh);
     slide_store<float, HDP>(dst + (int64_t)kSlideKeys * a.hd, dv, 1.f, a.hd, hh);
   } else if (j < a.Nk) {
-    slide_store<T, HDP>(row<T>(a.dk, b, j, kvh), dk, a.scale, a.hd, hh);
-    slide_store<T, HDP>(row<T>(a.dv, b, j, kvh), dv, 1.f, a.hd, hh);
+    slide_store<T, HDP>(row<T>(a.dk, to.b, j, to.kvh), dk, a.scale, a.hd, hh);
+    slide_store<T, HDP>(row<T>(a.dv, to.b, j, to.kvh), dv, 1.f, a.hd, hh);
   }
 }
 
-// dK, dV rows of the sink tiles = the sum of their chunks, in order.  One thread per 4 elements.
+// dK, dV rows of the tiles with partial sums = their sum, in order.  One thread per 4 elements.
 template <typename T>
 __global__ __launch_bounds__(256) void slide_dkv_sum(SlideArgs a) {
   const int per = kSlideKeys * a.hd / 4;
   const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= per * 2 * a.sink_tiles) return;
   const int e = i % per * 4, which = i / per % 2, tile = i / per / 2, j = tile * kSlideKeys + e / a.hd;
-  if (j >= a.Nk) return;
-  const float* src = a.part + (((int64_t)blockIdx.z * a.Hk + blockIdx.y) * a.sink_tiles + tile) * (a.far_chunks + 1) * 2 *
+  if (j >= a.Nk || (a.near_chunks == 1 && tile >= a.sink_tiles)) return;
+  const int far = tile < a.sink_tiles ? a.far_chunks : 0;
+  const float* src = a.part + (((int64_t)blockIdx.z * a.Hk + blockIdx.y) * slide_parts(a) + slide_part(a, tile)) * 2 *
                                   kSlideKeys * a.hd + (int64_t)which * kSlideKeys * a.hd + e;
   f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-  for (int c = j < a.sinks ? 0 : a.far_chunks; c <= a.far_chunks; ++c) s += *(const f32x4*)(src + (int64_t)c * 2 * kSlideKeys * a.hd);
+  for (int c = j < a.sinks ? 0 : far; c < far + a.near_chunks; ++c) s += *(const f32x4*)(src + (int64_t)c * 2 * kSlideKeys * a.hd);
   Tile<T>::store4(row<T>(which ? a.dv : a.dk, blockIdx.z, j, blockIdx.y) + e % a.hd, s);
 }
 
@@ -620,22 +664,38 @@ static SlideArgs slide_args(int B, int H, int Hk, int Nq, int Nk, int hd, float 
   return a;
 }
 
-// The far queries of the sink tiles.  An item's length is its 64-query tiles; the launch runs about
-// `slots` workgroups at a time.  Where even the longest item (a sink tile with every query) is within
-// a slot's share of the whole, each sink tile has one owner; else its far queries go in chunks of a
-// quarter of that share (at least 256 queries), so the partial sums stay below 2^29 bytes.
-static void slide_far(SlideArgs& a) {
-  const int64_t slots = 512, G = a.H / a.Hk;
+// How the queries of the key tiles are cut.  An item's length is its 64-query tiles over all heads of the group.
+// Near queries: where the tiles alone leave CUs without a workgroup (fewer than 256), each tile's range goes in chunks
+// whose length is a CU's share of the whole (at least two).  Measured, dK and dV with their sum: 80 to 34 us (one
+// sequence of 2956, 2 key heads of 64, window 489), 586 to 207 (4096, 4 of 128, no window), 60 to 20 (2 x 500, 2 of
+// 64), fp32 78 to 50 (3 x 777, 3 of 80, window 100).  Far queries of the sink tiles: on such small grids in chunks of that length too; else the launch runs about
+// `slots` workgroups at a time, and where even the longest item (a sink tile with every query) is within a slot's
+// share of the whole, each sink tile has one owner; else its far queries go in chunks of a quarter of that share (at
+// least 256 queries), so the partial sums stay below 2^29 bytes.
+static void slide_cut(SlideArgs& a) {
+  const int64_t slots = 512, G = a.H / a.Hk, heads = a.B * (int64_t)a.Hk, tiles = cdiv(a.Nk, kSlideKeys);
   a.sink_tiles = cdiv(a.sinks, kSlideKeys);
+  a.far_rows = a.far_chunks = 0;
+  a.near_chunks = 1;
   // the first sink tile has the most far queries: positions from 127 + window on
   const int64_t most = (int64_t)a.Nk - (kSlideKeys - 1) - a.window, rows = most < a.Nq ? most : a.Nq;
-  a.far_rows = a.far_chunks = 0;
-  if (!a.sink_tiles || rows <= 0) return;
-  const int64_t near = cdiv(a.window + kSlideKeys < a.Nq ? a.window + kSlideKeys : a.Nq, 64) * G, far = cdiv(rows, 64) * G;
-  const int64_t share = a.B * (int64_t)a.Hk * (cdiv(a.Nk, kSlideKeys) * near + a.sink_tiles * far) / slots;
-  if (near + far <= share) return;
-  int64_t n = share / 4 / G * 64;
-  if (n < 256) n = 256;
+  const bool whole = a.window + kSlideKeys >= a.Nq;  // no window to speak of: later tiles have fewer queries
+  const int64_t walk = cdiv(whole ? a.Nq : a.window + kSlideKeys, 64), near = walk * G;
+  const int64_t far = a.sink_tiles && rows > 0 ? cdiv(rows, 64) * G : 0;
+  int64_t n;
+  if (heads * tiles < 256) {
+    int64_t share = heads * (tiles * (whole ? near / 2 + 1 : near) + a.sink_tiles * far) / 256 + 1;
+    if (share < 2) share = 2;
+    const int64_t cut = cdiv(near, share);
+    a.near_chunks = (int)(cut < walk ? cut : walk);
+    n = cdiv(share, G) * 64;
+  } else {
+    const int64_t share = heads * (tiles * near + a.sink_tiles * far) / slots;
+    if (near + far <= share) return;
+    n = share / 4 / G * 64;
+    if (n < 256) n = 256;
+  }
+  if (!far) return;
   a.far_rows = (int)n;
   a.far_chunks = cdiv(rows, n);
 }
@@ -694,9 +754,9 @@ extern "C" size_t capk_sliding_attention_bwd_workspace(int B, int H, int Hk, int
                                                        int sinks) {
   if (B < 1 || H < 1 || Hk < 1 || Nq < 1 || Nk < 1 || hd < 1 || window < 0 || sinks < 0) return 0;
   SlideArgs a = slide_args(B, H, Hk, Nq, Nk, hd, 0.f, window, sinks, nullptr, nullptr);
-  slide_far(a);
+  slide_cut(a);
   const size_t delta = ((size_t)B * H * Nq * 4 + 15) / 16 * 16;
-  return delta + (a.far_chunks ? (size_t)B * Hk * a.sink_tiles * (a.far_chunks + 1) * 2 * kSlideKeys * hd * 4 : 0);
+  return delta + (size_t)B * Hk * slide_parts(a) * 2 * kSlideKeys * hd * 4;
 }
 
 extern "C" int capk_sliding_attention_bwd(int dtype, int B, int H, int Hk, int Nq, int Nk, int hd, float scale,
@@ -718,27 +778,32 @@ extern "C" int capk_sliding_attention_bwd(int dtype, int B, int H, int Hk, int N
   CAPK_CHECK_ARG(lse && ws && ws_bytes >= need && (uintptr_t)ws % 16 == 0,
                  "capk_sliding_attention_bwd: need lse and a 16-B aligned workspace of %zu bytes", need);
   SlideArgs a = slide_args(B, H, Hk, Nq, Nk, hd, scale, window, sinks, key_pad, kv_len);
-  slide_far(a);
+  slide_cut(a);
   a.q = vs[0]; a.k = vs[1]; a.v = vs[2]; a.o = vs[3]; a.dout = vs[4]; a.dq = vs[5]; a.dk = vs[6]; a.dv = vs[7];
   a.lse = (float*)lse;
   a.delta = (float*)ws;
   a.part = (float*)((char*)ws + ((size_t)B * H * Nq * 4 + 15) / 16 * 16);
   const int hdp = slide_hdp(hd), es = dtype == CAPK_BF16 ? 2 : 4;
-  const dim3 gq(cdiv(Nq, 128) * H * B), gk((cdiv(Nk, kSlideKeys) + a.sink_tiles * a.far_chunks) * Hk * B);
+  const dim3 gq(cdiv(Nq, 128) * H * B), gk((cdiv(Nk, kSlideKeys) * a.near_chunks + a.sink_tiles * a.far_chunks) * Hk * B);
   hipStream_t st = S(stream);
+  const bool cut = a.near_chunks > 1;
   SLIDE_HD(hdp, {
     if (dtype == CAPK_BF16) {
       const size_t shm = SlidePair<bf16, HDP>::LDS;
       if ((rc = slide_launch(slide_dq<bf16, HDP>, gq, shm, st, a, "slide_dq"))) return rc;
-      if ((rc = slide_launch(slide_dkv<bf16, HDP>, gk, shm + 1024, st, a, "slide_dkv"))) return rc;
+      rc = cut ? slide_launch(slide_dkv<bf16, HDP, true>, gk, shm + 1024, st, a, "slide_dkv")
+               : slide_launch(slide_dkv<bf16, HDP, false>, gk, shm + 1024, st, a, "slide_dkv");
     } else {
       const size_t shm = SlidePair<float, HDP>::LDS;
       if ((rc = slide_launch(slide_dq<float, HDP>, gq, shm, st, a, "slide_dq"))) return rc;
-      if ((rc = slide_launch(slide_dkv<float, HDP>, gk, shm + 1024, st, a, "slide_dkv"))) return rc;
+      rc = cut ? slide_launch(slide_dkv<float, HDP, true>, gk, shm + 1024, st, a, "slide_dkv")
+               : slide_launch(slide_dkv<float, HDP, false>, gk, shm + 1024, st, a, "slide_dkv");
     }
+    if (rc) return rc;
   });
-  if (a.far_chunks) {
-    const dim3 gs(cdiv((int64_t)kSlideKeys * hd / 4 * 2 * a.sink_tiles, 256), Hk, B);
+  if (slide_parts(a)) {
+    const int64_t n = a.near_chunks > 1 ? cdiv(Nk, kSlideKeys) : a.sink_tiles;
+    const dim3 gs(cdiv((int64_t)kSlideKeys * hd / 4 * 2 * n, 256), Hk, B);
     if (es == 2) return slide_launch(slide_dkv_sum<bf16>, gs, 0, st, a, "slide_dkv_sum");
     return slide_launch(slide_dkv_sum<float>, gs, 0, st, a, "slide_dkv_sum");
   }

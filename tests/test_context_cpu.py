@@ -41,10 +41,12 @@ def test_sliding_attention_refusals():
     assert _fwd(L, Nq=1, Nk=100000, window=0, sinks=0) == EINVAL  # a step without its workspace
     assert _fwd(L, Nq=1, Nk=100000, window=0, sinks=0, ws=P, wsb=need - 1) == EINVAL
     assert L.capk_sliding_attention_fwd_workspace(1, 1, 4, 2, 1000, 100000, 64, 0, 0) == 0
-    # the backward's workspace covers the far queries of the keys that stay visible
-    small = L.capk_sliding_attention_bwd_workspace(1, 4, 2, 5000, 5000, 64, 100, 0)
-    assert small == 4 * 5000 * 4
-    assert L.capk_sliding_attention_bwd_workspace(1, 4, 2, 5000, 5000, 64, 100, 4) > small
+    # the backward's workspace covers the far queries of the keys that stay visible, and on small grids the chunks
+    # of the near ones
+    small = L.capk_sliding_attention_bwd_workspace(8, 8, 8, 5000, 5000, 64, 100, 0)
+    assert small == 64 * 5000 * 4
+    assert L.capk_sliding_attention_bwd_workspace(8, 8, 8, 5000, 5000, 64, 100, 4) > small
+    assert L.capk_sliding_attention_bwd_workspace(1, 4, 2, 5000, 5000, 64, 100, 0) > 4 * 5000 * 4
 
 
 def test_kv4_and_verify_refusals():

@@ -825,3 +825,19 @@ def test_calls_on_two_streams_and_graphs_that_take_turns():
     torch.cuda.synchronize()
     for o, a in zip(outs, alone):
         assert all(torch.equal(x, y) for x, y in zip(o, a))
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("B,N,H,Hk,hd,window,sinks", [
+    (22, 400, 4, 4, 32, 40, 5), (33, 300, 8, 4, 64, 30, 140), (65, 257, 2, 2, 96, 0, 0), (1, 1400, 4, 1, 128, 70, 9),
+    (1, 1400, 4, 1, 64, 0, 0), (2, 1000, 6, 1, 32, 5, 300)])
+def test_sliding_attention_large_and_small_grids(dtype, B, N, H, Hk, hd, window, sinks):
+    """Enough key tiles for every compute unit, and so few that their queries are cut into chunks."""
+    _slide_case(dtype, B, N, N, H, Hk, hd, window, sinks)
+
+
+@pytest.mark.parametrize("B,window,sinks", [(30, 60, 3), (30, 0, 0), (4, 60, 150)])
+def test_sliding_attention_grids_of_ragged_sequences(B, window, sinks):
+    pad, kv_len = (tuple((1 + k * i) % 301 for i in range(B)) for k in (37, 113))
+    _slide_case("bf16", B, 200, 300, 8, 4, 64, window, sinks, pad, None, seed=5)
+    _slide_case("bf16", B, 200, 300, 8, 4, 64, window, sinks, None, kv_len, seed=6)

@@ -841,3 +841,19 @@ def test_sliding_attention_grids_of_ragged_sequences(B, window, sinks):
     pad, kv_len = (tuple((1 + k * i) % 301 for i in range(B)) for k in (37, 113))
     _slide_case("bf16", B, 200, 300, 8, 4, 64, window, sinks, pad, None, seed=5)
     _slide_case("bf16", B, 200, 300, 8, 4, 64, window, sinks, None, kv_len, seed=6)
+
+
+def test_axis_rope_gradient_of_one_output():
+    """Only q', only k', neither, and expanded gradients."""
+    from capk import context
+    freq, axis = context.axis_frequencies((8, 12, 12))
+    pos = torch.randint(0, 5000, (3, 2, 9), device="cuda")
+    q, k = (_rand(2, 9, h, 64, seed=261 + h).requires_grad_() for h in (4, 2))
+    gq, gk = _rand(2, 9, 1, 64, seed=265).expand(2, 9, 4, 64), _rand(2, 9, 2, 64, seed=266)
+    both = torch.autograd.grad(context.axis_rope(q, k, pos, freq, axis), (q, k), (gq, gk))
+    dq, = torch.autograd.grad(context.axis_rope(q, k, pos, freq, axis)[0], q, gq)
+    dk, none = torch.autograd.grad(context.axis_rope(q, k, pos, freq, axis)[1], (k, q), gk, allow_unused=True)
+    alone, = torch.autograd.grad(context.axis_rope(q, None, pos, freq, axis)[0], q, gq)
+    assert torch.equal(both[0], dq) and torch.equal(both[1], dk) and none is None and torch.equal(alone, dq)
+    back, _ = _rope_ref(gq, pos, freq, axis, False, -1.0)
+    _close(dq, back, gq.double().abs().amax(-1, keepdim=True).expand_as(back) * 2.0 ** -19 + 2.0 ** -24 * back.abs())

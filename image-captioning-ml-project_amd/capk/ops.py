@@ -1373,6 +1373,8 @@ def _sliding_args(what, q, k, v, window, sinks, key_pad, kv_len):
     kB, Nk, Hk, khd = k.shape
     if kB != B or khd != hd or v.shape != k.shape:
         raise ValueError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+    if Hk < 1 or H < Hk or H % Hk:
+        raise ValueError(f"{what}: {H} query heads over {Hk} key heads")
     if key_pad is not None:
         if key_pad.dtype not in (torch.bool, torch.uint8) and not key_pad.dtype.is_floating_point:
             key_pad = key_pad != 0

@@ -159,6 +159,8 @@ extern "C" int capk_kv4_read(int dtype, int B, int n, int Hk, int hd, const void
   return CAPK_OK;
 }
 
+constexpr int kKv4Heads = 1 << 20;  // query heads: 65535 workgroups of 16 columns (head, query) at most
+
 static StepArgs kv4_step(int B, int H, int Hk, int Nq, int hd, float scale, int window, int sinks, int pages, int page,
                          int table_cols) {
   StepArgs a{};
@@ -172,7 +174,10 @@ static StepArgs kv4_step(int B, int H, int Hk, int Nq, int hd, float scale, int 
 
 extern "C" size_t capk_kv4_attention_workspace(int dtype, int B, int H, int Hk, int Nq, int hd, int window, int sinks,
                                                int page, int table_cols) {
-  if (B < 1 || Hk < 1 || H < Hk || Nq < 1 || hd < 1 || window < 0 || sinks < 0 || page < 1 || table_cols < 1) return 0;
+  // (sizes that the entry refuses have no workspace)
+  if (B < 1 || B > 65535 || Hk < 1 || H < Hk || H > kKv4Heads || H % Hk || Nq < 1 || Nq > 64 || hd < 1 || hd > 128 ||
+      window < 0 || sinks < 0 || page < 1 || table_cols < 1 || (int64_t)table_cols * page > (1 << 28))
+    return 0;
   int splits;
   return step_workspace(dtype, kv4_step(B, H, Hk, Nq, hd, 0.f, window, sinks, 1, page, table_cols), &splits);
 }
@@ -186,7 +191,7 @@ extern "C" int capk_kv4_attention(int dtype, int B, int H, int Hk, int Nq, int h
   int rc = kv4_check("capk_kv4_attention", dtype, B, Nq, Hk, hd, qv, ov, codes, scales, pages, page, table, table_ld, table_cols);
   if (rc) return rc;
   if (B == 0) return CAPK_OK;
-  CAPK_CHECK_ARG(H >= Hk && H % Hk == 0, "capk_kv4_attention: %d query heads over %d key heads", H, Hk);
+  CAPK_CHECK_ARG(H >= Hk && H <= kKv4Heads && H % Hk == 0, "capk_kv4_attention: %d query heads over %d key heads", H, Hk);
   CAPK_CHECK_ARG(Nq >= 1 && Nq <= 64, "capk_kv4_attention: Nq=%d must be 1..64", Nq);
   CAPK_CHECK_ARG(B <= 65535 && Hk * (int64_t)cdiv((int64_t)Nq * (H / Hk), 16) <= 65535, "capk_kv4_attention: too many heads or sequences");
   CAPK_CHECK_ARG(window >= 0 && sinks >= 0, "capk_kv4_attention: window and sinks must not be negative");

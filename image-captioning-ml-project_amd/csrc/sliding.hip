@@ -635,6 +635,12 @@ static int slide_launch(K kernel, dim3 grid, size_t shm, hipStream_t st, const S
   return CAPK_OK;
 }
 
+// sizes that a workspace query may compute with (the entries refuse the others, with a message)
+static bool slide_sizes(int B, int H, int Hk, int Nq, int Nk, int hd, int window, int sinks) {
+  return B >= 1 && B <= 65535 && Hk >= 1 && H >= Hk && H <= 65535 && H % Hk == 0 && Nq >= 1 && Nq <= (1 << 28) && Nk >= 1 && Nk <= (1 << 28) &&
+         hd >= 1 && hd <= 128 && window >= 0 && sinks >= 0;
+}
+
 static int slide_check(const char* who, int dtype, int B, int H, int Hk, int Nq, int Nk, int hd, int window, int sinks,
                        float scale, const SlideView* v, int n) {
   CAPK_CHECK_ARG(dtype == CAPK_F32 || dtype == CAPK_BF16, "%s: dtype", who);
@@ -716,7 +722,7 @@ static StepArgs slide_step(const SlideArgs& a) {
 
 extern "C" size_t capk_sliding_attention_fwd_workspace(int dtype, int B, int H, int Hk, int Nq, int Nk, int hd,
                                                        int window, int sinks) {
-  if (B < 1 || Hk < 1 || H < Hk || Nq < 1 || Nk < 1 || hd < 1 || window < 0 || sinks < 0 || !slide_few(Nq)) return 0;
+  if (!slide_sizes(B, H, Hk, Nq, Nk, hd, window, sinks) || !slide_few(Nq)) return 0;
   int splits;
   return step_workspace(dtype, slide_step(slide_args(B, H, Hk, Nq, Nk, hd, 0.f, window, sinks, nullptr, nullptr)), &splits);
 }
@@ -752,7 +758,7 @@ extern "C" int capk_sliding_attention_fwd(int dtype, int B, int H, int Hk, int N
 
 extern "C" size_t capk_sliding_attention_bwd_workspace(int B, int H, int Hk, int Nq, int Nk, int hd, int window,
                                                        int sinks) {
-  if (B < 1 || H < 1 || Hk < 1 || Nq < 1 || Nk < 1 || hd < 1 || window < 0 || sinks < 0) return 0;
+  if (!slide_sizes(B, H, Hk, Nq, Nk, hd, window, sinks)) return 0;
   SlideArgs a = slide_args(B, H, Hk, Nq, Nk, hd, 0.f, window, sinks, nullptr, nullptr);
   slide_cut(a);
   const size_t delta = ((size_t)B * H * Nq * 4 + 15) / 16 * 16;

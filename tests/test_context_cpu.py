@@ -130,3 +130,20 @@ def test_backward_workspace_stays_small():
                 for B in (1, 4):
                     size = L.capk_sliding_attention_bwd_workspace(B, Hk * G, Hk, N, N, hd, window, sinks)
                     assert size <= B * Hk * G * N * 4 + (1 << 29), (N, Hk, G, hd, window, sinks, B)
+
+
+def test_workspace_queries_of_refused_sizes():
+    """A size that the entry refuses has a workspace of 0 bytes: the query neither divides by a group of no heads nor
+    overflows."""
+    L = _lib()
+    for B, H, Hk, Nq, Nk, hd in ((1, 1, 2, 20, 20, 64), (1, 3, 2, 20, 20, 64), (1, 0, 1, 20, 20, 64), (1, 1, 0, 20, 20, 64),
+                                 (0, 1, 1, 20, 20, 64), (1, 1 << 28, 1, 16, 20, 64), (1, 1, 1, 2, (1 << 31) - 1, 64), (1, 1, 1, 20, 20, 0)):
+        assert L.capk_sliding_attention_bwd_workspace(B, H, Hk, Nq, Nk, hd, 8, 2) == 0, (B, H, Hk, Nq, Nk, hd)
+        assert L.capk_sliding_attention_fwd_workspace(1, B, H, Hk, min(Nq, 16), Nk, hd, 8, 2) == 0, (B, H, Hk, Nq, Nk, hd)
+    for kw in (dict(H=1), dict(H=3), dict(H=1 << 27, Hk=1), dict(Nq=0), dict(Nq=65), dict(page=4096, cols=1 << 20), dict(cols=0), dict(B=0)):
+        a = dict(dict(B=1, H=2, Hk=2, Nq=64, page=64, cols=1000), **kw)
+        assert L.capk_kv4_attention_workspace(1, a["B"], a["H"], a["Hk"], a["Nq"], 64, 0, 0, a["page"], a["cols"]) == 0, kw
+    assert L.capk_kv4_attention_workspace(1, 1, 2, 2, 64, 64, 0, 0, 64, 1000) > 0
+    # (the same overflow in the entry itself)
+    assert L.capk_kv4_attention(1, 1, 1 << 30, 1, 64, 64, 1.0, 0, 0, P, 0, 256, 64, P, P, 8, 64, P, 4, 4, P, P, 0, 256, 64, None, P,
+                                1 << 30, None) == EINVAL

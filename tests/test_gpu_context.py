@@ -857,3 +857,18 @@ def test_axis_rope_gradient_of_one_output():
     assert torch.equal(both[0], dq) and torch.equal(both[1], dk) and none is None and torch.equal(alone, dq)
     back, _ = _rope_ref(gq, pos, freq, axis, False, -1.0)
     _close(dq, back, gq.double().abs().amax(-1, keepdim=True).expand_as(back) * 2.0 ** -19 + 2.0 ** -24 * back.abs())
+
+
+def test_fewer_query_heads_than_key_heads_are_refused():
+    """In the forward, in the backward (whose workspace is asked for before its entry checks the sizes) and over the
+    4-bit cache."""
+    from capk import context, ops
+    from capk._lib import CapkError
+    q, lse = _rand(1, 20, 1, 64, seed=271), torch.zeros(1, 1, 20, device="cuda")
+    for Hk in (2, 3):
+        k = _rand(1, 20, Hk, 64, seed=272)
+        cache, table = context.KV4Cache.empty(2, Hk, 64, 16), torch.zeros(1, 2, dtype=torch.int32, device="cuda")
+        for call in (lambda: ops.sliding_attention_bwd(q, k, k, q, q, lse, 8, 2, 1.0), lambda: ops.sliding_attention_fwd(q, k, k, 8, 2, 1.0),
+                     lambda: context.sliding_attention(q, k, k, window=8, sinks=2), lambda: cache.attend(q, table, table[:, 0] + 20)):
+            with pytest.raises((CapkError, ValueError)):
+                call()

@@ -107,7 +107,7 @@ static int kv4_check(const char* who, int dtype, int B, int n, int Hk, int hd, c
   CAPK_CHECK_ARG(hd == 32 || hd == 64 || hd == 96 || hd == 128, "%s: hd=%d must be 32, 64, 96 or 128", who, hd);
   CAPK_CHECK_ARG(page >= 16 && page % 16 == 0 && page <= 4096, "%s: page=%d must be a multiple of 16, <= 4096", who, page);
   CAPK_CHECK_ARG(pages >= 1 && codes && scales && (uintptr_t)codes % 16 == 0, "%s: pages must be 16-B aligned", who);
-  CAPK_CHECK_ARG(table && table_cols >= 1 && table_ld >= table_cols && (int64_t)table_cols * page <= (1 << 28),
+  CAPK_CHECK_ARG((table || B == 0 || n == 0) && table_cols >= 1 && table_ld >= table_cols && (int64_t)table_cols * page <= (1 << 28),
                  "%s: page table of %d columns (at most 2^28 tokens)", who, table_cols);
   const int ea = dtype == CAPK_BF16 ? 8 : 4;
   for (const SlideView* x : {&k, &v})

@@ -147,3 +147,16 @@ def test_workspace_queries_of_refused_sizes():
     # (the same overflow in the entry itself)
     assert L.capk_kv4_attention(1, 1, 1 << 30, 1, 64, 64, 1.0, 0, 0, P, 0, 256, 64, P, P, 8, 64, P, 4, 4, P, P, 0, 256, 64, None, P,
                                 1 << 30, None) == EINVAL
+
+
+def test_kv4_empty_batches():
+    """A batch of no sequences, whose tensors have no memory, is nothing to do."""
+    L = _lib()
+    assert L.capk_kv4_append(1, 0, 4, 2, 64, None, 0, 128, 64, None, 0, 128, 64, P, P, 8, 16, None, 4, 4, None, None, None) == OK
+    assert L.capk_kv4_read(1, 0, 4, 2, 64, P, P, 8, 16, None, 4, 4, None, None, 0, 128, 64, None, 0, 128, 64, None) == OK
+    assert L.capk_kv4_attention(1, 0, 4, 2, 1, 64, 1.0, 0, 0, None, 0, 256, 64, P, P, 8, 64, None, 4, 4, None, None, 0, 256, 64,
+                                None, None, 0, None) == OK
+    # with sequences the table is needed
+    assert L.capk_kv4_append(1, 1, 4, 2, 64, P, 0, 128, 64, P, 0, 128, 64, P, P, 8, 16, None, 4, 4, P, None, None) == EINVAL
+    assert L.capk_kv4_attention(1, 1, 4, 2, 1, 64, 1.0, 0, 0, P, 0, 256, 64, P, P, 8, 64, None, 4, 4, P, P, 0, 256, 64, None, P,
+                                1 << 30, None) == EINVAL

@@ -872,3 +872,20 @@ def test_fewer_query_heads_than_key_heads_are_refused():
                      lambda: context.sliding_attention(q, k, k, window=8, sinks=2), lambda: cache.attend(q, table, table[:, 0] + 20)):
             with pytest.raises((CapkError, ValueError)):
                 call()
+
+
+@pytest.mark.parametrize("dtype", DT)
+def test_kv4_empty_batches(dtype):
+    """No sequences, or no tokens: append, read and attend leave the pages alone and give empty results."""
+    from capk import context
+    cache, dt = context.KV4Cache.empty(3, 2, 64, 16), DT[dtype]
+    before = cache.codes.clone()
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    x, table = _rand(0, 5, 2, 64, dtype=dt), torch.zeros(0, 2, dtype=torch.int32, device="cuda")
+    cache.append(x, x, table, none, none)
+    k, v = cache.read(table, none, 5, dt)
+    assert k.shape == v.shape == (0, 5, 2, 64) and k.dtype == dt
+    assert cache.attend(_rand(0, 1, 4, 64, dtype=dt), table, none).shape == (0, 1, 4, 64)
+    x, table, zero = _rand(1, 0, 2, 64, dtype=dt), torch.zeros(1, 2, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    cache.append(x, x, table, zero)
+    assert cache.read(table, zero, 0, dt)[0].shape == (1, 0, 2, 64) and torch.equal(cache.codes, before)

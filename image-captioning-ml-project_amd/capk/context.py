@@ -8,13 +8,17 @@
     o = cache.attend(q, table, kv_len, window=1024, sinks=4)
     accepted, tokens = verify_drafts(target, ids, u, draft)
 
-The tensor-level wrappers are capk.ops.axis_rope, sliding_attention_fwd / _bwd, kv4_* and verify_drafts;
+axis_rope and sliding_attention have backward passes (once) and no forward-mode derivatives; what the cache holds
+and what the verification returns has none: KV4Cache.attend refuses queries that require a gradient, append stores
+its tensors' values alone.  The tensor-level wrappers, which know nothing of gradients, are capk.ops.axis_rope, sliding_attention_fwd / _bwd, kv4_* and verify_drafts;
 layouts and rules are those of include/capk.h.
 """
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import ops
+from ._lib import CapkError
 from .ops import verify_drafts  # noqa: F401
 
 
@@ -42,6 +46,14 @@ def _rows(t):
 
 def _unit(t):
     return t if t is None or t.dim() != 4 or t.stride(3) == 1 else t.contiguous()
+
+
+def _differentiable(what, *ts):
+    """Whether a call on `ts` needs a graph.  A forward-mode dual tensor requires no gradient and would lose its
+    tangent without a word, so it is refused."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise CapkError(f"{what} has no forward-mode derivatives")
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
 
 # (The backward passes run in the engine's thread, on a cold core: what can be checked, converted and looked up is,
@@ -74,7 +86,7 @@ class _AxisRope(torch.autograd.Function):
 
 def axis_rope(q, k, pos, freq, axis, *, interleaved=False):
     """(q', k') turned by their positions (ops.axis_rope); k may be None.  Differentiable in q and k."""
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+    if _differentiable("axis_rope", q, k):
         return _AxisRope.apply(q, k, pos, freq, axis, interleaved)
     return ops.axis_rope(_unit(q), _unit(k), pos, freq, axis, interleaved=interleaved)
 
@@ -103,11 +115,12 @@ def sliding_attention(q, k, v, *, window=0, sinks=0, scale=None, key_pad=None, k
     j <= p with j < sinks or p - j < window (0: no window), less key_pad[b, j].  k / v [B, Nk, Hk, hd] with
     H % Hk == 0; scale defaults to hd ** -0.5.  Differentiable in q, k and v."""
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    track = _differentiable("sliding_attention", q, k, v)
     if q.dim() == 4 and k.dim() == 4 and not (q.numel() and k.numel()):  # nothing to attend, or to
         if q.dtype != k.dtype or q.dtype != v.dtype or k.shape != v.shape or q.shape[0] != k.shape[0]:
             raise ValueError(f"sliding_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
         return q.masked_fill(torch.ones_like(q, dtype=torch.bool), 0)  # (zeros, of q's graph)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if track:
         return _SlidingAttention.apply(q, k, v, window, sinks, scale, key_pad, kv_len)
     return ops.sliding_attention_fwd(_rows(q), _rows(k), _rows(v), window, sinks, scale, key_pad, kv_len,
                                      want_lse=False)[0]
@@ -131,7 +144,8 @@ class KV4Cache:
                    torch.full((pages, 2, heads, page, head_dim // 32), 127, dtype=torch.uint8, device=device))
 
     def append(self, k, v, table, start, count=None):
-        """k, v [B, n, heads, hd] become tokens start[b] + i (i < count[b]); tokens without a page are dropped."""
+        """The values of k, v [B, n, heads, hd] become tokens start[b] + i (i < count[b]); tokens without a page are
+        dropped."""
         ops.kv4_append(_rows(k), _rows(v), self.codes, self.scales, table, start, count)
 
     def read(self, table, start, n, dtype=torch.bfloat16):
@@ -139,6 +153,9 @@ class KV4Cache:
         return ops.kv4_read(self.codes, self.scales, table, start, n, dtype)
 
     def attend(self, q, table, kv_len, *, window=0, sinks=0, scale=None):
-        """o [B, Nq, H, hd] of the last Nq <= 64 tokens of kv_len[b], visible as in sliding_attention."""
+        """o [B, Nq, H, hd] of the last Nq <= 64 tokens of kv_len[b], visible as in sliding_attention.  For decoding:
+        a q that requires a gradient is refused (detach it, or call under torch.no_grad())."""
+        if _differentiable("KV4Cache.attend", q):
+            raise CapkError("KV4Cache.attend has no gradient: detach q, or call it under torch.no_grad()")
         scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
         return ops.kv4_attention(_rows(q), self.codes, self.scales, table, kv_len, window, sinks, scale)

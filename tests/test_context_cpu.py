@@ -160,3 +160,32 @@ def test_kv4_empty_batches():
     assert L.capk_kv4_append(1, 1, 4, 2, 64, P, 0, 128, 64, P, 0, 128, 64, P, P, 8, 16, None, 4, 4, P, None, None) == EINVAL
     assert L.capk_kv4_attention(1, 1, 4, 2, 1, 64, 1.0, 0, 0, P, 0, 256, 64, P, P, 8, 64, None, 4, 4, P, P, 0, 256, 64, None, P,
                                 1 << 30, None) == EINVAL
+
+
+def test_derivatives_are_not_dropped():
+    """Forward-mode tangents, and a gradient through attention over the 4-bit cache, are refused in words (ahead of
+    the refusal of a tensor that is not on a GPU)."""
+    import torch.autograd.forward_ad as fw
+
+    from capk import context
+    from capk._lib import CapkError
+    x = torch.ones(1, 2, 2, 64)
+    pos, (freq, axis) = torch.zeros(3, 2, dtype=torch.int32), context.axis_frequencies((8, 12, 12), device="cpu")
+    cache, table = context.KV4Cache.empty(2, 2, 64, 16, device="cpu"), torch.zeros(1, 2, dtype=torch.int32)
+    n = torch.ones(1, dtype=torch.int32)
+    with fw.dual_level():
+        d = fw.make_dual(x, x)
+        for call in (lambda: context.axis_rope(d, x, pos, freq, axis), lambda: context.axis_rope(x, d, pos, freq, axis),
+                     lambda: context.axis_rope(d, None, pos, freq, axis), lambda: context.sliding_attention(d, x, x, window=1),
+                     lambda: context.sliding_attention(x, d, x, window=1), lambda: context.sliding_attention(x, x, d, window=1),
+                     lambda: context.sliding_attention(x, x[:, :0], d[:, :0]), lambda: cache.attend(d, table, n)):
+            with pytest.raises(CapkError, match="forward-mode"):
+                call()
+        with pytest.raises(CapkError, match="GPU|device"):  # (no tangent: the usual refusal)
+            context.axis_rope(x, x, pos, freq, axis)
+    g = x.clone().requires_grad_()
+    with pytest.raises(CapkError, match="no gradient"):
+        cache.attend(g, table, n)
+    for q in (g.detach(), g):
+        with torch.no_grad(), pytest.raises(CapkError, match="GPU|device"):
+            cache.attend(q, table, n)

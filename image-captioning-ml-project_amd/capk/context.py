@@ -110,6 +110,20 @@ class _SlidingAttention(torch.autograd.Function):
         return dq, dk, dv, None, None, None, None, None
 
 
+class _NoAttention(torch.autograd.Function):
+    """No queries or no keys: zeros, and zeros as the gradients of all three operands."""
+
+    @staticmethod
+    def forward(ctx, q, k, v):
+        ctx.shapes = (q.shape, k.shape, v.shape)
+        return q.new_zeros(q.shape)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do):
+        return tuple(do.new_zeros(s) if need else None for s, need in zip(ctx.shapes, ctx.needs_input_grad))
+
+
 def sliding_attention(q, k, v, *, window=0, sinks=0, scale=None, key_pad=None, kv_len=None):
     """o [B, Nq, H, hd]: the queries are the last Nq positions of kv_len[b] (default Nk) keys; position p sees
     j <= p with j < sinks or p - j < window (0: no window), less key_pad[b, j].  k / v [B, Nk, Hk, hd] with
@@ -117,9 +131,10 @@ def sliding_attention(q, k, v, *, window=0, sinks=0, scale=None, key_pad=None, k
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     track = _differentiable("sliding_attention", q, k, v)
     if q.dim() == 4 and k.dim() == 4 and not (q.numel() and k.numel()):  # nothing to attend, or to
-        if q.dtype != k.dtype or q.dtype != v.dtype or k.shape != v.shape or q.shape[0] != k.shape[0]:
-            raise ValueError(f"sliding_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
-        return q.masked_fill(torch.ones_like(q, dtype=torch.bool), 0)  # (zeros, of q's graph)
+        ops._sliding_args("sliding_attention", q, k, v, window, sinks, key_pad, kv_len)
+        if window < 0 or sinks < 0:
+            raise ValueError(f"sliding_attention: window {window} and sinks {sinks} must not be negative")
+        return _NoAttention.apply(q, k, v) if track else q.new_zeros(q.shape)
     if track:
         return _SlidingAttention.apply(q, k, v, window, sinks, scale, key_pad, kv_len)
     return ops.sliding_attention_fwd(_rows(q), _rows(k), _rows(v), window, sinks, scale, key_pad, kv_len,

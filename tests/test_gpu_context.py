@@ -889,3 +889,28 @@ def test_kv4_empty_batches(dtype):
     x, table, zero = _rand(1, 0, 2, 64, dtype=dt), torch.zeros(1, 2, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
     cache.append(x, x, table, zero)
     assert cache.read(table, zero, 0, dt)[0].shape == (1, 0, 2, 64) and torch.equal(cache.codes, before)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("B,Nq,Nk", [(2, 3, 0), (2, 0, 5), (0, 3, 5), (2, 0, 0)])
+def test_sliding_attention_of_nothing(dtype, B, Nq, Nk):
+    """No queries, keys or sequences: zeros, gradients of zeros for each operand that asks for one, and the refusals of
+    any other call."""
+    from capk import context
+    from capk._lib import CapkError
+    dt = DT[dtype]
+    q0, k0, v0 = (_rand(B, n, h, 64, seed=281, dtype=dt) for n, h in ((Nq, 4), (Nk, 2), (Nk, 2)))
+    assert not context.sliding_attention(q0, k0, v0, window=3).any()
+    for need in ((True, True, True), (False, True, True), (True, False, False), (False, False, True)):
+        x = [t.detach().clone().requires_grad_(r) for t, r in zip((q0, k0, v0), need)]
+        o = context.sliding_attention(*x, window=3, sinks=1)
+        assert o.shape == q0.shape and o.dtype == dt and not o.any()
+        o.sum().backward()
+        for t, r in zip(x, need):
+            assert (t.grad is not None and t.grad.shape == t.shape and not t.grad.any()) if r else t.grad is None
+    for call in (lambda: context.sliding_attention(q0.half(), k0.half(), v0.half()), lambda: context.sliding_attention(q0[:, :, :3], k0, v0),
+                 lambda: context.sliding_attention(q0, k0[..., :32], v0[..., :32]), lambda: context.sliding_attention(q0, k0, v0, window=-1),
+                 lambda: context.sliding_attention(q0, k0, v0, sinks=-1), lambda: context.sliding_attention(q0.cpu(), k0.cpu(), v0.cpu()),
+                 lambda: context.sliding_attention(q0, k0, v0, key_pad=torch.zeros(B, Nk + 1, dtype=torch.bool, device="cuda"))):
+        with pytest.raises((CapkError, ValueError)):
+            call()

@@ -914,3 +914,161 @@ def test_sliding_attention_of_nothing(dtype, B, Nq, Nk):
                  lambda: context.sliding_attention(q0, k0, v0, key_pad=torch.zeros(B, Nk + 1, dtype=torch.bool, device="cuda"))):
         with pytest.raises((CapkError, ValueError)):
             call()
+
+
+# ------------------------------------------------------------------- 32 bits through three parts ---
+# fp32 products run as six products of bf16 parts, x = h + m + l.  The bounds below are those of 32-bit arithmetic
+# alone (a value of two parts is off by up to 2^-17, 128 F); every test also shows on the CPU that operands of two
+# parts would break its bound.  E counts a product x y: three dropped part products (2^-26 in all, F / 4 at most)
+# and six additions of at most 2 F each, rounded up.
+E = 16 * F
+
+
+def _full(*shape, seed, scale=1.0):
+    """Values in +-[scale, 2 scale) with all 24 bits in use."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randint(1 << 23, 1 << 24, shape, generator=g).float() * 2.0 ** -23
+    return x * scale * (torch.randint(0, 2, shape, generator=g) * 2 - 1)
+
+
+def _two_parts(x):
+    h = x.bfloat16().float()
+    return h.double() + (x - h).bfloat16().double()
+
+
+def _tight(got, ref, tol, planted=None, what=""):
+    """`got` within `tol` of `ref`, and the value of two-part operands not."""
+    if planted is not None:
+        assert float(((planted - ref).abs() - 1.5 * tol).max()) > 0, f"{what}: the bound would not see two parts"
+    _close(got.cpu(), ref, tol, what)
+
+
+def _columns(hd, at, x):
+    """[..., hd] with x in one column and zeros beside it."""
+    y = torch.zeros(*x.shape, hd)
+    y[..., at] = x
+    return y
+
+
+FP32_FORMS = [(1, 12, 2, 64), (1, 300, 2, 32), (1, 300, 2, 64), (1, 300, 1, 80), (1, 300, 2, 128), (32, 300, 4, 32), (32, 300, 4, 64),
+              (32, 300, 4, 96), (32, 300, 4, 128)]  # few queries; small grids (two groups, cut queries); large grids
+
+
+@pytest.mark.parametrize("B,N,H,hd", FP32_FORMS)
+def test_fp32_scores_keep_32_bits(B, N, H, hd):
+    """One visible key: lse = scale q k.  Off by a product (E), the rounded factor, product with it, ln 2 and result
+    (6 F), and log2 (2^-20)."""
+    from capk import ops
+    q, k = _full(B, N, H, seed=1, scale=16.0), _full(B, N, H, seed=2, scale=8.0)
+    v = torch.zeros(B, N, H, hd).cuda()
+    lse = ops.sliding_attention_fwd(_columns(hd, 3, q).cuda(), _columns(hd, 3, k).cuda(), v, 1, 0, 0.75)[1]
+    ref = 0.75 * q.double() * k.double()
+    planted = 0.75 * _two_parts(q) * _two_parts(k)
+    t = lambda x: x.permute(0, 2, 1)  # noqa: E731
+    _tight(lse, t(ref), t((E + 6 * F) * ref.abs() + 2.0 ** -20), t(planted), "lse")
+
+
+@pytest.mark.parametrize("B,N,H,hd", FP32_FORMS)
+def test_fp32_values_and_gradients_keep_32_bits(B, N, H, hd):
+    """Scores of zero and one visible key: P = 1, o = v and dv = do, off by the sums of their three parts (4 F)."""
+    from capk import context
+    q = torch.zeros(B, N, H, hd).cuda().requires_grad_()
+    k, v = (_full(B, N, H, hd, seed=s).cuda().requires_grad_() for s in (3, 4))
+    do = _full(B, N, H, hd, seed=5)
+    o = context.sliding_attention(q, k, v, window=1)
+    dv, = torch.autograd.grad(o, v, do.cuda())
+    for got, x, name in ((o, v.detach().cpu(), "o"), (dv, do, "dv")):
+        _tight(got.detach(), x.double(), 4 * F * x.double().abs(), _two_parts(x) if N > 16 or name == "dv" else None, name)
+
+
+@pytest.mark.parametrize("B,N,H,hd", FP32_FORMS)
+def test_fp32_probabilities_keep_32_bits(B, N, H, hd):
+    """Two visible keys, scores in [-1/2, 1/2): P = exp2(c s - m).  Exponents are off by at most 4 F (the factor, its
+    product, the maximum's, their difference), so a P by 3 F and exp2's 2 F, relative.  o with v = 1 at every other
+    key is one P over the sum of two: 10 F, the sum of its parts 4 F, of the row F, quotient and product 2 F.  dv with
+    do = 1 at every other row is one P recomputed from lse, each rounding at most 2 F where values reach 1.8: c s and its
+    difference from lse 4 F; in lse the row's sum, off by 6 F, or 9 F of its log2, log2 itself 2 F, the maximum and
+    three roundings 5 F; back to base 2 3 F; 23 F in all, times ln 2 16 F, exp2 2 F, parts 4 F."""
+    from capk import context
+    k = _full(B, N, H, seed=6, scale=0.25)
+    even = (torch.arange(N) % 2 == 0).float()
+    q = _columns(hd, 1, torch.ones(B, N, H)).cuda()
+    v = even.view(1, N, 1, 1).expand(B, N, H, hd).contiguous().cuda().requires_grad_()
+    o = context.sliding_attention(q, _columns(hd, 1, k).cuda(), v, window=2, scale=1.0)
+    do = even.view(1, N, 1, 1).expand(B, N, H, hd).contiguous().cuda()
+    dv, = torch.autograd.grad(o, v, do)
+    s = k.double()
+    prev = torch.cat([torch.full_like(s[:, :1], -math.inf), s[:, :-1]], 1)
+    top = torch.maximum(s, prev)
+    p1, p0 = (s - top).exp(), (prev - top).exp()  # own key, the one before
+    z = p1 + p0
+    e = even.view(1, N, 1).double()
+    ref = (p1 * e + p0 * (1 - e)) / z
+    ref[:, 0] = 1
+    planted = (_two_parts(p1.float()) * e + _two_parts(p0.float()) * (1 - e)) / z
+    planted[:, 0] = 1
+    wide = lambda x: x.unsqueeze(-1).expand(B, N, H, hd)  # noqa: E731
+    _tight(o.detach(), wide(ref), wide(17 * F * ref), wide(planted) if N > 16 else None, "o")
+    own, before = p1 / z, torch.cat([(p0 / z)[:, 1:], torch.zeros_like(s[:, :1])], 1)  # P of key j in rows j and j + 1
+    rows = torch.cat([even[1:], torch.zeros(1)]).view(1, N, 1).double()
+    ref = own * e + before * rows
+    planted = _two_parts(own.float()) * e + _two_parts(before.float()) * rows
+    _tight(dv, wide(ref), wide(24 * F * ref), wide(planted), "dv")
+
+
+@pytest.mark.parametrize("B,N,H,hd", FP32_FORMS)
+def test_fp32_score_gradients_keep_32_bits(B, N, H, hd):
+    """Two visible keys of score zero (q and k in different columns), P = 1/2; v, q and k are zero at every odd token,
+    so a row has one do v = x, dS = +-x / 4, and dq, dk have one term each, scale dS k and scale dS q.  Off by: x (E), P
+    (exponent 3 F, times ln 2 2 F, exp2 2 F), D = P x (6 F), x - D = x / 2 (7 F), P again and the product (5 F), the
+    last product (E) and the scale (F): 2 E + 13 F."""
+    from capk import context
+    even = (torch.arange(N) % 2 == 0).float().view(1, N, 1)
+    qx, kx, vx = (_full(B, N, H, seed=7 + i) * even for i in range(3))
+    dx = _full(B, N, H, seed=10)
+    dx[:, 0] = 0
+    q, k, v = (_columns(hd, c, x).cuda().requires_grad_() for c, x in ((1, qx), (2, kx), (5, vx)))
+    do = _columns(hd, 5, dx).cuda()
+    scale = 0.75
+    dq, dk, _ = torch.autograd.grad(context.sliding_attention(q, k, v, window=2, scale=scale), (q, k, v), do)
+
+    def grads(q, k, v, d, cut):
+        shift = lambda x: torch.cat([torch.zeros_like(x[:, :1]), x[:, :-1]], 1)  # noqa: E731
+        own, prev = d * v, d * shift(v)                      # do v^T of a row's two keys, one of them zero
+        ds1, ds0 = cut((own - prev) / 4), cut((prev - own) / 4)
+        dk0 = torch.cat([(ds0 * q)[:, 1:], torch.zeros_like(q[:, :1])], 1)  # of the row behind, at key j
+        return scale * (ds1 * k + ds0 * shift(k)), scale * (ds1 * q + dk0)
+
+    ref = grads(*(x.double() for x in (qx, kx, vx, dx)), lambda x: x)
+    planted = grads(*(_two_parts(x) for x in (qx, kx, vx, dx)), lambda x: _two_parts(x.float()))
+    for got, r, p, c, name in ((dq, ref[0], planted[0], 2, "dq"), (dk, ref[1], planted[1], 1, "dk")):
+        _tight(got[..., c], r, (2 * E + 13 * F) * r.abs(), p if B * N * H > 100 else None, name)  # (of 12 dk all may lie within)
+
+
+def test_fp32_queries_over_the_4_bit_cache_keep_32_bits():
+    """One visible key: lse = scale q k (three part products, 6 F of sums, and 6 F as above); two, with v = 1 and 0:
+    o = P_0 / (P_0 + P_1) as above with 3 F more for each score."""
+    from capk import context, ops
+    B, H, hd = 300, 4, 64
+    cache, table = context.KV4Cache.empty(B, 2, hd, 16), torch.arange(B, dtype=torch.int32).view(B, 1).cuda()
+    lev = torch.tensor([0.5, 1, 1.5, 2, 3, 4, 6])
+    kx = lev[torch.randint(0, 7, (B, 2, 2), generator=torch.Generator().manual_seed(11))] * 0.125
+    vx = torch.tensor([1.0, 0.0]).view(1, 2, 1, 1).expand(B, 2, 2, hd)
+    cache.append(_columns(hd, 9, kx).cuda(), vx.contiguous().cuda(), table, torch.zeros(B, dtype=torch.int32, device="cuda"))
+    kx = kx.repeat_interleave(2, 2)  # [B, 2 keys, H]
+    for n, size in ((1, 64.0), (2, 2.0 ** -2)):
+        q = _full(B, 1, H, seed=12, scale=size)
+        lse = torch.empty(B, H, 1, device="cuda")
+        o = ops.kv4_attention(_columns(hd, 9, q).cuda(), cache.codes, cache.scales, table, torch.full((B,), n, device="cuda"), 0, 0,
+                              1.0, lse=lse)
+        s, cut = (x * kx.double() for x in (q.double(), _two_parts(q)))  # [B, 2, H]
+        if n == 1:
+            _tight(lse[..., 0], s[:, 0], 12 * F * s[:, 0].abs() + 2.0 ** -20, cut[:, 0], "lse")
+        else:
+            p = torch.softmax(s, 1)
+            e = (s - s.amax(1, keepdim=True)).exp()
+            planted = (_two_parts(e.float()) / e.sum(1, keepdim=True))[:, 0]
+            # (exponents up to 0.75 log2 e: 2 F and 3 F of the score each; both weighted by the other's share)
+            tol = (4 + 2 * 8) * F * p[:, 0] * p[:, 1] + 7 * F * p[:, 0]
+            wide = lambda x: x.unsqueeze(-1).expand(B, H, hd)  # noqa: E731
+            _tight(o[:, 0], wide(p[:, 0]), wide(tol), wide(planted), "o")

@@ -1072,3 +1072,86 @@ def test_fp32_queries_over_the_4_bit_cache_keep_32_bits():
             tol = (4 + 2 * 8) * F * p[:, 0] * p[:, 1] + 7 * F * p[:, 0]
             wide = lambda x: x.unsqueeze(-1).expand(B, H, hd)  # noqa: E731
             _tight(o[:, 0], wide(p[:, 0]), wide(tol), wide(planted), "o")
+
+
+# ------------------------------------------------------------------- what a call may not touch, outputs ---
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("hd,page", [(32, 16), (64, 48), (96, 16), (128, 32)])
+def test_kv4_append_leaves_all_other_codes_and_scales(dtype, hd, page):
+    """Pages of random bytes: only the written slots change, of codes and of scales, whatever a block holds (zeros, NaN
+    and infinities too)."""
+    from capk import context
+    B, n, Hk, cols = 3, 21, 3, 4
+    g = torch.Generator(device="cuda").manual_seed(301)
+    pages = B * cols + 3
+    codes, scales = (torch.randint(0, 256, (pages, 2, Hk, page, hd // d), generator=g, device="cuda", dtype=torch.uint8) for d in (2, 32))
+    cache, table = context.KV4Cache(codes.clone(), scales.clone()), _table(B, cols, pages, seed=4)
+    table[1, 1] = -1
+    k, v = (_rand(B, n, Hk, hd, seed=302 + i, dtype=DT[dtype]) for i in (0, 1))
+    k[0, 2], v[0, 3, 0], k[2, 5, 1, 7], v[2, 6, 2, 0] = 0, 0, math.nan, math.inf
+    start = torch.tensor([0, page - 5, 2 * page + 1], dtype=torch.int32, device="cuda")
+    count = torch.tensor([n, n, n - 4], dtype=torch.int32, device="cuda")
+    cache.append(k, v, table, start, count)
+    written = torch.zeros(pages, page, dtype=torch.bool, device="cuda")
+    for b in range(B):
+        for t in range(int(start[b]), int(start[b]) + int(count[b])):
+            pg = int(table[b, t // page])
+            if pg >= 0:
+                written[pg, t % page] = True
+    for now, before in ((cache.codes, codes), (cache.scales, scales)):
+        beside = ~written.view(pages, 1, 1, page, 1).expand_as(now)
+        assert torch.equal(now[beside], before[beside])
+    # the written slots hold what the same append into cleared pages holds
+    clean = context.KV4Cache.empty(pages, Hk, hd, page)
+    clean.append(k, v, table, start, count)
+    for now, other in ((cache.codes, clean.codes), (cache.scales, clean.scales)):
+        at = written.view(pages, 1, 1, page, 1).expand_as(now)
+        assert torch.equal(now[at], other[at])
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("B,Nq,H,Hk,hd,cols,kv_len", [
+    (70, 3, 8, 8, 64, 4, (0, 1, 2, 3, 50) + tuple(range(5, 64)) + (0, 64, 64, 63, 33, 32)),  # a workgroup for each: not split
+    (3, 2, 8, 2, 128, 60, (0, 960, 500))])                                                    # split and joined
+def test_kv4_attention_lse(dtype, B, Nq, H, Hk, hd, cols, kv_len):
+    """lse of the 4-bit cache, -inf where a query sees nothing."""
+    from capk import _lib, context, ops
+    dt, page = DT[dtype], 16
+    cache, table = context.KV4Cache.empty(B * cols + 1, Hk, hd, page), _table(B, cols, B * cols + 1, seed=5)
+    k, v = (_rand(B, cols * page, Hk, hd, seed=311 + i) for i in (0, 1))
+    zero = torch.zeros(B, dtype=torch.int32, device="cuda")
+    cache.append(k, v, table, zero)
+    k, v = cache.read(table, zero, cols * page, torch.float32)
+    kv_len = torch.tensor(kv_len, dtype=torch.int32, device="cuda")
+    q, lse = _rand(B, Nq, H, hd, seed=313, dtype=dt), torch.full((B, H, Nq), 7.0, device="cuda")
+    split = _lib.load().capk_kv4_attention_workspace(1, B, H, Hk, Nq, hd, 0, 0, page, cols) > 0
+    assert split == (B == 3)
+    o = ops.kv4_attention(q, cache.codes, cache.scales, table, kv_len, 0, 0, hd ** -0.5, lse=lse)
+    ref = _attention_ref(q, k, v, _see(B, Nq, cols * page, 0, 0, None, kv_len), u=U[dt])
+    _close(o, *ref["o"], "o")
+    none = torch.isinf(ref["lse"][0])
+    assert bool(none[0].all()) and torch.equal(none, lse == -math.inf)
+    _close(lse.masked_fill(none, 0), ref["lse"][0].masked_fill(none, 0), ref["lse"][1].nan_to_num(0, 0).masked_fill(none, 0), "lse")
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("Nq,Nk", [(1, 2000), (5, 40), (150, 150)])
+def test_sliding_attention_into_a_strided_output(dtype, Nq, Nk):
+    """out= inside a larger buffer, heads outside tokens: the result's bits, and nothing beside them; with and without
+    lse, and refusals of another shape, type or alignment."""
+    from capk import ops
+    from capk._lib import CapkError
+    B, H, hd, dt = 2, 4, 64, DT[dtype]
+    q, k, v = (_rand(B, n, H, hd, seed=321 + i, dtype=dt) for i, n in enumerate((Nq, Nk, Nk)))
+    rule = (30, 2, hd ** -0.5)
+    ref, lse = ops.sliding_attention_fwd(q, k, v, *rule)
+    big = torch.full((B, H, Nq + 3, hd + 8), 3.0, dtype=dt, device="cuda")
+    out = big[:, :, 1:Nq + 1, :hd].transpose(1, 2)
+    for want in (True, False):
+        out.zero_()
+        got, got_lse = ops.sliding_attention_fwd(q, k, v, *rule, out=out, want_lse=want)
+        assert got is out and torch.equal(out, ref) and (torch.equal(got_lse, lse) if want else got_lse is None)
+        assert (big[:, :, 0] == 3).all() and (big[:, :, Nq + 1:] == 3).all() and (big[..., hd:] == 3).all()
+    for bad in (ref[:, :, :2], ref.double(), ref.cpu(), torch.zeros(B, Nq, H, hd + 1, dtype=dt, device="cuda")[..., 1:]):
+        with pytest.raises((CapkError, ValueError)):
+            ops.sliding_attention_fwd(q, k, v, *rule, out=bad)

@@ -62,7 +62,8 @@ struct StepArgs {
   float *po, *pml;
   int splits;
 };
-// bytes of partial results (0: the keys are not split) and the launch
+// workgroups without a split of the keys, bytes of partial results (0: the keys are not split), and the launch
+int64_t step_blocks(int dtype, const StepArgs& a);
 size_t step_workspace(int dtype, const StepArgs& a, int* splits);
 int step_launch(int dtype, StepArgs a, void* ws, size_t ws_bytes, hipStream_t st);
 

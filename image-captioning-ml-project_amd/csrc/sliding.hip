@@ -710,8 +710,6 @@ static void slide_cut(SlideArgs& a) {
 
 using namespace capk;
 
-// Few queries (a decoding step, drafted tokens): the kernel that reads the cache once for all of them
-static bool slide_few(int Nq) { return Nq <= 16; }
 static StepArgs slide_step(const SlideArgs& a) {
   StepArgs s{};
   s.B = a.B; s.H = a.H; s.Hk = a.Hk; s.Nq = a.Nq; s.cap = a.Nk; s.hd = a.hd;
@@ -719,12 +717,33 @@ static StepArgs slide_step(const SlideArgs& a) {
   s.q = a.q; s.k = a.k; s.v = a.v; s.o = a.o; s.len = a.len; s.pad = a.pad; s.lse = a.lse;
   return s;
 }
+// Few queries for their keys (a decoding step, drafted tokens, a chunk of a prompt): the kernel that splits the keys
+// over workgroups.  slide_fwd walks a query tile's keys in one chain, whatever else is idle: 10 to 14 ns a key in bf16
+// (heads of 64 to 128), 41 to 99 in fp32, as long as its workgroups find a CU each.  The other takes 0.05 ns (fp32 0.1)
+// times the keys times its workgroups of up to 64 columns (query, head), and about 20 us: even at 210 to 260 of them
+// (fp32 430 to 900) on long caches.  The rule stays below that, and lower on shorter caches.  Measured, us, slide_fwd /
+// this: bf16, 16 / 4 heads of 128, 131072 keys 1905 / 114 (17 queries), 1907 / 253 (64), 1912 / 917 (256); 8192 keys 122 /
+// 26, 123 / 35, 126 / 81; eight sequences of 8192 126 / 65, 128 / 137, 153 / 476; 2048 keys 35 / 15, 36 / 26, 37 / 37; 12
+// heads of 64, 8192 keys 90 / 17, 91 / 30, 92 / 53; 512 keys 12 to 16 / 15 to 26.  fp32, 16 / 4 heads of 128, 512 keys
+// 57 / 17, 57 / 19, 59 / 41; 32768 3240 / 107, 3243 / 257, 3260 / 916.  At most 512 queries (four tiles): beyond, a whole
+// pass is meant, where later queries see more keys than earlier ones and slide_fwd does not compute the difference.
+// Up to 16 queries are the step's own case, on short caches too (512 keys: 14.8 / 15.1).
+static bool slide_few(int dtype, const SlideArgs& a) {
+  if (a.Nq <= 16) return true;
+  if (a.Nq > 512) return false;
+  // keys that a tile of 128 queries sees, and those that all queries together see
+  const int64_t w = (int64_t)a.window + a.sinks, keys = w + 128 < a.Nk ? w + 128 : a.Nk, span = w + a.Nq < a.Nk ? w + a.Nq : a.Nk;
+  const int64_t blocks = step_blocks(dtype, slide_step(a));
+  if (dtype == CAPK_BF16) return keys >= 2048 && blocks * 64 <= keys && blocks * span <= 128 * keys;
+  return keys >= 512 && blocks * 2 <= keys && blocks * span <= 384 * keys;
+}
 
 extern "C" size_t capk_sliding_attention_fwd_workspace(int dtype, int B, int H, int Hk, int Nq, int Nk, int hd,
                                                        int window, int sinks) {
-  if (!slide_sizes(B, H, Hk, Nq, Nk, hd, window, sinks) || !slide_few(Nq)) return 0;
+  if (!slide_sizes(B, H, Hk, Nq, Nk, hd, window, sinks)) return 0;
+  const SlideArgs a = slide_args(B, H, Hk, Nq, Nk, hd, 0.f, window, sinks, nullptr, nullptr);
   int splits;
-  return step_workspace(dtype, slide_step(slide_args(B, H, Hk, Nq, Nk, hd, 0.f, window, sinks, nullptr, nullptr)), &splits);
+  return slide_few(dtype, a) ? step_workspace(dtype, slide_step(a), &splits) : 0;
 }
 
 extern "C" int capk_sliding_attention_fwd(int dtype, int B, int H, int Hk, int Nq, int Nk, int hd, float scale,
@@ -740,7 +759,7 @@ extern "C" int capk_sliding_attention_fwd(int dtype, int B, int H, int Hk, int N
   if (rc) return rc;
   SlideArgs a = slide_args(B, H, Hk, Nq, Nk, hd, scale, window, sinks, key_pad, kv_len);
   a.q = vs[0]; a.k = vs[1]; a.v = vs[2]; a.o = vs[3]; a.lse = lse;
-  if (slide_few(Nq)) return step_launch(dtype, slide_step(a), ws, ws_bytes, S(stream));
+  if (slide_few(dtype, a)) return step_launch(dtype, slide_step(a), ws, ws_bytes, S(stream));
   const int hdp = slide_hdp(hd);
   const dim3 grid(cdiv(Nq, 128) * H * B);
   // up to one workgroup per CU: a second group of waves shares its tiles (117 to 82 us at 256 workgroups of

@@ -377,9 +377,13 @@ static int step_nrt(int dtype, bool kv4, int hd, int rows) {
   return rows <= 16 || most == 1 ? 1 : rows <= 32 || most == 2 ? 2 : 4;
 }
 
+int64_t step_blocks(int dtype, const StepArgs& a) {
+  const int rows = a.Nq * (a.H / a.Hk);  // (entries: 512 queries of 65535 heads, 64 of 2^20)
+  return (int64_t)a.B * a.Hk * cdiv(rows, 16 * step_nrt(dtype, a.page != 0, a.hd, rows));
+}
+
 size_t step_workspace(int dtype, const StepArgs& a, int* splits) {
-  const int rows = a.Nq * (a.H / a.Hk), nrt = step_nrt(dtype, a.page != 0, a.hd, rows);
-  const int64_t blocks = (int64_t)a.B * a.Hk * cdiv(rows, 16 * nrt);
+  const int64_t blocks = step_blocks(dtype, a);
   // two workgroups (what registers hold) on every CU, with at least a tile of 32 keys for each wave of a
   // split.  131072 keys, 8 key heads of 128, 20 columns: 32 + 6 us (join) at 512 workgroups, 37 + 8 at 768,
   // 39 + 10 at 1024

@@ -686,8 +686,8 @@ int capk_axis_rope(int dtype, int B, int N, int hd, int pairs, int interleaved, 
  *   lse (fp32 [B, H, Nq], optional forward) its log denominator; a query that sees nothing has
  *   o = 0, lse = -inf (rows before position 0 may hold anything, in q and in the backward's dout).
  *   Keys hidden from every query of a call are never used: NaN there is harmless; a value that is
- *   not finite may reach any query of its sequence and head.  Nq <= 16 runs the decoding-step kernel
- *   (split over the keys, partial results in ws).  Backward: dq, dk, dv (all of them written),
+ *   not finite may reach any query of its sequence and head.  Nq <= 16, and up to 512 queries over
+ *   many more keys, run the decoding-step kernel (split over the keys, partial results in ws).  Backward: dq, dk, dv (all of them written),
  *   deterministic.  hd % 8 == 0, hd <= 128; scale positive and finite; lengths up to 2^28, B <=
  *   65535; tokens less than 2^22 elements apart (0 <= rs); no dropout. */
 size_t capk_sliding_attention_fwd_workspace(int dtype, int B, int H, int Hk, int Nq, int Nk, int hd, int window,

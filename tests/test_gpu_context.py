@@ -1155,3 +1155,20 @@ def test_sliding_attention_into_a_strided_output(dtype, Nq, Nk):
     for bad in (ref[:, :, :2], ref.double(), ref.cpu(), torch.zeros(B, Nq, H, hd + 1, dtype=dt, device="cuda")[..., 1:]):
         with pytest.raises((CapkError, ValueError)):
             ops.sliding_attention_fwd(q, k, v, *rule, out=bad)
+
+
+# ------------------------------------------------------------------- a chunk of queries over a long cache ---
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("B,Nq,Nk,H,Hk,hd,window,sinks,pad,kv_len,split", [
+    (1, 16, 4100, 4, 2, 64, 0, 0, None, None, True), (1, 17, 4100, 4, 2, 64, 0, 0, None, None, True),
+    (1, 17, 300, 4, 2, 64, 0, 0, None, None, False), (1, 64, 2500, 8, 1, 128, 0, 0, None, (2311,), True),
+    (1, 129, 3000, 3, 1, 80, 2000, 5, (2900,), None, True), (2, 100, 3001, 2, 2, 32, 2200, 300, None, (3001, 60), True),
+    (2, 100, 3001, 2, 1, 96, 0, 0, (3000, 5), (2999, 3001), True), (1, 512, 2100, 2, 1, 64, 0, 0, None, None, True),
+    (1, 513, 2100, 2, 1, 64, 0, 0, None, None, False), (1, 40, 4000, 4, 2, 64, 100, 3, None, None, False),
+    (70, 20, 2100, 6, 6, 32, 0, 0, None, tuple(range(0, 2100, 30)), False)])
+def test_sliding_attention_chunks_over_a_long_cache(dtype, B, Nq, Nk, H, Hk, hd, window, sinks, pad, kv_len, split):
+    """Both sides of the rule that sends a chunk of queries to the kernel that splits the keys."""
+    from capk import _lib
+    ws = _lib.load().capk_sliding_attention_fwd_workspace(dtype == "bf16", B, H, Hk, Nq, Nk, hd, window, sinks)
+    assert (ws > 0) == split, ws
+    _slide_case(dtype, B, Nq, Nk, H, Hk, hd, window, sinks, pad, kv_len, grad=Nq <= 129 and B < 70, seed=331)

@@ -10,19 +10,25 @@
 // query on each lane, so the row statistics need one swap, and P^T, already in B-operand order, is
 // multiplied by V^T fragments read transposed from LDS.  A tile's 16 + 16 products of 32 cycles (hd 128)
 // stand beside about 1100 cycles of softmax and 1000 of LDS reads (each wave reads the whole tile for its 32
-// queries), so no unit is saturated: 187 us for 16384 tokens, window 1024, 16 heads of 128 (146 GFLOP, 780
-// TF/s of the 1600 that a large product reaches); 64 queries per wave would halve the LDS reads, but its 128
-// sums then travel between the two halves of the register file every tile (700 us).
+// queries), one after another within a wave, so no unit is saturated: 187 us for 16384 tokens, window 1024, 16 heads
+// of 128 (134 GFLOP of visible pairs: 715 TF/s of the 1600 that a large product reaches); 64 queries per wave would
+// halve the LDS reads, but its 128 sums then travel between the two halves of the register file every tile (700 us).
 // Backward: D = rowsum(do * o); P = exp(s - lse); dS = P (do v^T - D) scale.  One kernel owns queries
 // (dQ^T += K^T dS^T), one owns keys and walks their queries over all heads of the group
 // (dV^T += dO^T P, dK^T += Q^T dS): every sum has one owner, so results do not depend on timing.  S and dP are
 // computed in both (seven products for five): one kernel for all would add dQ through atomics.  The same
-// tokens: dQ 233 us (940 TF/s), dK and dV 300 us (970), bound by LDS reads as the forward is.  Keys
-// that stay visible are seen by all later queries: those far queries are cut into chunks with owners
-// of their own, whose 32-bit partial sums one more kernel adds in a fixed order (7 us).
+// tokens: dQ 236 us (three products: 850 TF/s of visible pairs), dK and dV 300 us (four: 890), with matrix, vector and
+// LDS work each about a third of the time, as in the forward.  Keys that stay visible are seen by all later
+// queries: those far queries are cut into chunks with owners of their own, whose 32-bit partial sums one more kernel
+// adds in a fixed order (7 us).
 //
-// fp32: three bf16 parts per value and six part products per product (tiles.h), at 16 times the rate of the fp32
-// matrix instructions.
+// Roundings of the bf16 forms, besides inputs and results: P before P V and P^T dO, dS before its products (each
+// half a bf16 step, 2^-9 to 2^-8 of the value, and independent, so sums of many keys average them), as the matrix
+// unit takes bf16 operands and an fp32 operand costs six products; D comes from the rounded output where a row sees
+// many keys.  Scores, maxima, sums, lse and D are 32-bit.  16384 tokens: relative error 2.4e-3 against 64 bits, 1.7e-3
+// of which are the results' own rounding.
+// fp32: three bf16 parts per value and six part products per product (tiles.h), 2.7 times as fast as the fp32 matrix
+// instructions.  Magnitudes from 3.39e38 on (the largest bf16) have no finite first part and give NaN.
 #include "sliding.h"
 
 namespace capk {
@@ -725,8 +731,8 @@ static StepArgs slide_step(const SlideArgs& a) {
 // this: bf16, 16 / 4 heads of 128, 131072 keys 1905 / 114 (17 queries), 1907 / 253 (64), 1912 / 917 (256); 8192 keys 122 /
 // 26, 123 / 35, 126 / 81; eight sequences of 8192 126 / 65, 128 / 137, 153 / 476; 2048 keys 35 / 15, 36 / 26, 37 / 37; 12
 // heads of 64, 8192 keys 90 / 17, 91 / 30, 92 / 53; 512 keys 12 to 16 / 15 to 26.  fp32, 16 / 4 heads of 128, 512 keys
-// 57 / 17, 57 / 19, 59 / 41; 32768 3240 / 107, 3243 / 257, 3260 / 916.  At most 512 queries (four tiles): beyond, a whole
-// pass is meant, where later queries see more keys than earlier ones and slide_fwd does not compute the difference.
+// 57 / 17, 57 / 19, 59 / 41; 32768 3240 / 107, 3243 / 257, 3260 / 916.  At most 512 queries (four tiles): beyond, a whole pass is meant, where
+// later queries see more keys than earlier ones and slide_fwd does not compute the difference.
 // Up to 16 queries are the step's own case, on short caches too (512 keys: 14.8 / 15.1).
 static bool slide_few(int dtype, const SlideArgs& a) {
   if (a.Nq <= 16) return true;
@@ -763,7 +769,8 @@ extern "C" int capk_sliding_attention_fwd(int dtype, int B, int H, int Hk, int N
   const int hdp = slide_hdp(hd);
   const dim3 grid(cdiv(Nq, 128) * H * B);
   // up to one workgroup per CU: a second group of waves shares its tiles (117 to 82 us at 256 workgroups of
-  // 66 tiles, heads of 128); fp32 images of wider heads leave no room for it
+  // 66 tiles, heads of 128).  fp32: at 128 the second pair of images does not fit in LDS, at 96 (144 of 160 KiB) two
+  // waves per SIMD leave 256 registers and the kernel spills 76
   const bool two = grid.x <= 256;
   SLIDE_HD(hdp, {
     constexpr int L16 = SlidePair<bf16, HDP>::LDS, L32 = SlidePair<float, HDP>::LDS, G32 = HDP <= 64 ? 2 : 1;

@@ -9,10 +9,11 @@
 // nothing is lost before the products; 32-bit queries and probabilities go through the bf16 matrix unit
 // as three bf16 parts (3 x 8 significant bits: exact).  Bound: HBM, the visible keys' bytes once; with 4 bits
 // the conversions (64 per tile and wave) and the softmax take as long as the loads.  The key axis is cut
-// over workgroups (and over the 4 waves of each), whose partial softmaxes are joined.
-// Heads of 128, 8 key heads of 4 bits: 46 us for 64 sequences of 2048 to 4096 tokens (214 MB, 4.6 TB/s), 32 + 6
-// (join) for 5 queries over 131072 tokens (143 MB); dense bf16, 32 windows of 2048, 4 key heads: 31 + 4 us for
-// 134 MB.
+// over workgroups (and over the 4 waves of each), whose partial softmaxes are joined.  bf16 probabilities are rounded
+// (half a bf16 step each) before P V, where the matrix unit takes bf16 operands; sums are 32-bit.
+// Heads of 128, 8 key heads of 4 bits: 46 us for 64 sequences of 2048 to 4096 tokens (215 MB, 4.7 TB/s), 36 + 6
+// (join) for 5 queries over 131072 tokens (143 MB); dense bf16, 32 windows of 2048, 4 key heads: 32 + 4 us for
+// 134 MB.  fp32: 57 us, 67 + 6 over 65536 to 131072 tokens, dense 64 + 4 for 269 MB.
 #include "sliding.h"
 
 namespace capk {
@@ -385,7 +386,7 @@ int64_t step_blocks(int dtype, const StepArgs& a) {
 size_t step_workspace(int dtype, const StepArgs& a, int* splits) {
   const int64_t blocks = step_blocks(dtype, a);
   // two workgroups (what registers hold) on every CU, with at least a tile of 32 keys for each wave of a
-  // split.  131072 keys, 8 key heads of 128, 20 columns: 32 + 6 us (join) at 512 workgroups, 37 + 8 at 768,
+  // split.  65536 to 131072 keys, 8 key heads of 128, 20 columns: 32 + 6 us (join) at 512 workgroups, 37 + 8 at 768,
   // 39 + 10 at 1024
   int64_t most = (int64_t)a.window + a.Nq + a.sinks + 64;
   if (most > a.cap) most = a.cap;

@@ -10,7 +10,8 @@
 // from in chunks; the draw within its chunk.  (Drawing in the last workgroup of the second launch was
 // slower, 27 for 10 us alone and 80 for 22 us at 64 sequences: its fences write the L2 back.)
 // Bound: a 64-bit exp per logit, about 26 vector instructions, of which the first launch runs nine tenths of
-// the time (25 us over 8 of 64 x 15 rows of 50257 bf16 logits in the mean, 2 TB/s; the second 13, the third 8).
+// the time (25 us over 8 of 64 x 15 rows of 50257 bf16 logits in the mean, 2 TB/s; the second 13, the third 8; fp32 the
+// same; without draft logits 15, 10 and 7).
 #include "common.h"
 
 namespace capk {

@@ -684,7 +684,9 @@ int capk_axis_rope(int dtype, int B, int N, int hd, int pairs, int interleaved, 
  *   j < sinks or p - j < window (window 0: every j <= p), less those with key_pad[b*Nk + j] != 0.
  *   H query heads share Hk key heads (head h reads h / (H / Hk)).  o = softmax(scale q k^T) v,
  *   lse (fp32 [B, H, Nq], optional forward) its log denominator; a query that sees nothing has
- *   o = 0, lse = -inf (rows before position 0 may hold anything, in q and in the backward's dout).
+ *   o = 0, lse = -inf (rows before position 0 may hold anything, in q and in the backward's dout; a
+ *   row that padding hides every key from needs finite values in the backward).  fp32 values below
+ *   3.38e38 in magnitude.
  *   Keys hidden from every query of a call are never used: NaN there is harmless; a value that is
  *   not finite may reach any query of its sequence and head.  Nq <= 16, and up to 512 queries over
  *   many more keys, run the decoding-step kernel (split over the keys, partial results in ws).  Backward: dq, dk, dv (all of them written),

@@ -731,7 +731,8 @@ static StepArgs slide_step(const SlideArgs& a) {
 // this: bf16, 16 / 4 heads of 128, 131072 keys 1905 / 114 (17 queries), 1907 / 253 (64), 1912 / 917 (256); 8192 keys 122 /
 // 26, 123 / 35, 126 / 81; eight sequences of 8192 126 / 65, 128 / 137, 153 / 476; 2048 keys 35 / 15, 36 / 26, 37 / 37; 12
 // heads of 64, 8192 keys 90 / 17, 91 / 30, 92 / 53; 512 keys 12 to 16 / 15 to 26.  fp32, 16 / 4 heads of 128, 512 keys
-// 57 / 17, 57 / 19, 59 / 41; 32768 3240 / 107, 3243 / 257, 3260 / 916.  At most 512 queries (four tiles): beyond, a whole pass is meant, where
+// 57 / 17, 57 / 19, 59 / 41; 32768 3240 / 107, 3243 / 257, 3260 / 916; 512 queries
+// of 12 heads of 64 over 512 keys 27 / 33.  At most 512 queries (four tiles): beyond, a whole pass is meant, where
 // later queries see more keys than earlier ones and slide_fwd does not compute the difference.
 // Up to 16 queries are the step's own case, on short caches too (512 keys: 14.8 / 15.1).
 static bool slide_few(int dtype, const SlideArgs& a) {
@@ -741,7 +742,7 @@ static bool slide_few(int dtype, const SlideArgs& a) {
   const int64_t w = (int64_t)a.window + a.sinks, keys = w + 128 < a.Nk ? w + 128 : a.Nk, span = w + a.Nq < a.Nk ? w + a.Nq : a.Nk;
   const int64_t blocks = step_blocks(dtype, slide_step(a));
   if (dtype == CAPK_BF16) return keys >= 2048 && blocks * 64 <= keys && blocks * span <= 128 * keys;
-  return keys >= 512 && blocks * 2 <= keys && blocks * span <= 384 * keys;
+  return keys >= 512 && blocks * 3 <= keys && blocks * span <= 384 * keys;
 }
 
 extern "C" size_t capk_sliding_attention_fwd_workspace(int dtype, int B, int H, int Hk, int Nq, int Nk, int hd,

@@ -1321,6 +1321,11 @@ def _view4(what, t):
     return t.data_ptr(), s[0] if shape[0] > 1 else 0, s[1] if shape[1] > 1 else 0, s[2] if shape[2] > 1 else 0
 
 
+def _reach(n):
+    """A window or a number of sinks for the C entries' 32-bit integers: past 2^30 it reaches past every key."""
+    return max(-1, min(int(n), 1 << 30))
+
+
 def _axis_rope_args(q, k, pos, freq, axis):
     """(sizes, pos, freq, axis) of a rotation of q and k after all checks; the tensors in the kernel's types."""
     _same("axis_rope", q, k)
@@ -1381,7 +1386,7 @@ def _sliding_args(what, q, k, v, window, sinks, key_pad, kv_len):
         key_pad = _index(f"{what}: key_pad", key_pad, (B, Nk), torch.uint8, dev)
     if kv_len is not None:
         kv_len = _index(f"{what}: kv_len", kv_len, (B,), torch.int32, dev)
-    return dtype_code(q), (B, H, Hk, Nq, Nk, hd), (int(window), int(sinks)), views, key_pad, kv_len
+    return dtype_code(q), (B, H, Hk, Nq, Nk, hd), (_reach(window), _reach(sinks)), views, key_pad, kv_len
 
 
 def _sliding_fwd_run(code, dims, rule, views, key_pad, kv_len, q, scale, out, want_lse):
@@ -1494,10 +1499,10 @@ def kv4_attention(q, codes, scales, table, kv_len, window, sinks, scale, *, lse=
     kv_len = _index(f"{what}: kv_len", kv_len, (B,), torch.int32, q.device)
     if kv_len is None:
         raise ValueError(f"{what}: kv_len is needed")
-    o = q.new_empty(q.shape)
-    wsb = _ws_bytes("capk_kv4_attention_workspace", code, B, H, Hk, Nq, hd, int(window), int(sinks), page, table.shape[1])
+    o, window, sinks = q.new_empty(q.shape), _reach(window), _reach(sinks)
+    wsb = _ws_bytes("capk_kv4_attention_workspace", code, B, H, Hk, Nq, hd, window, sinks, page, table.shape[1])
     ws = _ws(wsb, q.device)
-    _launch(q.device, "capk_kv4_attention", code, B, H, Hk, Nq, hd, float(scale), int(window), int(sinks), *qv,
+    _launch(q.device, "capk_kv4_attention", code, B, H, Hk, Nq, hd, float(scale), window, sinks, *qv,
             codes.data_ptr(), scales.data_ptr(), pages, page, *targs, _p(kv_len), *_view4(what, o), _p(lse), _p(ws), wsb)
     return o
 

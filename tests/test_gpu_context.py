@@ -1172,3 +1172,31 @@ def test_sliding_attention_chunks_over_a_long_cache(dtype, B, Nq, Nk, H, Hk, hd,
     ws = _lib.load().capk_sliding_attention_fwd_workspace(dtype == "bf16", B, H, Hk, Nq, Nk, hd, window, sinks)
     assert (ws > 0) == split, ws
     _slide_case(dtype, B, Nq, Nk, H, Hk, hd, window, sinks, pad, kv_len, grad=Nq <= 129 and B < 70, seed=331)
+
+
+def test_windows_and_sinks_past_32_bits():
+    """A window or a number of sinks of any size means what it says: past all keys, none are hidden."""
+    import sys
+
+    from capk import context
+    from capk._lib import CapkError
+    q, k = _rand(1, 40, 2, 64, seed=341), _rand(1, 40, 2, 64, seed=342)
+    cache, table = context.KV4Cache.empty(4, 2, 64, 16), torch.arange(4, device="cuda").view(1, 4)
+    zero = torch.zeros(1, dtype=torch.int32, device="cuda")
+    cache.append(k, k, table, zero)
+    n = zero + 40
+    for nq in (40, 3):
+        x = q[:, :nq]
+        whole = context.sliding_attention(x, k, k)
+        few = context.sliding_attention(x, k, k, window=5)
+        for big in (1 << 31, (1 << 32) + 5, (1 << 32) - 1, sys.maxsize):
+            assert torch.equal(context.sliding_attention(x, k, k, window=big), whole), big
+            assert torch.equal(context.sliding_attention(x, k, k, window=5, sinks=big), whole), big
+            assert torch.equal(cache.attend(x, table, n, window=big), cache.attend(x, table, n)), big
+            assert torch.equal(cache.attend(x, table, n, window=5, sinks=big), cache.attend(x, table, n)), big
+            for kw in (dict(window=-big), dict(sinks=-big)):
+                with pytest.raises((CapkError, ValueError)):
+                    context.sliding_attention(x, k, k, **kw)
+                with pytest.raises((CapkError, ValueError)):
+                    cache.attend(x, table, n, **kw)
+        assert not torch.equal(few, whole)

@@ -152,9 +152,9 @@ class KV4Cache:
 
     @classmethod
     def empty(cls, pages, heads, head_dim, page=64, device="cuda"):
-        if head_dim % 32 or not 32 <= head_dim <= 128 or page % 16 or page < 16 or pages < 1 or heads < 1:
+        if head_dim % 32 or not 32 <= head_dim <= 128 or page % 16 or not 16 <= page <= 4096 or pages < 1 or heads < 1:
             raise ValueError(f"KV4Cache: {pages} pages of {page} tokens, {heads} heads x {head_dim}: need head_dim "
-                             "32, 64, 96 or 128 and pages of a multiple of 16 tokens")
+                             "32, 64, 96 or 128 and pages of a multiple of 16 tokens, up to 4096")
         return cls(torch.zeros(pages, 2, heads, page, head_dim // 2, dtype=torch.uint8, device=device),
                    torch.full((pages, 2, heads, page, head_dim // 32), 127, dtype=torch.uint8, device=device))
 

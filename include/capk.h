@@ -742,8 +742,8 @@ int capk_kv4_attention(int dtype, int B, int H, int Hk, int Nq, int hd, float sc
  *   max(p_n - q_n, 0) after a refusal (from p_n where that leaves nothing), from p_n after draft_len
  *   acceptances: the first token whose cumulative mass exceeds u times the whole.  tokens[b][0..K]
  *   = the accepted ids, the drawn token, -1.  64-bit sums.  u in [0, 1) fp32 [B][K + 1]; K <= 1024,
- *   B (2K + 1) <= 65535, temperature >= 1e-300.  A logit of -inf or NaN has no mass; a row without
- *   any draws token 0. */
+ *   B (2K + 1) <= 65535, temperature >= 1e-300.  A logit of -inf or NaN has no mass, nor has a row
+ *   with +inf; a row without any draws token 0. */
 size_t capk_verify_drafts_workspace(int B, int K, int V);
 int capk_verify_drafts(int dtype, int B, int K, int V, const void* target, int64_t t_bs, int64_t t_rs,
                        const void* draft, int64_t d_bs, int64_t d_rs, const int64_t* ids, int64_t ids_bs,

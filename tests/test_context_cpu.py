@@ -189,3 +189,11 @@ def test_derivatives_are_not_dropped():
     for q in (g.detach(), g):
         with torch.no_grad(), pytest.raises(CapkError, match="GPU|device"):
             cache.attend(q, table, n)
+
+
+def test_kv4_pages_that_no_call_takes():
+    from capk import context
+    for page in (4112, 8192):
+        with pytest.raises(ValueError):
+            context.KV4Cache.empty(1, 1, 64, page, device="cpu")
+    assert context.KV4Cache.empty(1, 1, 64, 4096, device="cpu").codes.shape == (1, 2, 1, 4096, 32)

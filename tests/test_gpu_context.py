@@ -1200,3 +1200,22 @@ def test_windows_and_sinks_past_32_bits():
                 with pytest.raises((CapkError, ValueError)):
                     cache.attend(x, table, n, **kw)
         assert not torch.equal(few, whole)
+
+
+@pytest.mark.parametrize("V", [50, 9000])
+@pytest.mark.parametrize("dtype", DT)
+def test_verify_drafts_rows_with_an_infinity(dtype, V):
+    """A target row with +inf has no mass: its draft is refused and token 0 drawn.  A draft row with one accepts nothing,
+    and the next token is drawn from the target."""
+    from capk import context
+    B, K, dt = 3, 2, DT[dtype]
+    target, draft = _rand(B, K + 1, V, seed=351, dtype=dt), _rand(B, K, V, seed=352, dtype=dt)
+    ids = target[:, :K].float().argmax(-1)
+    u = torch.full((B, K + 1), 0.5, device="cuda")
+    u[:, :K] = 0
+    ref = context.verify_drafts(target, ids, u, draft)
+    target[0, 0, V - 3], draft[1, 0, 7] = math.inf, math.inf
+    n, tok = context.verify_drafts(target, ids, u, draft)
+    assert n.tolist() == [0, 0, K] and tok[0].tolist() == [0, -1, -1] and torch.equal(tok[2], ref[1][2])
+    c = torch.softmax(target[1, 0].double(), -1).cumsum(-1)
+    assert tok[1].tolist() == [int((c > 0.5 * c[-1]).long().argmax()), -1, -1]

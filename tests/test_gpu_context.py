@@ -1219,3 +1219,37 @@ def test_verify_drafts_rows_with_an_infinity(dtype, V):
     assert n.tolist() == [0, 0, K] and tok[0].tolist() == [0, -1, -1] and torch.equal(tok[2], ref[1][2])
     c = torch.softmax(target[1, 0].double(), -1).cumsum(-1)
     assert tok[1].tolist() == [int((c > 0.5 * c[-1]).long().argmax()), -1, -1]
+
+
+@pytest.mark.parametrize("dtype", DT)
+def test_sliding_attention_chunks_and_what_is_hidden(dtype):
+    """A chunk that splits its keys: NaN behind kv_len, under key_pad, between the sinks and every window, and in the
+    rows before position 0 changes nothing; the replays of a captured call equal the eager ones."""
+    from capk import _lib, ops
+    B, Nq, Nk, H, hd, dt = 2, 100, 6000, 2, 64, DT[dtype]
+    assert _lib.load().capk_sliding_attention_fwd_workspace(dtype == "bf16", B, H, H, Nq, Nk, hd, 2500, 40) > 0
+    q, k, v = (_rand(B, n, H, hd, seed=361 + i, dtype=dt) for i, n in enumerate((Nq, Nk, Nk)))
+    n = torch.tensor([5500, 60], dtype=torch.int32, device="cuda")
+    pad = torch.zeros(B, Nk, dtype=torch.bool, device="cuda")
+    pad[:, 5100:5110] = True
+    args = (2500, 40, hd ** -0.5, pad, n)
+    clean = ops.sliding_attention_fwd(q, k, v, *args)
+    for x in (k, v):
+        for b in range(B):
+            x[b, int(n[b]):] = math.nan
+        x[0, 5100:5110], x[0, 40:5500 - Nq - 2500 + 1] = math.nan, math.inf
+    q[1, :Nq - 60] = math.nan
+    got = ops.sliding_attention_fwd(q, k, v, *args)
+    assert all(torch.equal(a, b) for a, b in zip(got, clean)) and not got[0][1, :Nq - 60].any()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        out = ops.sliding_attention_fwd(q, k, v, *args)
+    for r in range(3):
+        q.copy_(_rand(B, Nq, H, hd, seed=371 + r, dtype=dt))
+        n.copy_(torch.tensor([5000 + r, 200], dtype=torch.int32))
+        k.copy_(_rand(B, Nk, H, hd, seed=381 + r, dtype=dt))
+        v.copy_(_rand(B, Nk, H, hd, seed=391 + r, dtype=dt))
+        graph.replay()
+        got = [t.clone() for t in out]
+        assert all(torch.equal(a, b) for a, b in zip(got, ops.sliding_attention_fwd(q, k, v, *args))), r
